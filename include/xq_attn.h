@@ -353,6 +353,139 @@ xq_status xq_kv_store(const float* src, const int32_t* positions, int32_t n_toke
 size_t xq_kv_record_bytes(int32_t kv_type, int32_t head_dim);
 
 /* ---------------------------------------------------------------------------
+ * A KV cache in pages
+ * ------------------------------------------------------------------------- */
+
+/* The cache of one layer, kept in pages that any sequence may hold and several
+ * may share. k and v are pools [D, page_rows, n_head_kv, n_pages] of one KV type
+ * with free row, head and page strides (nb[1..3]; records contiguous): a plane
+ * [capacity][n_head_kv][record] is the pool with nb = {type size, n_head_kv *
+ * record, record, page_rows * n_head_kv * record}. Row r of sequence b is row
+ * r % page_rows of page table[b * table_cols + r / page_rows]. rows[b] is the number
+ * of rows that sequence b holds. table and rows are device memory, so a captured
+ * graph replays with what they hold then. The rows of the new tokens of a call
+ * (rows[b] + 0, 1, ...) need their pages in the table too (xq_kv_pages_reserve).
+ * A page id outside [0, n_pages), and a row past the table's columns, is a
+ * caller's error that is met without an access outside the pools: rows of such a
+ * page are not stored, moved or seen. */
+typedef struct xq_kv_pages {
+    xq_tensor k, v;
+    const int32_t* table; /* [n_seq][table_cols] */
+    const int32_t* rows;  /* [n_seq] */
+    int32_t n_seq;
+    int32_t table_cols;
+} xq_kv_pages;
+
+/* Which elements of a head turn together: rotary index i (0 <= i < n_rot / 2) takes
+ * elements i and i + n_rot/2, or 2i and 2i + 1. */
+enum xq_rope_mode {
+    XQ_ROPE_HALVES = 0,
+    XQ_ROPE_PAIRS = 1,
+};
+
+typedef struct xq_rope_params {
+    int32_t n_rot;      /* elements of a head that turn (the first ones); the rest pass */
+    int32_t mode;       /* enum xq_rope_mode */
+    float freq_base;    /* angle of index i: position * freq_scale * freq_base^(-2i/n_rot) / freq_factors[i] */
+    float freq_scale;
+    float attn_factor;  /* factor on the turned elements */
+    float eps;          /* of the norm */
+    int32_t q8_variant; /* as in xq_kv_store */
+    int32_t reserved;
+} xq_rope_params;
+
+/* Queries, keys and values of new tokens, from the projections to where attention
+ * reads them, in one pass: each query and key head is RMS-normalised,
+ *   x * weight / sqrt(mean(x^2) + eps),
+ * and turned by its token's position; queries go to q_out, keys and values to the
+ * rows rows[b] + i of their sequence's pages.
+ *   q      F32|BF16 [D, n_q, n_head, n_seq], k, v the same type [D, n_q, n_head_kv, n_seq];
+ *          elements contiguous, other strides free
+ *   positions I32 [n_seq][n_q] (device): the position that token i of sequence b turns by
+ *   n_tok  I32 [n_seq] (device), or NULL: all n_q. Tokens from n_tok[b] on are padding:
+ *          neither read nor written
+ *   q_weight, k_weight F32 [D] (device); NULL: those heads are turned, not normalised
+ *   freq_factors F32 [n_rot / 2] (device), or NULL: ones
+ *   q_out  F32|BF16 of q's shape (what xq_fa_tree and xq_flash_attn_ext take), elements
+ *          contiguous, other strides free; may be q itself
+ *   cache  pools of F32, F16, BF16, E5M2, Q8_0 or Q4_0; D 64, 128 or 256; keys and values
+ *          enter in f32 and are stored as xq_kv_store stores them
+ * Norms are summed in f32; angles are formed in f64 (an f32 angle is off by 4e-3 at
+ * position 100 000). XQ_ROPE_HALVES needs n_rot to be a multiple of 8. */
+int xq_supports_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tensor* v, const xq_rope_params* params,
+                             const xq_tensor* q_out, const xq_kv_pages* cache);
+xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tensor* v, const int32_t* positions,
+                          const int32_t* n_tok, const float* q_weight, const float* k_weight, const float* freq_factors,
+                          const xq_rope_params* params, xq_tensor* q_out, const xq_kv_pages* cache, void* stream);
+
+/* Attention of drafted tokens over the paged cache. The tokens of a sequence form
+ * a tree (or several): token i of sequence b sees the rows [0, rows[b]) and, of the
+ * tokens' own rows rows[b] + j, its own and its ancestors'. One token is a decode step.
+ *   q       F32|BF16 [D, n_q, n_head, n_seq], 1 <= n_q <= 64, D 128 or 256; elements contiguous
+ *   cache   pools of F16, Q8_0, Q4_0 or E5M2, n_head a multiple of n_head_kv, group at most
+ *           32; the tokens' own rows are in it (xq_qk_norm_rope)
+ *   parents I32 [n_seq][n_q] (device): parents[i] < i is the token before token i, -1 none (any
+ *           other value counts as -1); NULL: token i follows token i - 1
+ *   n_tok   I32 [n_seq] (device), or NULL: all n_q. Rows of dst and lse from n_tok[b] on
+ *           are left as they were
+ *   dst     q's type [D, n_head, n_q, n_seq], strides multiples of 16 bytes
+ *   lse     F32 [n_seq][n_q][n_head], natural logarithm of the softmax sum, or NULL
+ *   scale   on the scores; finite
+ * Scores and values are those of the decoded cache, sums in f32. F32 q: operands enter
+ * the matrix cores as f16 hi + lo, about 22 bits. BF16 q: as one f16 (weights, and
+ * q8_0 / q4_0 values d * q, rounded to 11 bits; such a value beyond 65504 is infinite).
+ * A row that a token does not see has no part in its result, whatever it holds; a
+ * non-finite element of a row that it sees makes what it reaches non-finite.
+ * A sink joins by xq_fa_lse_merge, as a part with OUT 0 and LSE the sink. */
+int xq_supports_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst);
+xq_status xq_fa_tree_workspace(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, size_t* bytes);
+xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t* parents, const int32_t* n_tok,
+                     xq_tensor* dst, float* lse, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The pages themselves. `pools` are the pools (K and V of every layer, host array)
+ * that one table addresses; all have the same page_rows and n_pages. All other
+ * arrays are device memory. refs[p] is the number of sequences that hold page p: 0 is
+ * free. Entries of a table that hold no page are -1.
+ *
+ * copy: page dst[i] of every pool becomes page src[i]'s content. No dst may be
+ * another dst or a src of the same call. Pairs with an id out of range are skipped. */
+xq_status xq_kv_pages_copy(const xq_tensor* pools, int32_t n_pools, const int32_t* src, const int32_t* dst, int32_t n,
+                           void* stream);
+
+/* compact: after a tree's verify the rows of the accepted path move to the front:
+ * row rows[b] + path[b * path_cols + j] of sequence b becomes row rows[b] + j, for
+ * j < min(n_path[b], path_cols), and rows_out[b] = rows[b] + that number. A path rises
+ * (path[j] < path[j + 1]); an entry below j is skipped. rows_out is not rows. */
+xq_status xq_kv_pages_compact(const xq_tensor* pools, int32_t n_pools, const int32_t* table, const int32_t* rows,
+                              int32_t n_seq, int32_t table_cols, const int32_t* path, const int32_t* n_path,
+                              int32_t path_cols, int32_t* rows_out, void* stream);
+
+/* reserve: each sequence is given pages for rows [0, want[b]) where its table has
+ * none, sequence after sequence and column after column, the lowest free page
+ * first, until none is left; refs of a page given is 1. got[b] is the number of rows, up
+ * to table_cols * page_rows, that the sequence's unbroken first pages hold then. */
+xq_status xq_kv_pages_reserve_workspace(int32_t n_seq, int32_t n_pages, size_t* bytes);
+xq_status xq_kv_pages_reserve(int32_t* table, int32_t* refs, int32_t n_seq, int32_t table_cols, int32_t n_pages,
+                              int32_t page_rows, const int32_t* want, int32_t* got, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* fork: sequence children[i] becomes a second holder of parents[i]'s rows: it shares the
+ * parent's full pages (refs + 1) and takes the lowest free page for a last page
+ * that is not full, whose rows are copied in every pool. Forks take their pages in order.
+ * done[i] = 1, or 0 where nothing was done: an id out of range, a child that holds
+ * rows or a first page, is named twice (the first stands) or is a parent of this
+ * call, a row of the parent's last page that is no page's, or no page left. n at most 1024. */
+xq_status xq_kv_pages_fork_workspace(int32_t n, size_t* bytes);
+xq_status xq_kv_pages_fork(const xq_tensor* pools, int32_t n_pools, int32_t* table, int32_t* rows, int32_t* refs,
+                           int32_t n_seq, int32_t table_cols, const int32_t* parents, const int32_t* children, int32_t n,
+                           int32_t* done, void* workspace, size_t workspace_bytes, void* stream);
+
+/* release: the sequences seqs[0..n) hold no page and no rows any more; refs of each of
+ * their pages falls by one. An id out of range, or named again, releases nothing. */
+xq_status xq_kv_pages_release(int32_t* table, int32_t* rows, int32_t* refs, int32_t n_seq, int32_t table_cols,
+                              int32_t n_pages, const int32_t* seqs, int32_t n, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Misc
  * ------------------------------------------------------------------------- */
 

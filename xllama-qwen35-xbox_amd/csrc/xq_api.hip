@@ -10,7 +10,7 @@
 #include <mutex>
 #include <string>
 
-#include "xq_kernels.h"
+#include "xq_host.h"
 
 // ------------------------------------------------------------ no-alloc scratch
 // The workspace of xq_flash_attn_ext_noalloc: one array per GPU, part of the
@@ -21,6 +21,11 @@ constexpr size_t kScratchBytes = (size_t)32 << 20;
 static __device__ __align__(256) uint8_t scratch[kScratchBytes];
 
 namespace {
+
+using xq::aligned;
+using xq::cdiv;
+using xq::record_bytes;
+using xq::type_size;
 
 thread_local std::string g_last_error;
 
@@ -39,40 +44,14 @@ xq_status ok() {
     return XQ_OK;
 }
 
-size_t type_size(int t) {  // ggml_type_size: bytes of one element or block
-    switch (t) {
-    case XQ_TYPE_F32: return 4;
-    case XQ_TYPE_F16:
-    case XQ_TYPE_BF16: return 2;
-    case XQ_TYPE_Q8_0: return 34;
-    case XQ_TYPE_Q4_0: return 18;
-    case XQ_TYPE_E5M2: return 1;
-    default: return 0;
-    }
-}
-
 bool kv_type_ok(int t) {
     return t == XQ_TYPE_F16 || t == XQ_TYPE_Q8_0 || t == XQ_TYPE_Q4_0 || t == XQ_TYPE_E5M2;
-}
-
-size_t record_bytes(int t, int64_t d) {
-    switch (t) {
-    case XQ_TYPE_F32: return (size_t)d * 4;
-    case XQ_TYPE_F16:
-    case XQ_TYPE_BF16: return (size_t)d * 2;
-    case XQ_TYPE_Q8_0: return (size_t)(d / 32) * 34;
-    case XQ_TYPE_Q4_0: return (size_t)(d / 32) * 18;
-    case XQ_TYPE_E5M2: return (size_t)d;
-    default: return 0;
-    }
 }
 
 // Copy granularity of the K/V staging loads for a record size.
 size_t kv_chunk(size_t rec) { return rec % 16 == 0 ? 16 : rec % 8 == 0 ? 8 : 4; }
 
 // ------------------------------------------------------------ split policy
-
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Reference optimized modes (uwp/rkva/rkva-range-profile.h:82-107).
 int64_t opt_split_k(int64_t active, int mode) {
@@ -236,8 +215,6 @@ xq_status fa_check(const xq_tensor* q, const xq_tensor* k, const xq_tensor* v,
     if (plan) *plan = P;
     return XQ_OK;
 }
-
-bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 
 }  // namespace
 

@@ -14,6 +14,7 @@ Mirrors the ggml op interface of the reference path:
   ``fa_range``         RemoteAttnEngine::attend_range (uwp/rkva/remote-attn-engine.h:152-154)
   ``gated_delta_net``  GGML_OP_GATED_DELTA_NET (src/bridge/ggml_d3d12.cpp:77-158,1905-1942)
   ``kv_store``         KV append (shaders/rkva/rkva_store_f16.hlsl:63-85, all KV types)
+The paged KV cache (``qk_norm_rope``, ``fa_tree``, ``kv_pages_*``) is in ``paged.py``.
 """
 from __future__ import annotations
 
@@ -46,6 +47,9 @@ EXPORTS = (
     "xq_ggml_backend_init", "xq_ggml_backend_free", "xq_ggml_backend_name", "xq_ggml_backend_stream",
     "xq_ggml_backend_workspace_bytes", "xq_ggml_supports_op", "xq_ggml_supports_op_params",
     "xq_ggml_graph_compute",
+    "xq_supports_qk_norm_rope", "xq_qk_norm_rope", "xq_supports_fa_tree", "xq_fa_tree_workspace", "xq_fa_tree",
+    "xq_kv_pages_copy", "xq_kv_pages_compact", "xq_kv_pages_reserve_workspace", "xq_kv_pages_reserve",
+    "xq_kv_pages_fork_workspace", "xq_kv_pages_fork", "xq_kv_pages_release",
 )
 
 
@@ -150,6 +154,7 @@ def load() -> ctypes.CDLL:
         "xq_ggml_supports_op_params": (ctypes.c_int, [ctypes.POINTER(XqGgmlNode), ctypes.POINTER(XqGgmlBackendParams)]),
         "xq_ggml_graph_compute": (i32, [P, ctypes.POINTER(XqGgmlNode), i32]),
     }
+    sig.update(signatures())
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -510,3 +515,12 @@ class GgmlBackend:
 
     def __exit__(self, *exc):
         self.free()
+
+
+# ---------------------------------------------------------------------------
+# the paged KV cache (needs the names above)
+# ---------------------------------------------------------------------------
+
+from .paged import (ROPE_HALVES, ROPE_PAIRS, KvPages, XqKvPages, XqRopeParams, fa_tree, fa_tree_workspace,  # noqa: E402,F401
+                    kv_pages_compact, kv_pages_copy, kv_pages_fork, kv_pages_release, kv_pages_reserve, pool_tensor,
+                    qk_norm_rope, rope_params, signatures, supports_fa_tree, supports_qk_norm_rope)
