@@ -1,4 +1,7 @@
 // xq_fa_tree.hip — attention of drafted tokens (a tree, a chain, one token) over the paged cache.
+#include <type_traits>
+
+#include "xq_kv_codec.h"
 #include "xq_paged.h"
 
 namespace xq {
@@ -14,69 +17,712 @@ struct TreeArgs {
     PagesView pg;
     const int32_t* parents;
     const int32_t* n_tok;
-    int32_t n_q, H, G, B, kt, bf16;
+    int32_t n_q, H, G, B;
     float scale;
+    UDivFlat d_g, d_wgs;      // by the group; by the workgroups
+    int32_t max_ptiles;       // pair tiles of a sequence with n_q tokens
+    int32_t part_pairs;       // pairs of a part
+    float* part_o;            // [parts][part_pairs][D]
+    float2* part_ml;          // [parts][part_pairs] maximum, sum
 };
 
+typedef _Float16 h2t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8t __attribute__((ext_vector_type(8)));
+typedef float f4t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint16_t u16any __attribute__((aligned(1)));
+typedef uint32_t u4half __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f4el __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kTr = 64;                // KV rows of a tile: a lane per row
+constexpr float kTreeLog2e = 1.4426950408889634f, kTreeLn2 = 0.6931471805599453f;
+constexpr float kTreeLazy = 8.0f;      // base-2 headroom before the running maximum moves
+constexpr float kTreeOff = 4.0f;       // weights are 2^(x - max - 4), in (0, 16]
+
+template <int KT, int D, bool NARROW, int MT, int WR>
+struct TreeCfg {
+    static constexpr bool QUANT = KT == XQ_TYPE_Q8_0 || KT == XQ_TYPE_Q4_0;
+    static constexpr int PARTS = QUANT && !NARROW ? 2 : 1;                  // f16 parts of a cached value
+    static constexpr int QP = NARROW ? 1 : 2;                               // f16 parts of Q and of the weights
+    static constexpr int EL = KT == XQ_TYPE_F16 ? 8 : KT == XQ_TYPE_Q4_0 ? 32 : 16;  // elements of a 16-byte piece
+    static constexpr int PPR = D / EL;                                      // pieces per row
+    static constexpr int NPT = kTr * PPR / 256;                             // pieces per thread and tensor
+    static constexpr int RSK = 2 * D + 16, RSV = 2 * D + 32;                // image rows, bytes
+    static constexpr int KB = kTr * RSK, VB = kTr * RSV;                    // one part
+    static constexpr int IMG = PARTS * (KB + VB);
+    static constexpr int PW = 16 * MT * (WR == 4 ? 1 : 4);                  // pairs of a workgroup
+    static constexpr int MS = D + 4;                                        // merge row stride, floats
+    static constexpr int MERGE = WR == 4 ? 4 * 16 * MS * 4 : 0;
+    static constexpr int SMEM = IMG > MERGE ? IMG : MERGE;
+};
+
+// Element d of a record in f32 (rows with a non-finite value only).
 template <int KT>
 XQ_DEV float kv_element(const uint8_t* rec, int d) {
-    if constexpr (KT == XQ_TYPE_F16) return f16_bits_to_f32(*(const uint16_t*)(rec + 2 * d));
-    if constexpr (KT == XQ_TYPE_E5M2) return e5m2_to_f32(rec[d]);
-    if constexpr (KT == XQ_TYPE_Q8_0) {
+    if constexpr (KT == XQ_TYPE_F16) {
+        return f16_bits_to_f32(*(const u16any*)(rec + 2 * d));
+    } else if constexpr (KT == XQ_TYPE_E5M2) {
+        return e5m2_to_f32(rec[d]);
+    } else if constexpr (KT == XQ_TYPE_Q8_0) {
         const uint8_t* b = rec + d / 32 * 34;
-        return f16_bits_to_f32(*(const uint16_t*)b) * (float)(int8_t)b[2 + d % 32];
+        return f16_bits_to_f32(*(const u16any*)b) * (float)(int8_t)b[2 + d % 32];
+    } else {
+        const uint8_t* b = rec + d / 32 * 18;
+        const int n = d % 32 < 16 ? b[2 + d % 16] & 15 : b[2 + d % 16] >> 4;
+        return f16_bits_to_f32(*(const u16any*)b) * (float)(n - 8);
     }
-    const uint8_t* b = rec + d / 32 * 18;
-    const int n = d % 32 < 16 ? b[2 + d % 16] & 15 : b[2 + d % 16] >> 4;
-    return f16_bits_to_f32(*(const uint16_t*)b) * (float)(n - 8);
 }
 
-// One wave per (sequence, token, head), one row after another.
-template <int KT, int D>
-__global__ __launch_bounds__(64) void fa_tree_plain(TreeArgs a) {
-    const int lane = threadIdx.x;
-    const int h = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-    const int n_tok = a.n_tok ? min(a.n_tok[b], a.n_q) : a.n_q;
-    if (t >= n_tok) return;
-    const int64_t held = max(0, a.pg.rows[b]);
-    const int hk = h / a.G;
-    uint64_t seen = 0;
-    for (int j = t; j >= 0;) {
-        seen |= (uint64_t)1 << j;
-        const int p = a.parents ? a.parents[(int64_t)b * a.n_q + j] : j - 1;
-        j = p < j ? p : -1;
+XQ_DEV float across_rows_max(float x) {  // over lanes l, l^16, l^32, l^48
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+XQ_DEV float across_rows_sum(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// Nonzero halves (0x8000 each) of w that are Inf or NaN.
+XQ_DEV uint32_t bad_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+XQ_DEV uint32_t without_bad(uint32_t w) { return w & ~((bad_halves(w) >> 15) * 0xffffu); }
+
+// 16 bytes of a record as f16 pairs, exact: NW words. q8_0 / q4_0: the integers.
+template <int KT, int NW>
+XQ_DEV void piece_f16(const u4t raw, uint32_t (&o)[NW]) {
+    if constexpr (KT == XQ_TYPE_F16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = raw[i];
+    } else if constexpr (KT == XQ_TYPE_E5M2) {  // byte b -> f16 bits b << 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = __builtin_amdgcn_perm(raw[i], raw[i], 0x010c000cu);
+            o[2 * i + 1] = __builtin_amdgcn_perm(raw[i], raw[i], 0x030c020cu);
+        }
+    } else if constexpr (KT == XQ_TYPE_Q8_0) {  // (1024 + (q ^ 0x80)) - 1152
+        const h2t k = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = raw[i] ^ 0x80808080u;
+            o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, __builtin_amdgcn_perm(0x64646464u, w, 0x05010500u)) + k);
+            o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, __builtin_amdgcn_perm(0x64646464u, w, 0x05030502u)) + k);
+        }
+    } else {  // low nibbles n (elements 0..15), then high ones: (1024 + n) - 1032
+        const h2t k = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = h ? (raw[i] >> 4) & 0x0f0f0f0fu : raw[i] & 0x0f0f0f0fu;
+                o[8 * h + 2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, __builtin_amdgcn_perm(0x64646464u, w, 0x05010500u)) + k);
+                o[8 * h + 2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, __builtin_amdgcn_perm(0x64646464u, w, 0x05030502u)) + k);
+            }
     }
+}
+
+// Four rows of one column (rows 4lg.. of the 16 at p's row, column lr of 16) from the image.
+XQ_DEV uint2 column4(const uint8_t* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(__attribute__((address_space(3))) uint8_t*)p));
+}
+
+// Wait states between a group of matrix products and the first vector instruction that reads
+// them. The compiler inserts these itself, but leaves them out where that reader is the first
+// instruction of a block (seen as scores of one register in four from before the product);
+// nothing moves across this.
+XQ_DEV void products_done() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7\n\ts_nop 1");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Work of sequence b: its rows, tokens, row tiles and (KV head, pair tile, row tile) units.
+struct SeqWork {
+    int32_t held, n_tok, end;
+    uint32_t tiles, ptiles, units;
+};
+template <int PW>
+XQ_DEV SeqWork seq_work(const TreeArgs& a, int b) {
+    SeqWork s;
+    s.held = min(max(a.pg.rows[b], 0), a.pg.row_limit);
+    s.n_tok = a.n_tok ? min(max(a.n_tok[b], 0), a.n_q) : a.n_q;
+    s.end = (int32_t)min((uint32_t)s.held + (uint32_t)s.n_tok, (uint32_t)a.pg.row_limit);
+    s.tiles = s.n_tok ? ((uint32_t)s.end + kTr - 1) / kTr : 0u;
+    s.ptiles = (uint32_t)(s.n_tok * a.G + PW - 1) / PW;
+    s.units = s.tiles * s.ptiles * (uint32_t)a.pg.n_head_kv;
+    return s;
+}
+
+// The units of all sequences dealt to the workgroups in order, as evenly as they go.
+struct Deal {
+    uint32_t per, more;  // units per workgroup; the first `more` have one more
+    XQ_DEV Deal(uint32_t units, const UDivFlat& d_wgs) {
+        per = d_wgs.quot(units);
+        more = units - per * d_wgs.d;
+    }
+    XQ_DEV uint32_t first(uint32_t w) const { return w * per + min(w, more); }
+    XQ_DEV uint32_t owner(uint32_t u) const {  // the workgroup that has unit u
+        const uint32_t big = more * (per + 1);
+        return u < big ? u / (per + 1) : more + (u - big) / per;
+    }
+};
+
+XQ_DEV uint32_t wave_scan(uint32_t x) {  // inclusive, over the 64 lanes
+    const int lane = lane_id();
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_up(x, d);
+        x += lane >= d ? y : 0u;
+    }
+    return x;
+}
+XQ_DEV uint32_t lane_get(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
+
+template <int PW>
+XQ_DEV uint32_t all_units(const TreeArgs& a) {
+    uint32_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int b = b0 + lane_id();
+        total += lane_get(wave_scan(b < a.B ? seq_work<PW>(a, b).units : 0u), 63);
+    }
+    return total;
+}
+
+template <int KT, int D, bool NARROW, int MT, int WR>
+__global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
+    using C = TreeCfg<KT, D, NARROW, MT, WR>;
+    constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW;
+    constexpr bool QUANT = C::QUANT;
+    constexpr int RT = 4 / WR;              // 16-row score tiles of a wave
+    constexpr int GR = RT >= 2 ? 2 : 1;     // of them at a time
+    __shared__ __attribute__((aligned(16))) uint8_t img[C::SMEM];
+    __shared__ float sM[4][16 * MT], sL[4][16 * MT];
+    __shared__ int sEk[PARTS == 2 ? kTr : 1], sEv[PARTS == 2 ? kTr : 1];
+    __shared__ unsigned long long sBad[2];
+    const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x, lr = lane & 15, lg = lane >> 4;
+    uint8_t* const imgK = img;
+    uint8_t* const imgV = img + PARTS * C::KB;
+
+    const uint32_t w = xcd_remap(blockIdx.x, a.d_wgs.d);
+    const Deal deal(all_units<PW>(a), a.d_wgs);
+    uint32_t u = deal.first(w);
+    const uint32_t u_end = deal.first(w + 1);
+    // the chunk of 64 sequences that holds unit u: lane l has sequence b0 + l
+    int b0 = 0;
+    uint32_t carry = 0;
+    while (u < u_end) {
+        // ---- the segment (sequence, KV head, pair tile) that unit u belongs to
+        SeqWork mine{};
+        uint32_t upto = 0;
+        for (;;) {
+            mine = SeqWork{};
+            if (b0 + lane < a.B) mine = seq_work<PW>(a, b0 + lane);
+            upto = carry + wave_scan(mine.units);
+            const uint32_t last = lane_get(upto, 63);
+            if (u < last) break;
+            carry = last;
+            b0 += 64;
+        }
+        const int sl = __builtin_ctzll(__builtin_amdgcn_ballot_w64(u < upto));
+        const int b = b0 + sl;
+        const int held = (int)lane_get((uint32_t)mine.held, sl), n_tok = (int)lane_get((uint32_t)mine.n_tok, sl);
+        const int end = (int)lane_get((uint32_t)mine.end, sl);
+        const uint32_t tiles = lane_get(mine.tiles, sl), ptiles = lane_get(mine.ptiles, sl);
+        const uint32_t in_b = u - (lane_get(upto, sl) - lane_get(mine.units, sl));
+        const uint32_t seg = in_b / tiles, t_first = in_b - seg * tiles;
+        const int hk = (int)(seg / ptiles), pt = (int)(seg - (uint32_t)hk * ptiles);
+        const uint32_t t_last = min(tiles, t_first + (u_end - u));
+        const bool whole = t_first == 0 && t_last == tiles;
+        const int n_pairs = n_tok * a.G;
+        const int p0 = pt * PW + (WR == 4 ? 0 : wave * 16 * MT);  // this wave's first pair
+
+        const uint8_t* const kb = a.pg.k + hk * a.pg.k_head;
+        const uint8_t* const vb = a.pg.v + hk * a.pg.v_head;
+        // row lane of tile t: its page (~0u where there is none) and its place in it
+        auto lookup = [&](uint32_t t, uint32_t& page, uint32_t& in) {
+            const uint32_t r = t * kTr + lane;
+            page = ~0u;
+            in = 0;
+            if (t < t_last && r < (uint32_t)end) {
+                const uint32_t c = a.pg.d_page.quot(r);
+                page = (uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c];
+                in = r - c * a.pg.d_page.d;
+            }
+        };
+        u4t rk[NPT], rv[NPT];
+        uint32_t dk[QUANT ? NPT : 1], dv[QUANT ? NPT : 1];
+        auto fetch = [&](uint32_t page, uint32_t in) {
+#pragma unroll
+            for (int j = 0; j < NPT; ++j) {
+                const int i = tid + 256 * j, r = i / PPR, c = i % PPR;
+                const uint32_t p = (uint32_t)__shfl((int)page, r), x = (uint32_t)__shfl((int)in, r);
+                rk[j] = u4t{0, 0, 0, 0};
+                rv[j] = u4t{0, 0, 0, 0};
+                if constexpr (QUANT) dk[j] = dv[j] = 0u;
+                if (p < (uint32_t)a.pg.n_pages) {
+                    const uint8_t* k = kb + p * a.pg.k_page + x * a.pg.k_row;
+                    const uint8_t* v = vb + p * a.pg.v_page + x * a.pg.v_row;
+                    constexpr int BB = KT == XQ_TYPE_Q8_0 ? 34 : 18;
+                    const int blk = KT == XQ_TYPE_Q8_0 ? c / 2 : c;
+                    const int at = QUANT ? blk * BB + 2 + (KT == XQ_TYPE_Q8_0 ? c % 2 * 16 : 0) : 16 * c;
+                    rk[j] = *(const u4any*)(k + at);
+                    rv[j] = *(const u4any*)(v + at);
+                    if constexpr (QUANT) {
+                        dk[j] = *(const u16any*)(k + blk * BB);
+                        dv[j] = *(const u16any*)(v + blk * BB);
+                    }
+                }
+            }
+        };
+        // raw pieces -> image
+        auto put = [&](uint8_t* image, int rs, int part_bytes, const u4t raw, uint32_t d, int r, int c, int* exps, bool clean, uint32_t t) {
+            constexpr int NW = C::EL / 2;
+            uint32_t o[NW], lo[NW];
+            piece_f16<KT, NW>(raw, o);
+            if constexpr (QUANT && PARTS == 1) {
+                const uint32_t dd = d | (d << 16);
+#pragma unroll
+                for (int i = 0; i < NW; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, o[i]) * __builtin_bit_cast(h2t, dd));
+            } else if constexpr (QUANT) {
+                // the row's power of two: its largest finite block scale to [2^7, 2^8)
+                int e = (int)((__float_as_uint(f16_bits_to_f32(d)) >> 23) & 255u);
+                if (e == 255 || e == 0) e = 1;
+#pragma unroll
+                for (int s = 1; s < PPR; s *= 2) e = max(e, __shfl_xor(e, s));
+                e -= 127 + 7;
+                const float f = ldexpf(f16_bits_to_f32(d), -e);
+                if (c == 0) exps[r] = e;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    const h2t q = __builtin_bit_cast(h2t, o[i]);
+                    const float x = (float)q[0] * f, y = (float)q[1] * f;
+                    const h2t hi = {(_Float16)x, (_Float16)y};
+                    const h2t l2 = {(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])};
+                    o[i] = __builtin_bit_cast(uint32_t, hi);
+                    lo[i] = __builtin_bit_cast(uint32_t, l2);
+                }
+            }
+            if (clean) {
+                uint32_t bad = 0;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    bad |= bad_halves(o[i]);
+                    if constexpr (PARTS == 2) lo[i] &= ~((bad_halves(o[i]) >> 15) * 0xffffu);
+                    o[i] = without_bad(o[i]);
+                }
+                if (bad) atomicOr(&sBad[t & 1], 1ull << r);
+            }
+            uint8_t* y = image + r * rs + c * (2 * C::EL);
+#pragma unroll
+            for (int i = 0; i < NW; i += 4) {
+                *(u4t*)(y + 4 * i) = u4t{o[i], o[i + 1], o[i + 2], o[i + 3]};
+                if constexpr (PARTS == 2) *(u4t*)(y + part_bytes + 4 * i) = u4t{lo[i], lo[i + 1], lo[i + 2], lo[i + 3]};
+            }
+        };
+        auto commit = [&](uint32_t t) {
+            const bool clean = (t + 1) * kTr > (uint32_t)held;  // holds rows that only some tokens see
+#pragma unroll
+            for (int j = 0; j < NPT; ++j) {
+                const int i = tid + 256 * j, r = i / PPR, c = i % PPR;
+                put(imgK, C::RSK, C::KB, rk[j], QUANT ? dk[j] : 0u, r, c, sEk, false, t);
+                put(imgV, C::RSV, C::VB, rv[j], QUANT ? dv[j] : 0u, r, c, sEv, clean, t);
+            }
+        };
+
+        uint32_t page, in;
+        lookup(t_first, page, in);
+        const int32_t up = a.parents && lane < n_tok ? a.parents[(int64_t)b * a.n_q + lane] : lane - 1;
+
+        // ---- Q operands: pair 16m + lr, elements 8lg.. of each 32, times a power of two that
+        //      puts the row's largest element in [2^14, 2^15)
+        h8t qo[MT][NB][QP];
+        float qf[MT];
+        int tok[MT];
+        {
+            float xq[MT][NB][8];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int p = min(p0 + 16 * m + lr, n_pairs - 1);
+                tok[m] = (int)a.d_g.quot((uint32_t)p);
+                const uint8_t* q = a.q + b * a.q_nb3 + tok[m] * a.q_nb1 + (hk * a.G + p - tok[m] * a.G) * a.q_nb2;
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    const int e = 32 * c + 8 * lg;
+                    if constexpr (NARROW) {
+                        const u4half x = *(const u4half*)(q + 2 * e);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            xq[m][c][2 * i] = __uint_as_float(x[i] << 16);
+                            xq[m][c][2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+                        }
+                    } else {
+                        const f4el x = *(const f4el*)(q + 4 * e), y = *(const f4el*)(q + 4 * e + 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            xq[m][c][i] = x[i];
+                            xq[m][c][4 + i] = y[i];
+                        }
+                    }
+                }
+            }
+            fetch(page, in);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float big = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(xq[m][c][j]));
+                const int lift = 141 - min((int)(__float_as_uint(across_rows_max(big)) >> 23), 254);
+                qf[m] = ldexpf(a.scale * kTreeLog2e, -lift);
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = ldexpf(xq[m][c][j], lift);
+                        const _Float16 hi = (_Float16)x;
+                        qo[m][c][0][j] = hi;
+                        if constexpr (QP == 2) qo[m][c][1][j] = (_Float16)(x - (float)hi);
+                    }
+            }
+        }
+        uint64_t valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+        lookup(t_first + 1, page, in);
+
+        f4t acc[MT][ND];
+        float m_run[MT], l_run[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            m_run[m] = -INFINITY;
+            l_run[m] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) acc[m][n] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        int e_run = -1000;  // PARTS 2: the accumulators hold their sums times 2^-e_run
+        if (tid < 2) sBad[tid] = 0;
+
+        for (uint32_t t = t_first; t < t_last; ++t) {
+            __syncthreads();  // the image is free, the flags are zero
+            commit(t);
+            __syncthreads();
+            const uint64_t now = valid;
+            if (t + 1 < t_last) {
+                fetch(page, in);
+                valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+                lookup(t + 2, page, in);
+            }
+            if (tid == 0) sBad[(t + 1) & 1] = 0;
+
+            // which of the tile's rows each pair sees
+            const bool careful = (t + 1) * kTr > (uint32_t)held || now != ~0ull;
+            uint64_t sees[MT];
+            if (careful) {
+                // ancestors by doubling: lane i is token i
+                const int first = (int)(t * kTr);
+                uint64_t anc = 0;
+                if (first + kTr > held) {
+                    int32_t p = up >= 0 && up < lane ? up : -1;
+                    anc = 1ull << lane;
+#pragma unroll
+                    for (int d = 0; d < 6; ++d) {
+                        const int from = p < 0 ? lane : p;
+                        const uint32_t x = (uint32_t)__shfl((int)(uint32_t)anc, from), y = (uint32_t)__shfl((int)(uint32_t)(anc >> 32), from);
+                        anc |= ((uint64_t)y << 32) | x;
+                        const int32_t q = __shfl(p, from);
+                        p = p < 0 ? -1 : q;
+                    }
+                }
+                const int sh = held - first;  // rows of the tile that every token sees, below 0: of the tokens passed
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const uint64_t x = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(anc >> 32), tok[m]) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, tok[m]);
+                    uint64_t s = sh >= 64 ? ~0ull : sh >= 0 ? (x << sh) | ((1ull << sh) - 1) : sh > -64 ? x >> -sh : 0ull;
+                    sees[m] = s & now;
+                }
+            }
+            if constexpr (PARTS == 2) {
+                int e = sEv[lane];
+#pragma unroll
+                for (int s = 1; s < 64; s *= 2) e = max(e, __shfl_xor(e, s));
+                e = __builtin_amdgcn_readfirstlane(e);
+                if (e > e_run) {
+                    const float f = ldexpf(1.0f, e_run - e);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int n = 0; n < ND; ++n) acc[m][n] *= f;
+                    e_run = e;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < RT / GR; ++g) {
+                const int row0 = WR == 4 ? 16 * wave : 32 * g;
+                f4t s[MT][GR];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int r = 0; r < GR; ++r) s[m][r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int r = 0; r < GR; ++r) {
+                        const uint8_t* k = imgK + (row0 + 16 * r + lr) * C::RSK + 64 * c + 16 * lg;
+                        const h8t kh = *(const h8t*)k;
+                        h8t kl;
+                        if constexpr (PARTS == 2) kl = *(const h8t*)(k + C::KB);
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][0], s[m][r], 0, 0, 0);
+                            if constexpr (QP == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][1], s[m][r], 0, 0, 0);
+                            if constexpr (PARTS == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qo[m][c][0], s[m][r], 0, 0, 0);
+                        }
+                    }
+                products_done();
+                // base-2 scores; the lane's rows are row0 + 16r + 4lg + i
+                bool over = false;
+                float top[MT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    top[m] = -INFINITY;
+#pragma unroll
+                    for (int r = 0; r < GR; ++r) {
+                        s[m][r] *= qf[m];
+                        if constexpr (PARTS == 2) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[m][r][i] = ldexpf(s[m][r][i], sEk[row0 + 16 * r + 4 * lg + i]);
+                        }
+                        if (careful) {
+                            const uint32_t bits = (uint32_t)(sees[m] >> (row0 + 16 * r + 4 * lg));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[m][r][i] = (bits >> i) & 1u ? s[m][r][i] : -INFINITY;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top[m] = fmaxf(top[m], s[m][r][i]);
+                    }
+                    over |= top[m] > m_run[m] + kTreeLazy;
+                }
+                if (__builtin_amdgcn_ballot_w64(over)) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const float mt = across_rows_max(top[m]);
+                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) : m_run[m];
+                        const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
+                        l_run[m] *= f;
+#pragma unroll
+                        for (int n = 0; n < ND; ++n) acc[m][n] *= f;
+                        m_run[m] = mn;
+                    }
+                }
+                // weights
+                h4t ph[MT][GR], pl[QP == 2 ? MT : 1][QP == 2 ? GR : 1];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const float mu = m_run[m] == -INFINITY ? 0.0f : m_run[m] + kTreeOff;
+#pragma unroll
+                    for (int r = 0; r < GR; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float p = __builtin_amdgcn_exp2f(s[m][r][i] - mu);
+                            l_run[m] += p;
+                            if constexpr (PARTS == 2) p *= ldexpf(1.0f, sEv[row0 + 16 * r + 4 * lg + i] - e_run);
+                            ph[m][r][i] = (_Float16)p;
+                            if constexpr (QP == 2) pl[m][r][i] = (_Float16)(p - (float)ph[m][r][i]);
+                        }
+                }
+                // O^T += V^T P^T
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    const uint8_t* v = imgV + (row0 + 4 * lg + (lr >> 2)) * C::RSV + 32 * n + 8 * (lr & 3);
+                    h4t vh[GR], vl[PARTS == 2 ? GR : 1];
+#pragma unroll
+                    for (int r = 0; r < GR; ++r) {
+                        vh[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV));
+                        if constexpr (PARTS == 2) vl[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV + C::VB));
+                    }
+                    auto product = [&](const h4t (&x)[GR], const h4t (&p)[GR], f4t& o) {
+                        if constexpr (GR == 2)
+                            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(x[0], x[GR - 1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                      __builtin_shufflevector(p[0], p[GR - 1], 0, 1, 2, 3, 4, 5, 6, 7), o, 0, 0, 0);
+                        else
+                            o = __builtin_amdgcn_mfma_f32_16x16x16f16(x[0], p[0], o, 0, 0, 0);
+                    };
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        product(vh, ph[m], acc[m][n]);
+                        if constexpr (QP == 2) product(vh, pl[m], acc[m][n]);
+                        if constexpr (PARTS == 2) product(vl, ph[m], acc[m][n]);
+                    }
+                }
+            }
+            products_done();
+            // non-finite values of rows that not every token sees: to the tokens that do
+            if (careful) {
+                uint64_t bad = sBad[t & 1];
+                if constexpr (WR == 4) bad &= 0xffffull << (16 * wave);
+                bad = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(bad >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)bad);
+                while (bad) {
+                    const int r = __builtin_ctzll(bad);
+                    bad &= bad - 1;
+                    const uint32_t row = t * kTr + r, c = a.pg.d_page.quot(row);
+                    const uint8_t* v = vb + (uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c] * a.pg.v_page + (row - c * a.pg.d_page.d) * a.pg.v_row;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 16)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = kv_element<KT>(v, d + 4 * lg + i);
+                            const bool inf = PARTS == 2 ? !__builtin_isfinite(x) : !(fabsf(x) < 65520.0f);
+                            if (!__builtin_amdgcn_ballot_w64(inf)) continue;
+                            const float y = __builtin_isfinite(x) ? copysignf(INFINITY, x) : x;
+#pragma unroll
+                            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                                for (int n = 0; n < ND; ++n)
+                                    if (16 * n == d && inf && (sees[m] >> r) & 1) acc[m][n][i] += y;
+                        }
+                }
+            }
+        }
+        u += t_last - t_first;
+
+        // ---- the segment's result, or this workgroup's part of it
+        if constexpr (PARTS == 2) {
+            const float f = ldexpf(1.0f, max(e_run, -126));
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < ND; ++n) acc[m][n] *= f;
+        }
+        const uint32_t piece = w + (uint32_t)((b * a.pg.n_head_kv + hk) * a.max_ptiles + pt);
+        auto emit = [&](int p, int d, f4t o, float mm, float l, bool first) {  // pair p of the segment's tile, dims d..d+3
+            if (whole) {
+                const int q = pt * PW + p, t = (int)a.d_g.quot((uint32_t)q), h = hk * a.G + q - t * a.G;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                uint8_t* y = a.dst + b * a.d_nb3 + t * a.d_nb2 + h * a.d_nb1;
+                if constexpr (NARROW) {
+                    const uint32_t w0 = f32_to_bf16_bits(o[0] * inv) | (f32_to_bf16_bits(o[1] * inv) << 16);
+                    const uint32_t w1 = f32_to_bf16_bits(o[2] * inv) | (f32_to_bf16_bits(o[3] * inv) << 16);
+                    *(uint2*)(y + 2 * d) = make_uint2(w0, w1);
+                } else {
+                    *(f4t*)(y + 4 * d) = o * inv;
+                }
+                if (first && a.lse) a.lse[((int64_t)b * a.n_q + t) * a.H + h] = l == 0.0f ? -INFINITY : (mm + kTreeOff) * kTreeLn2 + logf(l);
+            } else {
+                const int64_t at = (int64_t)piece * a.part_pairs + p;
+                *(f4t*)(a.part_o + at * D + d) = o;
+                if (first) a.part_ml[at] = make_float2(mm, l);
+            }
+        };
+        if constexpr (WR == 4) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                l_run[m] = across_rows_sum(l_run[m]);
+                if (lg == 0) {
+                    sM[wave][16 * m + lr] = m_run[m];
+                    sL[wave][16 * m + lr] = l_run[m];
+                }
+            }
+            __syncthreads();  // the last tile is read, the states are there
+            float* const mg = (float*)img;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const float top = fmaxf(fmaxf(sM[0][16 * m + lr], sM[1][16 * m + lr]), fmaxf(sM[2][16 * m + lr], sM[3][16 * m + lr]));
+                const float f = m_run[m] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[m] - top);
+#pragma unroll
+                for (int n = 0; n < ND; ++n) *(f4t*)(mg + (16 * wave + lr) * C::MS + 16 * n + 4 * lg) = acc[m][n] * f;
+                __syncthreads();
+                for (int i = tid; i < 16 * D / 4; i += 256) {
+                    const int p = i / (D / 4), d = 4 * (i % (D / 4)), q = 16 * m + p;
+                    if (pt * PW + q < n_pairs) {
+                        const float mm = fmaxf(fmaxf(sM[0][q], sM[1][q]), fmaxf(sM[2][q], sM[3][q]));
+                        float l = 0.0f;
+                        f4t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (sM[x][q] != -INFINITY) l = fmaf(sL[x][q], __builtin_amdgcn_exp2f(sM[x][q] - mm), l);
+                            o += *(const f4t*)(mg + (16 * x + p) * C::MS + d);
+                        }
+                        emit(q, d, o, mm, l, d == 0);
+                    }
+                }
+                __syncthreads();
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const int p = p0 - pt * PW + 16 * m + lr;
+                const float l = across_rows_sum(l_run[m]);
+                if (p0 + 16 * m + lr < n_pairs) {
+#pragma unroll
+                    for (int n = 0; n < ND; ++n) emit(p, 16 * n + 4 * lg, acc[m][n], m_run[m], l, n == 0 && lg == 0);
+                }
+            }
+        }
+    }
+}
+
+// Joins the parts of the segments that more than one workgroup had: one wave per
+// (sequence, token, head), lane p the p-th part's maximum and sum, then all lanes the dims.
+template <int D, bool NARROW, int PW>
+__global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
+    const int lane = lane_id();
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
+    if (row >= (int64_t)a.B * a.n_q * a.H) return;
+    const int h = (int)(row % a.H), t = (int)(row / a.H % a.n_q), b = (int)(row / a.H / a.n_q);
+    const SeqWork s = seq_work<PW>(a, b);
+    if (t >= s.n_tok) return;
+    uint32_t before = 0, total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const uint32_t x = wave_scan(b0 + lane < a.B ? seq_work<PW>(a, b0 + lane).units : 0u);
+        if (b > b0) before = total + lane_get(x, min(b - b0, 64) - 1);
+        total += lane_get(x, 63);
+    }
+    const Deal deal(total, a.d_wgs);
+    const int hk = h / a.G, pair = t * a.G + h - hk * a.G, pt = pair / PW;
+    const uint32_t u0 = before + ((uint32_t)hk * s.ptiles + (uint32_t)pt) * s.tiles;
+    const uint32_t w0 = deal.owner(u0), w1 = deal.owner(u0 + s.tiles - 1);
+    if (w0 == w1) return;
+    const int64_t piece0 = (int64_t)w0 + (b * a.pg.n_head_kv + hk) * a.max_ptiles + pt;
+    const int n = (int)(w1 - w0) + 1, p = pair - pt * PW;
     constexpr int E = D / 64;
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-    const uint8_t* qp = a.q + b * a.q_nb3 + t * a.q_nb1 + h * a.q_nb2;
-    for (int i = 0; i < E; ++i) {
-        const int d = lane * E + i;
-        q[i] = a.bf16 ? bf16_bits_to_f32(*(const uint16_t*)(qp + 2 * d)) : *(const float*)(qp + 4 * d);
-        o[i] = 0.0f;
+    float o[E] = {}, l = 0.0f, top = -INFINITY;
+    for (int x = lane; x < n; x += 64) top = fmaxf(top, a.part_ml[(piece0 + x) * a.part_pairs + p].x);
+    top = wave_max(top);
+    for (int x0 = 0; x0 < n; x0 += 64) {
+        const int x = x0 + lane;
+        float f = 0.0f;
+        if (x < n) {
+            const float2 ml = a.part_ml[(piece0 + x) * a.part_pairs + p];
+            if (ml.x != -INFINITY) {
+                f = __builtin_amdgcn_exp2f(ml.x - top);
+                l = fmaf(ml.y, f, l);
+            }
+        }
+        const int m = min(64, n - x0);
+#pragma unroll 8
+        for (int i = 0; i < m; ++i) {
+            const float g = lane_read(f, i);
+            const float* y = a.part_o + ((piece0 + x0 + i) * a.part_pairs + p) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(g, y[e], o[e]);
+        }
     }
-    for (int64_t r = 0; r < held + n_tok && r < a.pg.row_limit; ++r) {
-        if (r >= held && !(seen >> (r - held) & 1)) continue;
-        const uint32_t page = a.pg.page(b, (uint32_t)r);
-        if (page >= (uint32_t)a.pg.n_pages) continue;
-        const int64_t in = r % a.pg.page_rows;
-        const uint8_t* k = a.pg.k + page * a.pg.k_page + in * a.pg.k_row + hk * a.pg.k_head;
-        const uint8_t* v = a.pg.v + page * a.pg.v_page + in * a.pg.v_row + hk * a.pg.v_head;
-        float s = 0.0f;
-        for (int i = 0; i < E; ++i) s = fmaf(q[i], kv_element<KT>(k, lane * E + i), s);
-        s = wave_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), f = m == mn ? 1.0f : expf(m - mn), w = expf(s - mn);
-        m = mn;
-        l = fmaf(l, f, w);
-        for (int i = 0; i < E; ++i) o[i] = fmaf(w, kv_element<KT>(v, lane * E + i), o[i] * f);
-    }
+    l = wave_sum(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint8_t* dp = a.dst + b * a.d_nb3 + t * a.d_nb2 + h * a.d_nb1;
-    for (int i = 0; i < E; ++i) {
-        const int d = lane * E + i;
-        if (a.bf16) *(__bf16*)(dp + 2 * d) = (__bf16)(o[i] * inv);
-        else *(float*)(dp + 4 * d) = o[i] * inv;
+    uint8_t* y = a.dst + b * a.d_nb3 + t * a.d_nb2 + h * a.d_nb1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if constexpr (NARROW)
+            *(uint16_t*)(y + 2 * (lane * E + e)) = (uint16_t)f32_to_bf16_bits(o[e] * inv);
+        else
+            *(float*)(y + 4 * (lane * E + e)) = o[e] * inv;
     }
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.n_q + t) * a.H + h] = l > 0.0f ? m + logf(l) : -INFINITY;
+    if (a.lse && lane == 0) a.lse[((int64_t)b * a.n_q + t) * a.H + h] = l == 0.0f ? -INFINITY : (top + kTreeOff) * kTreeLn2 + logf(l);
 }
 
 static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, PagesView* pg) {
@@ -105,6 +751,66 @@ static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const 
     return XQ_OK;
 }
 
+// The kernel variant, workgroups and workspace of a call: of its shapes alone.
+struct TreePlan {
+    int wr, mt, pw;           // waves over the rows (4) or over the pairs (1), pair tiles per wave, pairs of a workgroup
+    uint32_t wgs;
+    int32_t max_ptiles, part_pairs;
+    int64_t parts;
+    size_t ml_at, bytes;
+};
+static TreePlan tree_plan(const xq_tensor* q, const xq_kv_pages* c) {
+    TreePlan P{};
+    const int64_t D = q->ne[0], Hkv = c->k.ne[2], B = q->ne[3], pairs = q->ne[1] * (q->ne[2] / Hkv);
+    const bool narrow = q->type == XQ_TYPE_BF16;
+    const int most = narrow ? (D == 128 ? 4 : 2) : (D == 128 ? 2 : 1);
+    if (pairs <= 16) P.wr = 4, P.mt = 1;
+    else if (pairs <= 32) P.wr = 4, P.mt = 2;
+    else if (pairs <= 64 || most == 1) P.wr = 1, P.mt = 1;
+    else if (pairs <= 128 || most == 2) P.wr = 1, P.mt = 2;
+    else P.wr = 1, P.mt = 4;
+    P.pw = 16 * P.mt * (P.wr == 4 ? 1 : 4);
+    P.max_ptiles = (int32_t)cdiv(pairs, P.pw);
+    P.part_pairs = (int32_t)(pairs < P.pw ? pairs : P.pw);
+    const int64_t segs = B * Hkv * P.max_ptiles;
+    // tiles that the table could hold, at most
+    const int64_t tiles = cdiv((int64_t)c->table_cols * c->k.ne[1], kTr) * segs;
+    int64_t wgs = P.wr == 4 ? 1024 : 512;
+    if (wgs > tiles) wgs = tiles;
+    P.wgs = (uint32_t)wgs;
+    P.parts = wgs + segs;
+    const size_t o = (size_t)P.parts * P.part_pairs * D * 4;
+    P.ml_at = (o + 255) / 256 * 256;
+    P.bytes = P.ml_at + (size_t)P.parts * P.part_pairs * 8;
+    return P;
+}
+
+template <int KT, int D, bool NARROW>
+static void tree_launch(const TreePlan& P, const TreeArgs& a, hipStream_t s) {
+    const dim3 grid(P.wgs), block(256), rows((uint32_t)cdiv((int64_t)a.B * a.n_q * a.H, 4));
+    auto go = [&](auto mt_tag, auto wr_tag) {
+        constexpr int MT = decltype(mt_tag)::value, WR = decltype(wr_tag)::value;
+        launch("fa_tree", fa_tree_kernel<KT, D, NARROW, MT, WR>, grid, block, s, a);
+        launch("fa_tree_join", fa_tree_join<D, NARROW, TreeCfg<KT, D, NARROW, MT, WR>::PW>, rows, block, s, a);
+    };
+    std::integral_constant<int, 1> one;
+    std::integral_constant<int, 2> two;
+    std::integral_constant<int, 4> four;
+    if (P.wr == 4 && P.mt == 1) go(one, four);
+    else if (P.wr == 4) go(two, four);
+    else if (P.mt == 1) go(one, one);
+    else if constexpr (NARROW || D == 128) {
+        if (P.mt == 2) go(two, one);
+        else if constexpr (NARROW && D == 128) go(four, one);
+    }
+}
+
+template <int KT>
+static void tree_launch_type(const TreePlan& P, const TreeArgs& a, int64_t D, bool narrow, hipStream_t s) {
+    if (D == 128) narrow ? tree_launch<KT, 128, true>(P, a, s) : tree_launch<KT, 128, false>(P, a, s);
+    else narrow ? tree_launch<KT, 256, true>(P, a, s) : tree_launch<KT, 256, false>(P, a, s);
+}
+
 }  // namespace xq
 
 using namespace xq;
@@ -119,7 +825,7 @@ xq_status xq_fa_tree_workspace(const xq_tensor* q, const xq_kv_pages* cache, con
     if (!bytes) return failf(XQ_ERR_BAD_ARG, "bytes is null");
     const xq_status st = tree_check(q, cache, dst, nullptr);
     if (st != XQ_OK) return st;
-    *bytes = 256;
+    *bytes = tree_plan(q, cache).bytes;
     return done_ok();
 }
 
@@ -132,7 +838,8 @@ xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t
     if (!q->data || !dst->data || pages_null(cache)) return failf(XQ_ERR_BAD_ARG, "null data pointer");
     for (const void* x : {(const void*)parents, (const void*)n_tok, (const void*)lse, (const void*)cache->table, (const void*)cache->rows})
         if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
-    const size_t need = 256;
+    const TreePlan P = tree_plan(q, cache);
+    const size_t need = P.bytes;
     if (!workspace || workspace_bytes < need) return failf(XQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     if (!aligned(workspace, 256)) return failf(XQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
     a.q = (const uint8_t*)q->data;
@@ -142,15 +849,16 @@ xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t
     a.lse = lse, a.parents = parents, a.n_tok = n_tok, a.scale = scale;
     a.n_q = (int32_t)q->ne[1], a.H = (int32_t)q->ne[2], a.B = (int32_t)q->ne[3];
     a.G = a.H / a.pg.n_head_kv;
-    a.kt = cache->k.type, a.bf16 = q->type == XQ_TYPE_BF16;
-    const dim3 grid((uint32_t)a.H, (uint32_t)a.n_q, (uint32_t)a.B), block(64);
+    a.d_g = UDivFlat((uint32_t)a.G), a.d_wgs = UDivFlat(P.wgs);
+    a.max_ptiles = P.max_ptiles, a.part_pairs = P.part_pairs;
+    a.part_o = (float*)workspace, a.part_ml = (float2*)((uint8_t*)workspace + P.ml_at);
+    const bool narrow = q->type == XQ_TYPE_BF16;
     hipStream_t s = (hipStream_t)stream;
-    const bool wide = q->ne[0] == 256;
-    switch (a.kt) {
-    case XQ_TYPE_F16: launch("fa_tree", wide ? fa_tree_plain<XQ_TYPE_F16, 256> : fa_tree_plain<XQ_TYPE_F16, 128>, grid, block, s, a); break;
-    case XQ_TYPE_E5M2: launch("fa_tree", wide ? fa_tree_plain<XQ_TYPE_E5M2, 256> : fa_tree_plain<XQ_TYPE_E5M2, 128>, grid, block, s, a); break;
-    case XQ_TYPE_Q8_0: launch("fa_tree", wide ? fa_tree_plain<XQ_TYPE_Q8_0, 256> : fa_tree_plain<XQ_TYPE_Q8_0, 128>, grid, block, s, a); break;
-    default: launch("fa_tree", wide ? fa_tree_plain<XQ_TYPE_Q4_0, 256> : fa_tree_plain<XQ_TYPE_Q4_0, 128>, grid, block, s, a); break;
+    switch (cache->k.type) {
+    case XQ_TYPE_F16: tree_launch_type<XQ_TYPE_F16>(P, a, q->ne[0], narrow, s); break;
+    case XQ_TYPE_E5M2: tree_launch_type<XQ_TYPE_E5M2>(P, a, q->ne[0], narrow, s); break;
+    case XQ_TYPE_Q8_0: tree_launch_type<XQ_TYPE_Q8_0>(P, a, q->ne[0], narrow, s); break;
+    default: tree_launch_type<XQ_TYPE_Q4_0>(P, a, q->ne[0], narrow, s); break;
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return failf(XQ_ERR_HIP, "fa_tree launch: %s", hipGetErrorString(e));
