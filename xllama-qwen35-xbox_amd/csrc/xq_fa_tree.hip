@@ -36,26 +36,29 @@ typedef uint16_t u16any __attribute__((aligned(1)));
 typedef uint32_t u4half __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f4el __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kTr = 64;                // KV rows of a tile: a lane per row
 constexpr float kTreeLog2e = 1.4426950408889634f, kTreeLn2 = 0.6931471805599453f;
 constexpr float kTreeLazy = 8.0f;      // base-2 headroom before the running maximum moves
-constexpr float kTreeOff = 4.0f;       // weights are 2^(x - max - 4), in (0, 16]
+constexpr float kTreeOff = -7.0f;      // weights are 2^(x - max + 7), in (0, 2^15]: f16 keeps small ones normal
 
-template <int KT, int D, bool NARROW, int MT, int WR>
+template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 struct TreeCfg {
     static constexpr bool QUANT = KT == XQ_TYPE_Q8_0 || KT == XQ_TYPE_Q4_0;
     static constexpr int PARTS = QUANT && !NARROW ? 2 : 1;                  // f16 parts of a cached value
     static constexpr int QP = NARROW ? 1 : 2;                               // f16 parts of Q and of the weights
     static constexpr int EL = KT == XQ_TYPE_F16 ? 8 : KT == XQ_TYPE_Q4_0 ? 32 : 16;  // elements of a 16-byte piece
     static constexpr int PPR = D / EL;                                      // pieces per row
-    static constexpr int NPT = kTr * PPR / 256;                             // pieces per thread and tensor
+    static constexpr int TR = WR == 1 ? 32 : 64;                            // KV rows of a tile (a lane per row)
+    static constexpr int RT = TR / 16 / WR;                                 // 16-row score tiles of a wave
+    static constexpr int PIECES = TR * PPR;                                 // of a tile and tensor
+    static constexpr int NPT = (PIECES + 64 * NW - 1) / (64 * NW);          // per thread
     static constexpr int RSK = 2 * D + 16, RSV = 2 * D + 32;                // image rows, bytes
-    static constexpr int KB = kTr * RSK, VB = kTr * RSV;                    // one part
+    static constexpr int KB = TR * RSK, VB = TR * RSV;                      // one part
     static constexpr int IMG = PARTS * (KB + VB);
-    static constexpr int PW = 16 * MT * (WR == 4 ? 1 : 4);                  // pairs of a workgroup
+    static constexpr int PW = 16 * MT * (NW / WR);                          // pairs of a workgroup
     static constexpr int MS = D + 4;                                        // merge row stride, floats
-    static constexpr int MERGE = WR == 4 ? 4 * 16 * MS * 4 : 0;
+    static constexpr int MERGE = WR > 1 ? NW * 16 * MS * 4 : 0;
     static constexpr int SMEM = IMG > MERGE ? IMG : MERGE;
+    static constexpr int WAVES = D == 256 || MT == 2 || PARTS == 2 ? 2 : 3;  // per SIMD, that the registers allow
 };
 
 // Element d of a record in f32 (rows with a non-finite value only).
@@ -147,13 +150,13 @@ struct SeqWork {
     int32_t held, n_tok, end;
     uint32_t tiles, ptiles, units;
 };
-template <int PW>
+template <int PW, int TR>
 XQ_DEV SeqWork seq_work(const TreeArgs& a, int b) {
     SeqWork s;
     s.held = min(max(a.pg.rows[b], 0), a.pg.row_limit);
     s.n_tok = a.n_tok ? min(max(a.n_tok[b], 0), a.n_q) : a.n_q;
     s.end = (int32_t)min((uint32_t)s.held + (uint32_t)s.n_tok, (uint32_t)a.pg.row_limit);
-    s.tiles = s.n_tok ? ((uint32_t)s.end + kTr - 1) / kTr : 0u;
+    s.tiles = s.n_tok ? ((uint32_t)s.end + TR - 1) / TR : 0u;
     s.ptiles = (uint32_t)(s.n_tok * a.G + PW - 1) / PW;
     s.units = s.tiles * s.ptiles * (uint32_t)a.pg.n_head_kv;
     return s;
@@ -184,33 +187,33 @@ XQ_DEV uint32_t wave_scan(uint32_t x) {  // inclusive, over the 64 lanes
 }
 XQ_DEV uint32_t lane_get(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
 
-template <int PW>
+template <int PW, int TR>
 XQ_DEV uint32_t all_units(const TreeArgs& a) {
     uint32_t total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int b = b0 + lane_id();
-        total += lane_get(wave_scan(b < a.B ? seq_work<PW>(a, b).units : 0u), 63);
+        total += lane_get(wave_scan(b < a.B ? seq_work<PW, TR>(a, b).units : 0u), 63);
     }
     return total;
 }
 
-template <int KT, int D, bool NARROW, int MT, int WR>
-__global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
-    using C = TreeCfg<KT, D, NARROW, MT, WR>;
-    constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW;
+template <int KT, int D, bool NARROW, int MT, int WR, int NW>
+__global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES)) void fa_tree_kernel(TreeArgs a) {
+    using C = TreeCfg<KT, D, NARROW, MT, WR, NW>;
+    constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW, TR = C::TR, RT = C::RT;
     constexpr bool QUANT = C::QUANT;
-    constexpr int RT = 4 / WR;              // 16-row score tiles of a wave
-    constexpr int GR = RT >= 2 ? 2 : 1;     // of them at a time
     __shared__ __attribute__((aligned(16))) uint8_t img[C::SMEM];
-    __shared__ float sM[4][16 * MT], sL[4][16 * MT];
-    __shared__ int sEk[PARTS == 2 ? kTr : 1], sEv[PARTS == 2 ? kTr : 1];
+    __shared__ float sM[WR > 1 ? NW : 1][16 * MT], sL[WR > 1 ? NW : 1][16 * MT];
+    __shared__ int sEk[PARTS == 2 ? TR : 1], sEv[PARTS == 2 ? TR : 1];
     __shared__ unsigned long long sBad[2];
     const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x, lr = lane & 15, lg = lane >> 4;
+    const int wr = wave % WR, pg = wave / WR;  // the wave's rows and pairs of a tile
+    const int row0 = 16 * RT * wr;             // its first row
     uint8_t* const imgK = img;
     uint8_t* const imgV = img + PARTS * C::KB;
 
     const uint32_t w = xcd_remap(blockIdx.x, a.d_wgs.d);
-    const Deal deal(all_units<PW>(a), a.d_wgs);
+    const Deal deal(all_units<PW, TR>(a), a.d_wgs);
     uint32_t u = deal.first(w);
     const uint32_t u_end = deal.first(w + 1);
     // the chunk of 64 sequences that holds unit u: lane l has sequence b0 + l
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
         uint32_t upto = 0;
         for (;;) {
             mine = SeqWork{};
-            if (b0 + lane < a.B) mine = seq_work<PW>(a, b0 + lane);
+            if (b0 + lane < a.B) mine = seq_work<PW, TR>(a, b0 + lane);
             upto = carry + wave_scan(mine.units);
             const uint32_t last = lane_get(upto, 63);
             if (u < last) break;
@@ -240,16 +243,16 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
         const uint32_t t_last = min(tiles, t_first + (u_end - u));
         const bool whole = t_first == 0 && t_last == tiles;
         const int n_pairs = n_tok * a.G;
-        const int p0 = pt * PW + (WR == 4 ? 0 : wave * 16 * MT);  // this wave's first pair
+        const int p0 = pt * PW + pg * 16 * MT;  // this wave's first pair
 
         const uint8_t* const kb = a.pg.k + hk * a.pg.k_head;
         const uint8_t* const vb = a.pg.v + hk * a.pg.v_head;
         // row lane of tile t: its page (~0u where there is none) and its place in it
         auto lookup = [&](uint32_t t, uint32_t& page, uint32_t& in) {
-            const uint32_t r = t * kTr + lane;
+            const uint32_t r = t * TR + lane;
             page = ~0u;
             in = 0;
-            if (t < t_last && r < (uint32_t)end) {
+            if (t < t_last && r < (uint32_t)end && (TR == 64 || lane < TR)) {
                 const uint32_t c = a.pg.d_page.quot(r);
                 page = (uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c];
                 in = r - c * a.pg.d_page.d;
@@ -260,12 +263,12 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
         auto fetch = [&](uint32_t page, uint32_t in) {
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
-                const int i = tid + 256 * j, r = i / PPR, c = i % PPR;
+                const int i = tid + 64 * NW * j, r = i / PPR % TR, c = i % PPR;
                 const uint32_t p = (uint32_t)__shfl((int)page, r), x = (uint32_t)__shfl((int)in, r);
                 rk[j] = u4t{0, 0, 0, 0};
                 rv[j] = u4t{0, 0, 0, 0};
                 if constexpr (QUANT) dk[j] = dv[j] = 0u;
-                if (p < (uint32_t)a.pg.n_pages) {
+                if (p < (uint32_t)a.pg.n_pages && (C::PIECES % (64 * NW) == 0 || i < C::PIECES)) {
                     const uint8_t* k = kb + p * a.pg.k_page + x * a.pg.k_row;
                     const uint8_t* v = vb + p * a.pg.v_page + x * a.pg.v_row;
                     constexpr int BB = KT == XQ_TYPE_Q8_0 ? 34 : 18;
@@ -282,13 +285,13 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
         };
         // raw pieces -> image
         auto put = [&](uint8_t* image, int rs, int part_bytes, const u4t raw, uint32_t d, int r, int c, int* exps, bool clean, uint32_t t) {
-            constexpr int NW = C::EL / 2;
-            uint32_t o[NW], lo[NW];
-            piece_f16<KT, NW>(raw, o);
+            constexpr int WORDS = C::EL / 2;
+            uint32_t o[WORDS], lo[WORDS];
+            piece_f16<KT, WORDS>(raw, o);
             if constexpr (QUANT && PARTS == 1) {
                 const uint32_t dd = d | (d << 16);
 #pragma unroll
-                for (int i = 0; i < NW; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, o[i]) * __builtin_bit_cast(h2t, dd));
+                for (int i = 0; i < WORDS; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, o[i]) * __builtin_bit_cast(h2t, dd));
             } else if constexpr (QUANT) {
                 // the row's power of two: its largest finite block scale to [2^7, 2^8)
                 int e = (int)((__float_as_uint(f16_bits_to_f32(d)) >> 23) & 255u);
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
                 const float f = ldexpf(f16_bits_to_f32(d), -e);
                 if (c == 0) exps[r] = e;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) {
+                for (int i = 0; i < WORDS; ++i) {
                     const h2t q = __builtin_bit_cast(h2t, o[i]);
                     const float x = (float)q[0] * f, y = (float)q[1] * f;
                     const h2t hi = {(_Float16)x, (_Float16)y};
@@ -311,7 +314,7 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
             if (clean) {
                 uint32_t bad = 0;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) {
+                for (int i = 0; i < WORDS; ++i) {
                     bad |= bad_halves(o[i]);
                     if constexpr (PARTS == 2) lo[i] &= ~((bad_halves(o[i]) >> 15) * 0xffffu);
                     o[i] = without_bad(o[i]);
@@ -320,16 +323,17 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
             }
             uint8_t* y = image + r * rs + c * (2 * C::EL);
 #pragma unroll
-            for (int i = 0; i < NW; i += 4) {
+            for (int i = 0; i < WORDS; i += 4) {
                 *(u4t*)(y + 4 * i) = u4t{o[i], o[i + 1], o[i + 2], o[i + 3]};
                 if constexpr (PARTS == 2) *(u4t*)(y + part_bytes + 4 * i) = u4t{lo[i], lo[i + 1], lo[i + 2], lo[i + 3]};
             }
         };
         auto commit = [&](uint32_t t) {
-            const bool clean = (t + 1) * kTr > (uint32_t)held;  // holds rows that only some tokens see
+            const bool clean = (t + 1) * TR > (uint32_t)held;  // holds rows that only some tokens see
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
-                const int i = tid + 256 * j, r = i / PPR, c = i % PPR;
+                const int i = tid + 64 * NW * j, r = i / PPR, c = i % PPR;
+                if (C::PIECES % (64 * NW) && i >= C::PIECES) break;  // (whole waves: PIECES is a multiple of 64)
                 put(imgK, C::RSK, C::KB, rk[j], QUANT ? dk[j] : 0u, r, c, sEk, false, t);
                 put(imgV, C::RSV, C::VB, rv[j], QUANT ? dv[j] : 0u, r, c, sEv, clean, t);
             }
@@ -380,12 +384,13 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(xq[m][c][j]));
                 const int lift = 141 - min((int)(__float_as_uint(across_rows_max(big)) >> 23), 254);
-                qf[m] = ldexpf(a.scale * kTreeLog2e, -lift);
+                // (not below the smallest normal: an unseen score's -inf stays one)
+                qf[m] = fmaxf(ldexpf(fabsf(a.scale) * kTreeLog2e, -lift), 1.17549435e-38f);
 #pragma unroll
                 for (int c = 0; c < NB; ++c)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float x = ldexpf(xq[m][c][j], lift);
+                        const float x = ldexpf(a.scale < 0.0f ? -xq[m][c][j] : xq[m][c][j], lift);
                         const _Float16 hi = (_Float16)x;
                         qo[m][c][0][j] = hi;
                         if constexpr (QP == 2) qo[m][c][1][j] = (_Float16)(x - (float)hi);
@@ -420,13 +425,13 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
             if (tid == 0) sBad[(t + 1) & 1] = 0;
 
             // which of the tile's rows each pair sees
-            const bool careful = (t + 1) * kTr > (uint32_t)held || now != ~0ull;
+            const bool careful = (t + 1) * TR > (uint32_t)held || now != ~0ull >> (64 - TR);
             uint64_t sees[MT];
             if (careful) {
                 // ancestors by doubling: lane i is token i
-                const int first = (int)(t * kTr);
+                const int first = (int)(t * TR);
                 uint64_t anc = 0;
-                if (first + kTr > held) {
+                if (first + TR > held) {
                     int32_t p = up >= 0 && up < lane ? up : -1;
                     anc = 1ull << lane;
 #pragma unroll
@@ -447,7 +452,7 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
                 }
             }
             if constexpr (PARTS == 2) {
-                int e = sEv[lane];
+                int e = sEv[lane % TR];
 #pragma unroll
                 for (int s = 1; s < 64; s *= 2) e = max(e, __shfl_xor(e, s));
                 e = __builtin_amdgcn_readfirstlane(e);
@@ -460,116 +465,129 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
                     e_run = e;
                 }
             }
+            f4t s[MT][RT];
 #pragma unroll
-            for (int g = 0; g < RT / GR; ++g) {
-                const int row0 = WR == 4 ? 16 * wave : 32 * g;
-                f4t s[MT][GR];
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) s[m][r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < NB; ++c)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const uint8_t* k = imgK + (row0 + 16 * r + lr) * C::RSK + 64 * c + 16 * lg;
+                    const h8t kh = *(const h8t*)k;
+                    h8t kl;
+                    if constexpr (PARTS == 2) kl = *(const h8t*)(k + C::KB);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][0], s[m][r], 0, 0, 0);
+                        if constexpr (QP == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][1], s[m][r], 0, 0, 0);
+                        if constexpr (PARTS == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qo[m][c][0], s[m][r], 0, 0, 0);
+                    }
+                }
+            products_done();
+            // the lane's rows are row0 + 16r + 4lg + i; s * qf are base-2 scores
+            if constexpr (PARTS == 2) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const int4 e = *(const int4*)(sEk + row0 + 16 * r + 4 * lg);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                        s[m][r] = f4t{ldexpf(s[m][r][0], e.x), ldexpf(s[m][r][1], e.y), ldexpf(s[m][r][2], e.z), ldexpf(s[m][r][3], e.w)};
+                }
+            }
+            if (careful) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int r = 0; r < GR; ++r) s[m][r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int r = 0; r < RT; ++r) {
+                        const uint32_t bits = (uint32_t)(sees[m] >> (row0 + 16 * r + 4 * lg));
 #pragma unroll
-                for (int c = 0; c < NB; ++c)
-#pragma unroll
-                    for (int r = 0; r < GR; ++r) {
-                        const uint8_t* k = imgK + (row0 + 16 * r + lr) * C::RSK + 64 * c + 16 * lg;
-                        const h8t kh = *(const h8t*)k;
-                        h8t kl;
-                        if constexpr (PARTS == 2) kl = *(const h8t*)(k + C::KB);
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][0], s[m][r], 0, 0, 0);
-                            if constexpr (QP == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][1], s[m][r], 0, 0, 0);
-                            if constexpr (PARTS == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qo[m][c][0], s[m][r], 0, 0, 0);
-                        }
+                        for (int i = 0; i < 4; ++i) s[m][r][i] = (bits >> i) & 1u ? s[m][r][i] : -INFINITY;
                     }
-                products_done();
-                // base-2 scores; the lane's rows are row0 + 16r + 4lg + i
-                bool over = false;
-                float top[MT];
+            }
+            bool over = false;
+            float top[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                top[m] = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[m] = fmaxf(top[m], s[m][r][i]);
+                top[m] *= qf[m];
+                over |= top[m] > m_run[m] + kTreeLazy;
+            }
+            if (__builtin_amdgcn_ballot_w64(over)) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    top[m] = -INFINITY;
+                    const float mt = across_rows_max(top[m]);
+                    const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) : m_run[m];
+                    const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
+                    l_run[m] *= f;
 #pragma unroll
-                    for (int r = 0; r < GR; ++r) {
-                        s[m][r] *= qf[m];
-                        if constexpr (PARTS == 2) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[m][r][i] = ldexpf(s[m][r][i], sEk[row0 + 16 * r + 4 * lg + i]);
-                        }
-                        if (careful) {
-                            const uint32_t bits = (uint32_t)(sees[m] >> (row0 + 16 * r + 4 * lg));
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[m][r][i] = (bits >> i) & 1u ? s[m][r][i] : -INFINITY;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top[m] = fmaxf(top[m], s[m][r][i]);
-                    }
-                    over |= top[m] > m_run[m] + kTreeLazy;
+                    for (int n = 0; n < ND; ++n) acc[m][n] *= f;
+                    m_run[m] = mn;
                 }
-                if (__builtin_amdgcn_ballot_w64(over)) {
+            }
+            // weights
+            h4t ph[MT][RT], pl[QP == 2 ? MT : 1][QP == 2 ? RT : 1];
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const float mt = across_rows_max(top[m]);
-                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) : m_run[m];
-                        const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
-                        l_run[m] *= f;
+            for (int m = 0; m < MT; ++m) {
+                const float mu = m_run[m] == -INFINITY ? 0.0f : -(m_run[m] + kTreeOff);
 #pragma unroll
-                        for (int n = 0; n < ND; ++n) acc[m][n] *= f;
-                        m_run[m] = mn;
+                for (int r = 0; r < RT; ++r) {
+                    f4t p;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[i] = __builtin_amdgcn_exp2f(fmaf(s[m][r][i], qf[m], mu));
+                        l_run[m] += p[i];
+                    }
+                    if constexpr (PARTS == 2) {
+                        const int4 e = *(const int4*)(sEv + row0 + 16 * r + 4 * lg);
+                        p = f4t{ldexpf(p[0], e.x - e_run), ldexpf(p[1], e.y - e_run), ldexpf(p[2], e.z - e_run), ldexpf(p[3], e.w - e_run)};
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ph[m][r][i] = (_Float16)p[i];
+                        if constexpr (QP == 2) pl[m][r][i] = (_Float16)(p[i] - (float)ph[m][r][i]);
                     }
                 }
-                // weights
-                h4t ph[MT][GR], pl[QP == 2 ? MT : 1][QP == 2 ? GR : 1];
+            }
+            // O^T += V^T P^T
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const uint8_t* v = imgV + (row0 + 4 * lg + (lr >> 2)) * C::RSV + 32 * n + 8 * (lr & 3);
+                h4t vh[RT], vl[PARTS == 2 ? RT : 1];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    vh[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV));
+                    if constexpr (PARTS == 2) vl[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV + C::VB));
+                }
+                auto product = [&](const h4t (&x)[RT], const h4t (&p)[RT], f4t& o) {
+                    if constexpr (RT == 2)
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(x[0], x[RT - 1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                  __builtin_shufflevector(p[0], p[RT - 1], 0, 1, 2, 3, 4, 5, 6, 7), o, 0, 0, 0);
+                    else
+                        o = __builtin_amdgcn_mfma_f32_16x16x16f16(x[0], p[0], o, 0, 0, 0);
+                };
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const float mu = m_run[m] == -INFINITY ? 0.0f : m_run[m] + kTreeOff;
-#pragma unroll
-                    for (int r = 0; r < GR; ++r)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float p = __builtin_amdgcn_exp2f(s[m][r][i] - mu);
-                            l_run[m] += p;
-                            if constexpr (PARTS == 2) p *= ldexpf(1.0f, sEv[row0 + 16 * r + 4 * lg + i] - e_run);
-                            ph[m][r][i] = (_Float16)p;
-                            if constexpr (QP == 2) pl[m][r][i] = (_Float16)(p - (float)ph[m][r][i]);
-                        }
-                }
-                // O^T += V^T P^T
-#pragma unroll
-                for (int n = 0; n < ND; ++n) {
-                    const uint8_t* v = imgV + (row0 + 4 * lg + (lr >> 2)) * C::RSV + 32 * n + 8 * (lr & 3);
-                    h4t vh[GR], vl[PARTS == 2 ? GR : 1];
-#pragma unroll
-                    for (int r = 0; r < GR; ++r) {
-                        vh[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV));
-                        if constexpr (PARTS == 2) vl[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV + C::VB));
-                    }
-                    auto product = [&](const h4t (&x)[GR], const h4t (&p)[GR], f4t& o) {
-                        if constexpr (GR == 2)
-                            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(x[0], x[GR - 1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                                                      __builtin_shufflevector(p[0], p[GR - 1], 0, 1, 2, 3, 4, 5, 6, 7), o, 0, 0, 0);
-                        else
-                            o = __builtin_amdgcn_mfma_f32_16x16x16f16(x[0], p[0], o, 0, 0, 0);
-                    };
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        product(vh, ph[m], acc[m][n]);
-                        if constexpr (QP == 2) product(vh, pl[m], acc[m][n]);
-                        if constexpr (PARTS == 2) product(vl, ph[m], acc[m][n]);
-                    }
+                    product(vh, ph[m], acc[m][n]);
+                    if constexpr (QP == 2) product(vh, pl[m], acc[m][n]);
+                    if constexpr (PARTS == 2) product(vl, ph[m], acc[m][n]);
                 }
             }
             products_done();
             // non-finite values of rows that not every token sees: to the tokens that do
             if (careful) {
                 uint64_t bad = sBad[t & 1];
-                if constexpr (WR == 4) bad &= 0xffffull << (16 * wave);
+                if constexpr (WR > 1) bad &= (~0ull >> (64 - 16 * RT)) << row0;
                 bad = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(bad >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)bad);
                 while (bad) {
                     const int r = __builtin_ctzll(bad);
                     bad &= bad - 1;
-                    const uint32_t row = t * kTr + r, c = a.pg.d_page.quot(row);
+                    const uint32_t row = t * TR + r, c = a.pg.d_page.quot(row);
                     const uint8_t* v = vb + (uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c] * a.pg.v_page + (row - c * a.pg.d_page.d) * a.pg.v_row;
 #pragma unroll 1
                     for (int d = 0; d < D; d += 16)
@@ -618,7 +636,7 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
                 if (first) a.part_ml[at] = make_float2(mm, l);
             }
         };
-        if constexpr (WR == 4) {
+        if constexpr (WR > 1) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 l_run[m] = across_rows_sum(l_run[m]);
@@ -631,23 +649,31 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
             float* const mg = (float*)img;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const float top = fmaxf(fmaxf(sM[0][16 * m + lr], sM[1][16 * m + lr]), fmaxf(sM[2][16 * m + lr], sM[3][16 * m + lr]));
+                // the waves of a pair group bring their sums to their largest maximum
+                auto largest = [&](int first, int q) {
+                    float x = sM[first][q];
+#pragma unroll
+                    for (int i = 1; i < WR; ++i) x = fmaxf(x, sM[first + i][q]);
+                    return x;
+                };
+                const float top = largest(pg * WR, 16 * m + lr);
                 const float f = m_run[m] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[m] - top);
 #pragma unroll
                 for (int n = 0; n < ND; ++n) *(f4t*)(mg + (16 * wave + lr) * C::MS + 16 * n + 4 * lg) = acc[m][n] * f;
                 __syncthreads();
-                for (int i = tid; i < 16 * D / 4; i += 256) {
-                    const int p = i / (D / 4), d = 4 * (i % (D / 4)), q = 16 * m + p;
-                    if (pt * PW + q < n_pairs) {
-                        const float mm = fmaxf(fmaxf(sM[0][q], sM[1][q]), fmaxf(sM[2][q], sM[3][q]));
+                for (int i = tid; i < NW / WR * 16 * D / 4; i += 64 * NW) {
+                    const int g = i / (16 * D / 4), p = i / (D / 4) % 16, d = 4 * (i % (D / 4)), q = 16 * m + p;
+                    const int pair = g * 16 * MT + q;
+                    if (pt * PW + pair < n_pairs) {
+                        const float mm = largest(g * WR, q);
                         float l = 0.0f;
                         f4t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
+                        for (int x = g * WR; x < g * WR + WR; ++x) {
                             if (sM[x][q] != -INFINITY) l = fmaf(sL[x][q], __builtin_amdgcn_exp2f(sM[x][q] - mm), l);
                             o += *(const f4t*)(mg + (16 * x + p) * C::MS + d);
                         }
-                        emit(q, d, o, mm, l, d == 0);
+                        emit(pair, d, o, mm, l, d == 0);
                     }
                 }
                 __syncthreads();
@@ -668,17 +694,17 @@ __global__ __launch_bounds__(256) void fa_tree_kernel(TreeArgs a) {
 
 // Joins the parts of the segments that more than one workgroup had: one wave per
 // (sequence, token, head), lane p the p-th part's maximum and sum, then all lanes the dims.
-template <int D, bool NARROW, int PW>
+template <int D, bool NARROW, int PW, int TR>
 __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
     const int lane = lane_id();
     const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
     if (row >= (int64_t)a.B * a.n_q * a.H) return;
     const int h = (int)(row % a.H), t = (int)(row / a.H % a.n_q), b = (int)(row / a.H / a.n_q);
-    const SeqWork s = seq_work<PW>(a, b);
+    const SeqWork s = seq_work<PW, TR>(a, b);
     if (t >= s.n_tok) return;
     uint32_t before = 0, total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const uint32_t x = wave_scan(b0 + lane < a.B ? seq_work<PW>(a, b0 + lane).units : 0u);
+        const uint32_t x = wave_scan(b0 + lane < a.B ? seq_work<PW, TR>(a, b0 + lane).units : 0u);
         if (b > b0) before = total + lane_get(x, min(b - b0, 64) - 1);
         total += lane_get(x, 63);
     }
@@ -753,29 +779,43 @@ static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const 
 
 // The kernel variant, workgroups and workspace of a call: of its shapes alone.
 struct TreePlan {
-    int wr, mt, pw;           // waves over the rows (4) or over the pairs (1), pair tiles per wave, pairs of a workgroup
+    int form;                 // index into the forms below
+    int pw, tr;               // pairs of a workgroup, KV rows of a tile
     uint32_t wgs;
     int32_t max_ptiles, part_pairs;
     int64_t parts;
     size_t ml_at, bytes;
 };
+// Forms by the pairs (tokens x group) of a KV head: up to 16, 32: the waves share the rows;
+// above: they share the pairs, up to 64, 128, 256 of a workgroup.
+template <int MT_, int WR_, int NW_> struct TreeForm { static constexpr int MT = MT_, WR = WR_, NW = NW_; };
+template <int D, bool NARROW, typename F>
+static void tree_form(int form, F f) {
+    switch (form) {
+    case 0: f(TreeForm<1, 4, 4>{}); break;
+    case 1: f(TreeForm<1, 2, 4>{}); break;
+    case 2: f(TreeForm<1, 1, 4>{}); break;
+    case 3:
+        if constexpr (D == 128) f(TreeForm<2, 1, 4>{});
+        else f(TreeForm<1, 1, 8>{});
+        break;
+    default:
+        if constexpr (D == 128) f(TreeForm<2, 1, 8>{});
+        break;
+    }
+}
 static TreePlan tree_plan(const xq_tensor* q, const xq_kv_pages* c) {
     TreePlan P{};
     const int64_t D = q->ne[0], Hkv = c->k.ne[2], B = q->ne[3], pairs = q->ne[1] * (q->ne[2] / Hkv);
-    const bool narrow = q->type == XQ_TYPE_BF16;
-    const int most = narrow ? (D == 128 ? 4 : 2) : (D == 128 ? 2 : 1);
-    if (pairs <= 16) P.wr = 4, P.mt = 1;
-    else if (pairs <= 32) P.wr = 4, P.mt = 2;
-    else if (pairs <= 64 || most == 1) P.wr = 1, P.mt = 1;
-    else if (pairs <= 128 || most == 2) P.wr = 1, P.mt = 2;
-    else P.wr = 1, P.mt = 4;
-    P.pw = 16 * P.mt * (P.wr == 4 ? 1 : 4);
+    P.form = pairs <= 16 ? 0 : pairs <= 32 ? 1 : pairs <= 64 ? 2 : pairs <= 128 || D == 256 ? 3 : 4;
+    P.pw = 16 << P.form;
+    P.tr = P.form < 2 ? 64 : 32;
     P.max_ptiles = (int32_t)cdiv(pairs, P.pw);
     P.part_pairs = (int32_t)(pairs < P.pw ? pairs : P.pw);
     const int64_t segs = B * Hkv * P.max_ptiles;
     // tiles that the table could hold, at most
-    const int64_t tiles = cdiv((int64_t)c->table_cols * c->k.ne[1], kTr) * segs;
-    int64_t wgs = P.wr == 4 ? 1024 : 512;
+    const int64_t tiles = cdiv((int64_t)c->table_cols * c->k.ne[1], P.tr) * segs;
+    int64_t wgs = P.form < 2 ? 1024 : 512;
     if (wgs > tiles) wgs = tiles;
     P.wgs = (uint32_t)wgs;
     P.parts = wgs + segs;
@@ -787,22 +827,13 @@ static TreePlan tree_plan(const xq_tensor* q, const xq_kv_pages* c) {
 
 template <int KT, int D, bool NARROW>
 static void tree_launch(const TreePlan& P, const TreeArgs& a, hipStream_t s) {
-    const dim3 grid(P.wgs), block(256), rows((uint32_t)cdiv((int64_t)a.B * a.n_q * a.H, 4));
-    auto go = [&](auto mt_tag, auto wr_tag) {
-        constexpr int MT = decltype(mt_tag)::value, WR = decltype(wr_tag)::value;
-        launch("fa_tree", fa_tree_kernel<KT, D, NARROW, MT, WR>, grid, block, s, a);
-        launch("fa_tree_join", fa_tree_join<D, NARROW, TreeCfg<KT, D, NARROW, MT, WR>::PW>, rows, block, s, a);
-    };
-    std::integral_constant<int, 1> one;
-    std::integral_constant<int, 2> two;
-    std::integral_constant<int, 4> four;
-    if (P.wr == 4 && P.mt == 1) go(one, four);
-    else if (P.wr == 4) go(two, four);
-    else if (P.mt == 1) go(one, one);
-    else if constexpr (NARROW || D == 128) {
-        if (P.mt == 2) go(two, one);
-        else if constexpr (NARROW && D == 128) go(four, one);
-    }
+    const dim3 grid(P.wgs), rows((uint32_t)cdiv((int64_t)a.B * a.n_q * a.H, 4));
+    tree_form<D, NARROW>(P.form, [&](auto form) {
+        using F = decltype(form);
+        using C = TreeCfg<KT, D, NARROW, F::MT, F::WR, F::NW>;
+        launch("fa_tree", fa_tree_kernel<KT, D, NARROW, F::MT, F::WR, F::NW>, grid, dim3(64 * F::NW), s, a);
+        launch("fa_tree_join", fa_tree_join<D, NARROW, C::PW, C::TR>, rows, dim3(256), s, a);
+    });
 }
 
 template <int KT>
