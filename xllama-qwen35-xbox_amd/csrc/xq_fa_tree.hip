@@ -19,7 +19,9 @@ struct TreeArgs {
     const int32_t* n_tok;
     int32_t n_q, H, G, B;
     float scale;
-    UDivFlat d_g, d_wgs;      // by the group; by the workgroups
+    uint32_t k_page, k_row, v_page, v_row;  // strides, below 2^32
+    UDivFlat d_g, d_wgs, d_h, d_q;  // by the group, the workgroups, the heads, the tokens
+    uint32_t least;           // tiles that a workgroup takes at least
     int32_t max_ptiles;       // pair tiles of a sequence with n_q tokens
     int32_t part_pairs;       // pairs of a part
     float* part_o;            // [parts][part_pairs][D]
@@ -47,18 +49,24 @@ struct TreeCfg {
     static constexpr int QP = NARROW ? 1 : 2;                               // f16 parts of Q and of the weights
     static constexpr int EL = KT == XQ_TYPE_F16 ? 8 : KT == XQ_TYPE_Q4_0 ? 32 : 16;  // elements of a 16-byte piece
     static constexpr int PPR = D / EL;                                      // pieces per row
-    static constexpr int TR = WR == 1 ? 32 : 64;                            // KV rows of a tile (a lane per row)
-    static constexpr int RT = TR / 16 / WR;                                 // 16-row score tiles of a wave
+    static constexpr int TR = 64;                                           // KV rows of a tile (a lane per row)
+    static constexpr int RW = TR / WR;                                      // of a wave
+    static constexpr int RT = RW >= 32 ? 2 : 1;                             // 16-row score tiles of a wave at a time
     static constexpr int PIECES = TR * PPR;                                 // of a tile and tensor
     static constexpr int NPT = (PIECES + 64 * NW - 1) / (64 * NW);          // per thread
-    static constexpr int RSK = 2 * D + 16, RSV = 2 * D + 32;                // image rows, bytes
-    static constexpr int KB = TR * RSK, VB = TR * RSV;                      // one part
-    static constexpr int IMG = PARTS * (KB + VB);
+    static constexpr int RS = 2 * D + 32;                                   // image rows, bytes: 8 banks of 64 apart
+    static constexpr int PB = TR * RS;                                      // one part of K or V
+    static constexpr int IMG = 2 * PARTS * PB;
     static constexpr int PW = 16 * MT * (NW / WR);                          // pairs of a workgroup
     static constexpr int MS = D + 4;                                        // merge row stride, floats
     static constexpr int MERGE = WR > 1 ? NW * 16 * MS * 4 : 0;
     static constexpr int SMEM = IMG > MERGE ? IMG : MERGE;
+    // tiles whose loads are in flight while one is computed: two where their registers allow it
+    static constexpr int DEPTH = NPT * 2 * (QUANT ? 5 : 4) <= 20 ? 2 : 1;
     static constexpr int WAVES = D == 256 || MT == 2 || PARTS == 2 ? 2 : 3;  // per SIMD, that the registers allow
+    // workgroups that a CU holds
+    static constexpr int BY_LDS = 160 * 1024 / (SMEM + 2048), BY_WAVES = WAVES * 4 / NW;
+    static constexpr int PER_CU = BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES;
 };
 
 // Element d of a record in f32 (rows with a non-finite value only).
@@ -162,84 +170,94 @@ XQ_DEV SeqWork seq_work(const TreeArgs& a, int b) {
     return s;
 }
 
-// The units of all sequences dealt to the workgroups in order, as evenly as they go.
+// A number that every lane has, in a scalar register: what is formed from it stays scalar.
+XQ_DEV uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+
+// The units of all sequences dealt to the workgroups in order, `per` each.
 struct Deal {
-    uint32_t per, more;  // units per workgroup; the first `more` have one more
-    XQ_DEV Deal(uint32_t units, const UDivFlat& d_wgs) {
-        per = d_wgs.quot(units);
-        more = units - per * d_wgs.d;
-    }
-    XQ_DEV uint32_t first(uint32_t w) const { return w * per + min(w, more); }
-    XQ_DEV uint32_t owner(uint32_t u) const {  // the workgroup that has unit u
-        const uint32_t big = more * (per + 1);
-        return u < big ? u / (per + 1) : more + (u - big) / per;
-    }
+    uint32_t units, per;
+    XQ_DEV Deal(uint32_t n, const UDivFlat& d_wgs, uint32_t least) : units(n), per(uniform(max(d_wgs.quot(n + d_wgs.d - 1), least))) {}
+    XQ_DEV uint32_t first(uint32_t w) const { return uniform((uint32_t)min((uint64_t)w * per, (uint64_t)units)); }
+    XQ_DEV uint32_t owner(uint32_t u) const { return u / per; }  // the workgroup that has unit u
 };
 
-XQ_DEV uint32_t wave_scan(uint32_t x) {  // inclusive, over the 64 lanes
-    const int lane = lane_id();
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t y = __shfl_up(x, d);
-        x += lane >= d ? y : 0u;
-    }
-    return x;
+// Inclusive sum over the 64 lanes: inside rows of 16, then from row to row.
+template <int CTRL, int ROWS>
+XQ_DEV uint32_t dpp_add(uint32_t x) {
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+XQ_DEV uint32_t wave_scan(uint32_t x) {
+    x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3
+    return dpp_add<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
 }
 XQ_DEV uint32_t lane_get(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
 
+// 64 sequences at a time, a lane each: their work and the units up to and with each.
 template <int PW, int TR>
-XQ_DEV uint32_t all_units(const TreeArgs& a) {
-    uint32_t total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int b = b0 + lane_id();
-        total += lane_get(wave_scan(b < a.B ? seq_work<PW, TR>(a, b).units : 0u), 63);
+struct SeqChunk {
+    int b0;
+    uint32_t before, upto;  // units of the sequences before b0; up to this lane's
+    SeqWork mine;
+    XQ_DEV void load(const TreeArgs& a, int first, uint32_t units_before) {
+        b0 = first;
+        before = units_before;
+        mine = SeqWork{};
+        if (b0 + lane_id() < a.B) mine = seq_work<PW, TR>(a, b0 + lane_id());
+        upto = before + wave_scan(mine.units);
     }
-    return total;
-}
+    XQ_DEV uint32_t last() const { return lane_get(upto, 63); }
+    // All sequences' units; the first chunk is loaded after it.
+    XQ_DEV uint32_t total(const TreeArgs& a) {
+        load(a, 0, 0);
+        uint32_t n = last();
+        if (a.B > 64) {
+            while (b0 + 64 < a.B) {
+                load(a, b0 + 64, n);
+                n = last();
+            }
+            load(a, 0, 0);
+        }
+        return uniform(n);
+    }
+};
 
 template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES)) void fa_tree_kernel(TreeArgs a) {
     using C = TreeCfg<KT, D, NARROW, MT, WR, NW>;
     constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW, TR = C::TR, RT = C::RT;
     constexpr bool QUANT = C::QUANT;
+    constexpr int KC = PARTS == 2 ? 2 : 4;  // 32-element chunks of K read at once
+    constexpr int VC = PARTS == 2 ? 4 : 8;  // 16-element columns of V
     __shared__ __attribute__((aligned(16))) uint8_t img[C::SMEM];
     __shared__ float sM[WR > 1 ? NW : 1][16 * MT], sL[WR > 1 ? NW : 1][16 * MT];
     __shared__ int sEk[PARTS == 2 ? TR : 1], sEv[PARTS == 2 ? TR : 1];
     __shared__ unsigned long long sBad[2];
     const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x, lr = lane & 15, lg = lane >> 4;
     const int wr = wave % WR, pg = wave / WR;  // the wave's rows and pairs of a tile
-    const int row0 = 16 * RT * wr;             // its first row
+    const int r0 = tid / PPR, c0 = tid % PPR;  // row and piece of a tile that this thread brings (64 NW / PPR rows apart)
     uint8_t* const imgK = img;
-    uint8_t* const imgV = img + PARTS * C::KB;
+    uint8_t* const imgV = img + PARTS * C::PB;
 
     const uint32_t w = xcd_remap(blockIdx.x, a.d_wgs.d);
-    const Deal deal(all_units<PW, TR>(a), a.d_wgs);
+    SeqChunk<PW, TR> seqs;
+    const Deal deal(seqs.total(a), a.d_wgs, a.least);
     uint32_t u = deal.first(w);
     const uint32_t u_end = deal.first(w + 1);
-    // the chunk of 64 sequences that holds unit u: lane l has sequence b0 + l
-    int b0 = 0;
-    uint32_t carry = 0;
     while (u < u_end) {
         // ---- the segment (sequence, KV head, pair tile) that unit u belongs to
-        SeqWork mine{};
-        uint32_t upto = 0;
-        for (;;) {
-            mine = SeqWork{};
-            if (b0 + lane < a.B) mine = seq_work<PW, TR>(a, b0 + lane);
-            upto = carry + wave_scan(mine.units);
-            const uint32_t last = lane_get(upto, 63);
-            if (u < last) break;
-            carry = last;
-            b0 += 64;
-        }
-        const int sl = __builtin_ctzll(__builtin_amdgcn_ballot_w64(u < upto));
-        const int b = b0 + sl;
-        const int held = (int)lane_get((uint32_t)mine.held, sl), n_tok = (int)lane_get((uint32_t)mine.n_tok, sl);
-        const int end = (int)lane_get((uint32_t)mine.end, sl);
-        const uint32_t tiles = lane_get(mine.tiles, sl), ptiles = lane_get(mine.ptiles, sl);
-        const uint32_t in_b = u - (lane_get(upto, sl) - lane_get(mine.units, sl));
-        const uint32_t seg = in_b / tiles, t_first = in_b - seg * tiles;
-        const int hk = (int)(seg / ptiles), pt = (int)(seg - (uint32_t)hk * ptiles);
+        while (u >= seqs.last()) seqs.load(a, seqs.b0 + 64, seqs.last());
+        const int sl = __builtin_ctzll(__builtin_amdgcn_ballot_w64(u < seqs.upto));
+        const int b = seqs.b0 + sl;
+        const int held = (int)lane_get((uint32_t)seqs.mine.held, sl), n_tok = (int)lane_get((uint32_t)seqs.mine.n_tok, sl);
+        const int end = (int)lane_get((uint32_t)seqs.mine.end, sl);
+        const uint32_t tiles = lane_get(seqs.mine.tiles, sl), ptiles = lane_get(seqs.mine.ptiles, sl);
+        const uint32_t in_b = u - (lane_get(seqs.upto, sl) - lane_get(seqs.mine.units, sl));
+        const uint32_t seg = uniform(in_b / tiles), t_first = in_b - seg * tiles;
+        const int hk = (int)uniform(seg / ptiles), pt = (int)(seg - (uint32_t)hk * ptiles);
         const uint32_t t_last = min(tiles, t_first + (u_end - u));
         const bool whole = t_first == 0 && t_last == tiles;
         const int n_pairs = n_tok * a.G;
@@ -258,27 +276,30 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 in = r - c * a.pg.d_page.d;
             }
         };
-        u4t rk[NPT], rv[NPT];
-        uint32_t dk[QUANT ? NPT : 1], dv[QUANT ? NPT : 1];
-        auto fetch = [&](uint32_t page, uint32_t in) {
+        struct Raw {
+            u4t k[NPT], v[NPT];
+            uint32_t dk[QUANT ? NPT : 1], dv[QUANT ? NPT : 1];
+        };
+        Raw raw[C::DEPTH];
+        auto fetch = [&](Raw& set, uint32_t page, uint32_t in) {
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
-                const int i = tid + 64 * NW * j, r = i / PPR % TR, c = i % PPR;
+                const int r = (r0 + 64 * NW / PPR * j) % TR;
                 const uint32_t p = (uint32_t)__shfl((int)page, r), x = (uint32_t)__shfl((int)in, r);
-                rk[j] = u4t{0, 0, 0, 0};
-                rv[j] = u4t{0, 0, 0, 0};
-                if constexpr (QUANT) dk[j] = dv[j] = 0u;
-                if (p < (uint32_t)a.pg.n_pages && (C::PIECES % (64 * NW) == 0 || i < C::PIECES)) {
-                    const uint8_t* k = kb + p * a.pg.k_page + x * a.pg.k_row;
-                    const uint8_t* v = vb + p * a.pg.v_page + x * a.pg.v_row;
+                set.k[j] = u4t{0, 0, 0, 0};
+                set.v[j] = u4t{0, 0, 0, 0};
+                if constexpr (QUANT) set.dk[j] = set.dv[j] = 0u;
+                if (p < (uint32_t)a.pg.n_pages && (C::PIECES % (64 * NW) == 0 || tid + 64 * NW * j < C::PIECES)) {
+                    const uint8_t* k = kb + (uint64_t)p * a.k_page + (uint64_t)x * a.k_row;
+                    const uint8_t* v = vb + (uint64_t)p * a.v_page + (uint64_t)x * a.v_row;
                     constexpr int BB = KT == XQ_TYPE_Q8_0 ? 34 : 18;
-                    const int blk = KT == XQ_TYPE_Q8_0 ? c / 2 : c;
-                    const int at = QUANT ? blk * BB + 2 + (KT == XQ_TYPE_Q8_0 ? c % 2 * 16 : 0) : 16 * c;
-                    rk[j] = *(const u4any*)(k + at);
-                    rv[j] = *(const u4any*)(v + at);
+                    const int blk = KT == XQ_TYPE_Q8_0 ? c0 / 2 : c0;
+                    const int at = QUANT ? blk * BB + 2 + (KT == XQ_TYPE_Q8_0 ? c0 % 2 * 16 : 0) : 16 * c0;
+                    set.k[j] = *(const u4any*)(k + at);
+                    set.v[j] = *(const u4any*)(v + at);
                     if constexpr (QUANT) {
-                        dk[j] = *(const u16any*)(k + blk * BB);
-                        dv[j] = *(const u16any*)(v + blk * BB);
+                        set.dk[j] = *(const u16any*)(k + blk * BB);
+                        set.dv[j] = *(const u16any*)(v + blk * BB);
                     }
                 }
             }
@@ -293,22 +314,25 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, o[i]) * __builtin_bit_cast(h2t, dd));
             } else if constexpr (QUANT) {
-                // the row's power of two: its largest finite block scale to [2^7, 2^8)
-                int e = (int)((__float_as_uint(f16_bits_to_f32(d)) >> 23) & 255u);
+                // the row's power of two: its largest finite block scale to [2^7, 2^8), over the
+                // row's PPR (4, 8 or 16) lanes. Then d q = hi + lo exactly: hi its rounding, lo
+                // the remainder of at most 8 bits
+                const float df = f16_bits_to_f32(d);
+                int e = (int)((__float_as_uint(df) >> 23) & 255u);
                 if (e == 255 || e == 0) e = 1;
-#pragma unroll
-                for (int s = 1; s < PPR; s *= 2) e = max(e, __shfl_xor(e, s));
+                e = max(e, dpp_i<0xB1>(e));
+                e = max(e, dpp_i<0x4E>(e));
+                if constexpr (PPR >= 8) e = max(e, dpp_i<0x141>(e));
+                if constexpr (PPR >= 16) e = max(e, dpp_i<0x140>(e));
                 e -= 127 + 7;
-                const float f = ldexpf(f16_bits_to_f32(d), -e);
+                const _Float16 f = (_Float16)ldexpf(df, -e);
                 if (c == 0) exps[r] = e;
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i) {
-                    const h2t q = __builtin_bit_cast(h2t, o[i]);
-                    const float x = (float)q[0] * f, y = (float)q[1] * f;
-                    const h2t hi = {(_Float16)x, (_Float16)y};
-                    const h2t l2 = {(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])};
+                    const h2t q = __builtin_bit_cast(h2t, o[i]), ff = {f, f};
+                    const h2t hi = q * ff;
                     o[i] = __builtin_bit_cast(uint32_t, hi);
-                    lo[i] = __builtin_bit_cast(uint32_t, l2);
+                    lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(q, ff, -hi));
                 }
             }
             if (clean) {
@@ -328,14 +352,14 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 if constexpr (PARTS == 2) *(u4t*)(y + part_bytes + 4 * i) = u4t{lo[i], lo[i + 1], lo[i + 2], lo[i + 3]};
             }
         };
-        auto commit = [&](uint32_t t) {
+        auto commit = [&](const Raw& set, uint32_t t) {
             const bool clean = (t + 1) * TR > (uint32_t)held;  // holds rows that only some tokens see
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
-                const int i = tid + 64 * NW * j, r = i / PPR, c = i % PPR;
-                if (C::PIECES % (64 * NW) && i >= C::PIECES) break;  // (whole waves: PIECES is a multiple of 64)
-                put(imgK, C::RSK, C::KB, rk[j], QUANT ? dk[j] : 0u, r, c, sEk, false, t);
-                put(imgV, C::RSV, C::VB, rv[j], QUANT ? dv[j] : 0u, r, c, sEv, clean, t);
+                const int r = r0 + 64 * NW / PPR * j, c = c0;
+                if (C::PIECES % (64 * NW) && tid + 64 * NW * j >= C::PIECES) break;  // (whole waves: PIECES is a multiple of 64)
+                put(imgK, C::RS, C::PB, set.k[j], QUANT ? set.dk[j] : 0u, r, c, sEk, false, t);
+                put(imgV, C::RS, C::PB, set.v[j], QUANT ? set.dv[j] : 0u, r, c, sEv, clean, t);
             }
         };
 
@@ -375,7 +399,6 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     }
                 }
             }
-            fetch(page, in);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 float big = 0.0f;
@@ -397,8 +420,15 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     }
             }
         }
-        uint64_t valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+        fetch(raw[0], page, in);
+        uint64_t valid[C::DEPTH];  // rows that have a page, of the tile in each register set
+        valid[0] = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
         lookup(t_first + 1, page, in);
+        if constexpr (C::DEPTH == 2) {
+            fetch(raw[1], page, in);
+            valid[1] = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+            lookup(t_first + 2, page, in);
+        }
 
         f4t acc[MT][ND];
         float m_run[MT], l_run[MT];
@@ -412,15 +442,16 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
         int e_run = -1000;  // PARTS 2: the accumulators hold their sums times 2^-e_run
         if (tid < 2) sBad[tid] = 0;
 
-        for (uint32_t t = t_first; t < t_last; ++t) {
+        auto tile = [&](uint32_t t, auto set_tag) {
+            constexpr int SET = decltype(set_tag)::value;
             __syncthreads();  // the image is free, the flags are zero
-            commit(t);
+            commit(raw[SET], t);
             __syncthreads();
-            const uint64_t now = valid;
-            if (t + 1 < t_last) {
-                fetch(page, in);
-                valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
-                lookup(t + 2, page, in);
+            const uint64_t now = valid[SET];
+            if (t + C::DEPTH < t_last) {
+                fetch(raw[SET], page, in);
+                valid[SET] = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+                lookup(t + C::DEPTH + 1, page, in);
             }
             if (tid == 0) sBad[(t + 1) & 1] = 0;
 
@@ -465,105 +496,123 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     e_run = e;
                 }
             }
-            f4t s[MT][RT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) s[m][r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const uint8_t* k = imgK + (row0 + 16 * r + lr) * C::RSK + 64 * c + 16 * lg;
-                    const h8t kh = *(const h8t*)k;
-                    h8t kl;
-                    if constexpr (PARTS == 2) kl = *(const h8t*)(k + C::KB);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][0], s[m][r], 0, 0, 0);
-                        if constexpr (QP == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[m][c][1], s[m][r], 0, 0, 0);
-                        if constexpr (PARTS == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qo[m][c][0], s[m][r], 0, 0, 0);
-                    }
-                }
-            products_done();
-            // the lane's rows are row0 + 16r + 4lg + i; s * qf are base-2 scores
-            if constexpr (PARTS == 2) {
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const int4 e = *(const int4*)(sEk + row0 + 16 * r + 4 * lg);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                        s[m][r] = f4t{ldexpf(s[m][r][0], e.x), ldexpf(s[m][r][1], e.y), ldexpf(s[m][r][2], e.z), ldexpf(s[m][r][3], e.w)};
-                }
-            }
-            if (careful) {
+#pragma unroll 1
+            for (int sub = 0; sub < C::RW / (16 * RT); ++sub) {
+                const int row0 = C::RW * wr + 16 * RT * sub;  // the first of the wave's rows at this step
+                f4t s[MT][RT];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
+                    for (int r = 0; r < RT; ++r) s[m][r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+                // K rows, a batch of chunks at a time: all of its reads before its products
+                const uint8_t* const krow = imgK + (row0 + lr) * C::RS + 16 * lg;
+#pragma unroll
+                for (int c0 = 0; c0 < NB; c0 += KC) {
+                    h8t kh[KC][RT], kl[PARTS == 2 ? KC : 1][PARTS == 2 ? RT : 1];
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            const uint8_t* k = krow + 16 * r * C::RS + 64 * (c0 + c);
+                            kh[c][r] = *(const h8t*)k;
+                            if constexpr (PARTS == 2) kl[c][r] = *(const h8t*)(k + C::PB);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][r], qo[m][c0 + c][0], s[m][r], 0, 0, 0);
+                                if constexpr (QP == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][r], qo[m][c0 + c][1], s[m][r], 0, 0, 0);
+                                if constexpr (PARTS == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[c][r], qo[m][c0 + c][0], s[m][r], 0, 0, 0);
+                            }
+                }
+                // the first V columns come while the softmax runs
+                const uint8_t* const vrow = imgV + (row0 + 4 * lg + (lr >> 2)) * C::RS + 8 * (lr & 3);
+                h4t vh[2][VC][RT], vl[PARTS == 2 ? 2 : 1][PARTS == 2 ? VC : 1][PARTS == 2 ? RT : 1];
+                auto columns = [&](int n0, int x) {
+#pragma unroll
+                    for (int n = 0; n < VC; ++n)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            const uint8_t* v = vrow + 32 * (n0 + n) + 16 * r * C::RS;
+                            vh[x][n][r] = __builtin_bit_cast(h4t, column4(v));
+                            if constexpr (PARTS == 2) vl[x][n][r] = __builtin_bit_cast(h4t, column4(v + C::PB));
+                        }
+                };
+                columns(0, 0);
+                products_done();
+                // the lane's rows are row0 + 16r + 4lg + i; s * qf are base-2 scores
+                if constexpr (PARTS == 2) {
+#pragma unroll
                     for (int r = 0; r < RT; ++r) {
-                        const uint32_t bits = (uint32_t)(sees[m] >> (row0 + 16 * r + 4 * lg));
+                        const int4 e = *(const int4*)(sEk + row0 + 16 * r + 4 * lg);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[m][r][i] = (bits >> i) & 1u ? s[m][r][i] : -INFINITY;
+                        for (int m = 0; m < MT; ++m)
+                            s[m][r] = f4t{ldexpf(s[m][r][0], e.x), ldexpf(s[m][r][1], e.y), ldexpf(s[m][r][2], e.z), ldexpf(s[m][r][3], e.w)};
                     }
-            }
-            bool over = false;
-            float top[MT];
+                }
+                if (careful) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                top[m] = -INFINITY;
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                        for (int r = 0; r < RT; ++r) {
+                            const uint32_t bits = (uint32_t)(sees[m] >> (row0 + 16 * r + 4 * lg));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top[m] = fmaxf(top[m], s[m][r][i]);
-                top[m] *= qf[m];
-                over |= top[m] > m_run[m] + kTreeLazy;
-            }
-            if (__builtin_amdgcn_ballot_w64(over)) {
+                            for (int i = 0; i < 4; ++i) s[m][r][i] = (bits >> i) & 1u ? s[m][r][i] : -INFINITY;
+                        }
+                }
+                bool over = false;
+                float top[MT];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const float mt = across_rows_max(top[m]);
-                    const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) : m_run[m];
-                    const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
-                    l_run[m] *= f;
+                    top[m] = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < ND; ++n) acc[m][n] *= f;
-                    m_run[m] = mn;
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top[m] = fmaxf(top[m], s[m][r][i]);
+                    top[m] *= qf[m];
+                    over |= top[m] > m_run[m] + kTreeLazy;
                 }
-            }
-            // weights
-            h4t ph[MT][RT], pl[QP == 2 ? MT : 1][QP == 2 ? RT : 1];
+                if (__builtin_amdgcn_ballot_w64(over)) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const float mu = m_run[m] == -INFINITY ? 0.0f : -(m_run[m] + kTreeOff);
+                    for (int m = 0; m < MT; ++m) {
+                        const float mt = across_rows_max(top[m]);
+                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) : m_run[m];
+                        const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
+                        l_run[m] *= f;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    f4t p;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[i] = __builtin_amdgcn_exp2f(fmaf(s[m][r][i], qf[m], mu));
-                        l_run[m] += p[i];
-                    }
-                    if constexpr (PARTS == 2) {
-                        const int4 e = *(const int4*)(sEv + row0 + 16 * r + 4 * lg);
-                        p = f4t{ldexpf(p[0], e.x - e_run), ldexpf(p[1], e.y - e_run), ldexpf(p[2], e.z - e_run), ldexpf(p[3], e.w - e_run)};
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        ph[m][r][i] = (_Float16)p[i];
-                        if constexpr (QP == 2) pl[m][r][i] = (_Float16)(p[i] - (float)ph[m][r][i]);
+                        for (int n = 0; n < ND; ++n) acc[m][n] *= f;
+                        m_run[m] = mn;
                     }
                 }
-            }
-            // O^T += V^T P^T
+                // weights
+                h4t ph[MT][RT], pl[QP == 2 ? MT : 1][QP == 2 ? RT : 1];
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-                const uint8_t* v = imgV + (row0 + 4 * lg + (lr >> 2)) * C::RSV + 32 * n + 8 * (lr & 3);
-                h4t vh[RT], vl[PARTS == 2 ? RT : 1];
+                for (int m = 0; m < MT; ++m) {
+                    const float mu = m_run[m] == -INFINITY ? 0.0f : -(m_run[m] + kTreeOff);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    vh[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV));
-                    if constexpr (PARTS == 2) vl[r] = __builtin_bit_cast(h4t, column4(v + 16 * r * C::RSV + C::VB));
+                    for (int r = 0; r < RT; ++r) {
+                        f4t p;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = __builtin_amdgcn_exp2f(fmaf(s[m][r][i], qf[m], mu));
+                            l_run[m] += p[i];
+                        }
+                        if constexpr (PARTS == 2) {
+                            const int4 e = *(const int4*)(sEv + row0 + 16 * r + 4 * lg);
+                            p = f4t{ldexpf(p[0], e.x - e_run), ldexpf(p[1], e.y - e_run), ldexpf(p[2], e.z - e_run), ldexpf(p[3], e.w - e_run)};
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            ph[m][r][i] = (_Float16)p[i];
+                            if constexpr (QP == 2) pl[m][r][i] = (_Float16)(p[i] - (float)ph[m][r][i]);
+                        }
+                    }
                 }
+                // O^T += V^T P^T
                 auto product = [&](const h4t (&x)[RT], const h4t (&p)[RT], f4t& o) {
                     if constexpr (RT == 2)
                         o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(x[0], x[RT - 1], 0, 1, 2, 3, 4, 5, 6, 7),
@@ -572,23 +621,31 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                         o = __builtin_amdgcn_mfma_f32_16x16x16f16(x[0], p[0], o, 0, 0, 0);
                 };
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    product(vh, ph[m], acc[m][n]);
-                    if constexpr (QP == 2) product(vh, pl[m], acc[m][n]);
-                    if constexpr (PARTS == 2) product(vl, ph[m], acc[m][n]);
+                for (int n0 = 0; n0 < ND; n0 += VC) {
+                    const int x = n0 / VC % 2;
+                    if (n0 + VC < ND) columns(n0 + VC, 1 - x);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int n = 0; n < VC; ++n)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            product(vh[x][n], ph[m], acc[m][n0 + n]);
+                            if constexpr (QP == 2) product(vh[x][n], pl[m], acc[m][n0 + n]);
+                            if constexpr (PARTS == 2) product(vl[x][n], ph[m], acc[m][n0 + n]);
+                        }
                 }
             }
             products_done();
             // non-finite values of rows that not every token sees: to the tokens that do
             if (careful) {
                 uint64_t bad = sBad[t & 1];
-                if constexpr (WR > 1) bad &= (~0ull >> (64 - 16 * RT)) << row0;
+                if constexpr (WR > 1) bad &= (~0ull >> (64 - C::RW)) << (C::RW * wr);
                 bad = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(bad >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)bad);
                 while (bad) {
                     const int r = __builtin_ctzll(bad);
                     bad &= bad - 1;
                     const uint32_t row = t * TR + r, c = a.pg.d_page.quot(row);
-                    const uint8_t* v = vb + (uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c] * a.pg.v_page + (row - c * a.pg.d_page.d) * a.pg.v_row;
+                    const uint8_t* v = vb + (uint64_t)(uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c] * a.v_page + (uint64_t)(row - c * a.pg.d_page.d) * a.v_row;
 #pragma unroll 1
                     for (int d = 0; d < D; d += 16)
 #pragma unroll
@@ -605,8 +662,15 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                         }
                 }
             }
+        };
+        for (uint32_t t = t_first; t < t_last; t += C::DEPTH) {
+            tile(t, std::integral_constant<int, 0>{});
+            if constexpr (C::DEPTH == 2) {
+                if (t + 1 < t_last) tile(t + 1, std::integral_constant<int, 1>{});
+            }
         }
         u += t_last - t_first;
+        if (u < u_end) seqs.load(a, seqs.b0, seqs.before);  // again: not held in registers meanwhile
 
         // ---- the segment's result, or this workgroup's part of it
         if constexpr (PARTS == 2) {
@@ -692,63 +756,89 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
     }
 }
 
-// Joins the parts of the segments that more than one workgroup had: one wave per
-// (sequence, token, head), lane p the p-th part's maximum and sum, then all lanes the dims.
-template <int D, bool NARROW, int PW, int TR>
+// Joins the parts of the segments that more than one workgroup had. NWR waves per row
+// (sequence, token, head): D / 4 lanes read a part's dims, NG parts at a time and
+// four of those in flight, each group of lanes with a running maximum of its own.
+template <int D, bool NARROW, int PW, int TR, int NWR>
 __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
-    const int lane = lane_id();
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
-    if (row >= (int64_t)a.B * a.n_q * a.H) return;
-    const int h = (int)(row % a.H), t = (int)(row / a.H % a.n_q), b = (int)(row / a.H / a.n_q);
-    const SeqWork s = seq_work<PW, TR>(a, b);
-    if (t >= s.n_tok) return;
-    uint32_t before = 0, total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const uint32_t x = wave_scan(b0 + lane < a.B ? seq_work<PW, TR>(a, b0 + lane).units : 0u);
-        if (b > b0) before = total + lane_get(x, min(b - b0, 64) - 1);
-        total += lane_get(x, 63);
-    }
-    const Deal deal(total, a.d_wgs);
-    const int hk = h / a.G, pair = t * a.G + h - hk * a.G, pt = pair / PW;
-    const uint32_t u0 = before + ((uint32_t)hk * s.ptiles + (uint32_t)pt) * s.tiles;
-    const uint32_t w0 = deal.owner(u0), w1 = deal.owner(u0 + s.tiles - 1);
-    if (w0 == w1) return;
-    const int64_t piece0 = (int64_t)w0 + (b * a.pg.n_head_kv + hk) * a.max_ptiles + pt;
-    const int n = (int)(w1 - w0) + 1, p = pair - pt * PW;
-    constexpr int E = D / 64;
-    float o[E] = {}, l = 0.0f, top = -INFINITY;
-    for (int x = lane; x < n; x += 64) top = fmaxf(top, a.part_ml[(piece0 + x) * a.part_pairs + p].x);
-    top = wave_max(top);
-    for (int x0 = 0; x0 < n; x0 += 64) {
-        const int x = x0 + lane;
-        float f = 0.0f;
-        if (x < n) {
-            const float2 ml = a.part_ml[(piece0 + x) * a.part_pairs + p];
-            if (ml.x != -INFINITY) {
-                f = __builtin_amdgcn_exp2f(ml.x - top);
-                l = fmaf(ml.y, f, l);
-            }
-        }
-        const int m = min(64, n - x0);
-#pragma unroll 8
-        for (int i = 0; i < m; ++i) {
-            const float g = lane_read(f, i);
-            const float* y = a.part_o + ((piece0 + x0 + i) * a.part_pairs + p) * D + lane * E;
+    constexpr int L = D / 4, NG = 64 * NWR / L, UN = 4, RB = 4 / NWR;
+    __shared__ float sO[RB][NG][D], sM[RB][NG], sL[RB][NG];
+    const int rb = RB == 1 ? 0 : wave_id(), tid = threadIdx.x % (64 * NWR);
+    const uint32_t row = uniform(blockIdx.x * RB + rb);
+    const uint32_t bt = a.d_h.quot(row), h = row - bt * a.d_h.d;
+    const uint32_t b = a.d_q.quot(bt), t = bt - b * a.d_q.d;
+    SeqChunk<PW, TR> seqs;
+    const Deal deal(seqs.total(a), a.d_wgs, a.least);
+    const bool real = b < (uint32_t)a.B;
+    while (real && (uint32_t)seqs.b0 + 64 <= b) seqs.load(a, seqs.b0 + 64, seqs.last());
+    const int sl = real ? (int)b - seqs.b0 : 0;
+    const bool live = real && t < lane_get((uint32_t)seqs.mine.n_tok, sl);
+    const uint32_t tiles = lane_get(seqs.mine.tiles, sl), ptiles = lane_get(seqs.mine.ptiles, sl);
+    const uint32_t hk = a.d_g.quot(h), pair = t * a.G + h - hk * a.G, pt = pair / PW;
+    const uint32_t u0 = lane_get(seqs.upto, sl) - lane_get(seqs.mine.units, sl) + (hk * ptiles + pt) * tiles;
+    // (one part: its workgroup has written the row)
+    const uint32_t w0 = live ? deal.owner(u0) : 0u, n = live ? deal.owner(u0 + tiles - 1) - w0 + 1 : 1u;
+    const bool on = n > 1;
+    const int64_t part0 = ((int64_t)w0 + ((int64_t)b * a.pg.n_head_kv + hk) * a.max_ptiles + pt) * a.part_pairs + (pair - pt * PW);
+    const int g = tid / L, d = 4 * (tid % L);
+    f4t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t x0 = g; on && x0 < n; x0 += NG * UN) {
+        f4t y[UN];
+        float2 ml[UN];
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(g, y[e], o[e]);
+        for (int i = 0; i < UN; ++i) {
+            const int64_t at = part0 + (int64_t)min(x0 + NG * i, n - 1) * a.part_pairs;
+            ml[i] = a.part_ml[at];
+            y[i] = *(const f4t*)(a.part_o + at * D + d);
+            if (x0 + NG * i >= n) ml[i].x = -INFINITY;
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) top = fmaxf(top, ml[i].x);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        o *= f;
+        l *= f;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            if (ml[i].x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
+            l = fmaf(ml[i].y, w, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(y[i][e], w, o[e]);
         }
     }
-    l = wave_sum(l);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint8_t* y = a.dst + b * a.d_nb3 + t * a.d_nb2 + h * a.d_nb1;
+    *(f4t*)&sO[rb][g][d] = o;
+    if (d == 0) {
+        sM[rb][g] = m;
+        sL[rb][g] = l;
+    }
+    __syncthreads();
+    if (!on) return;
+    float top = sM[rb][0], sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
+    for (int i = 1; i < NG; ++i) top = fmaxf(top, sM[rb][i]);
+#pragma unroll
+    for (int e0 = 0; e0 < D; e0 += 64 * NWR) {
+        const int e = e0 + tid;
+        if (e >= D) break;
+        float v = 0.0f;
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const float w = sM[rb][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[rb][i] - top);
+            sum = fmaf(sL[rb][i], w, sum);
+            v = fmaf(sO[rb][i][e], w, v);
+        }
+        v *= sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint8_t* y = a.dst + b * a.d_nb3 + t * a.d_nb2 + h * a.d_nb1;
         if constexpr (NARROW)
-            *(uint16_t*)(y + 2 * (lane * E + e)) = (uint16_t)f32_to_bf16_bits(o[e] * inv);
+            ((uint16_t*)y)[e] = (uint16_t)f32_to_bf16_bits(v);
         else
-            *(float*)(y + 4 * (lane * E + e)) = o[e] * inv;
+            ((float*)y)[e] = v;
+        if (a.lse && e == 0) a.lse[(int64_t)bt * a.H + h] = sum == 0.0f ? -INFINITY : (top + kTreeOff) * kTreeLn2 + logf(sum);
     }
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.n_q + t) * a.H + h] = l == 0.0f ? -INFINITY : (top + kTreeOff) * kTreeLn2 + logf(l);
 }
 
 static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, PagesView* pg) {
@@ -770,10 +860,12 @@ static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const 
         return failf(XQ_ERR_UNSUPPORTED, "dst strides and pointer must be multiples of 16 bytes");
     const xq_status st = pages_check(cache, D, 0, B, kF16 | kE5M2 | kQ8 | kQ4, pg);
     if (st != XQ_OK) return st;
+    for (const xq_tensor* t : {&cache->k, &cache->v})
+        if (t->nb[1] >> 32 || t->nb[3] >> 32) return failf(XQ_ERR_UNSUPPORTED, "row and page strides must be below 2^32 bytes");
     const int64_t Hkv = cache->k.ne[2];
     if (H % Hkv) return failf(XQ_ERR_BAD_SHAPE, "n_head %% n_head_kv != 0");
     if (H / Hkv > 32) return failf(XQ_ERR_UNSUPPORTED, "GQA group above 32");
-    if (B > 65535 || H > 65535) return failf(XQ_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
+    if (B * T * H >= (int64_t)1 << 23) return failf(XQ_ERR_UNSUPPORTED, "2^23 query rows or more");
     return XQ_OK;
 }
 
@@ -781,7 +873,7 @@ static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const 
 struct TreePlan {
     int form;                 // index into the forms below
     int pw, tr;               // pairs of a workgroup, KV rows of a tile
-    uint32_t wgs;
+    uint32_t wgs, least;
     int32_t max_ptiles, part_pairs;
     int64_t parts;
     size_t ml_at, bytes;
@@ -804,42 +896,52 @@ static void tree_form(int form, F f) {
         break;
     }
 }
+template <int KT, typename F>
+static void tree_types(int64_t D, bool narrow, F f) {
+    if (D == 128) narrow ? f(std::integral_constant<int, 128>{}, std::true_type{}) : f(std::integral_constant<int, 128>{}, std::false_type{});
+    else narrow ? f(std::integral_constant<int, 256>{}, std::true_type{}) : f(std::integral_constant<int, 256>{}, std::false_type{});
+}
+// f(KT, D, NARROW, form) of the call
+template <typename F>
+static void tree_variant(int kt, int64_t D, bool narrow, int form, F f) {
+    auto at = [&](auto k) {
+        tree_types<decltype(k)::value>(D, narrow, [&](auto d, auto nar) {
+            tree_form<decltype(d)::value, decltype(nar)::value>(form, [&](auto fm) { f(k, d, nar, fm); });
+        });
+    };
+    switch (kt) {
+    case XQ_TYPE_F16: at(std::integral_constant<int, XQ_TYPE_F16>{}); break;
+    case XQ_TYPE_E5M2: at(std::integral_constant<int, XQ_TYPE_E5M2>{}); break;
+    case XQ_TYPE_Q8_0: at(std::integral_constant<int, XQ_TYPE_Q8_0>{}); break;
+    default: at(std::integral_constant<int, XQ_TYPE_Q4_0>{}); break;
+    }
+}
 static TreePlan tree_plan(const xq_tensor* q, const xq_kv_pages* c) {
     TreePlan P{};
     const int64_t D = q->ne[0], Hkv = c->k.ne[2], B = q->ne[3], pairs = q->ne[1] * (q->ne[2] / Hkv);
     P.form = pairs <= 16 ? 0 : pairs <= 32 ? 1 : pairs <= 64 ? 2 : pairs <= 128 || D == 256 ? 3 : 4;
-    P.pw = 16 << P.form;
-    P.tr = P.form < 2 ? 64 : 32;
+    int per_cu = 1;
+    tree_variant(c->k.type, D, q->type == XQ_TYPE_BF16, P.form, [&](auto k, auto d, auto nar, auto fm) {
+        using F = decltype(fm);
+        using C = TreeCfg<decltype(k)::value, decltype(d)::value, decltype(nar)::value, F::MT, F::WR, F::NW>;
+        P.pw = C::PW;
+        P.tr = C::TR;
+        per_cu = C::PER_CU;
+    });
     P.max_ptiles = (int32_t)cdiv(pairs, P.pw);
     P.part_pairs = (int32_t)(pairs < P.pw ? pairs : P.pw);
     const int64_t segs = B * Hkv * P.max_ptiles;
     // tiles that the table could hold, at most
     const int64_t tiles = cdiv((int64_t)c->table_cols * c->k.ne[1], P.tr) * segs;
-    int64_t wgs = P.form < 2 ? 1024 : 512;
+    int64_t wgs = 256 * per_cu;
     if (wgs > tiles) wgs = tiles;
     P.wgs = (uint32_t)wgs;
+    P.least = 1;
     P.parts = wgs + segs;
     const size_t o = (size_t)P.parts * P.part_pairs * D * 4;
     P.ml_at = (o + 255) / 256 * 256;
     P.bytes = P.ml_at + (size_t)P.parts * P.part_pairs * 8;
     return P;
-}
-
-template <int KT, int D, bool NARROW>
-static void tree_launch(const TreePlan& P, const TreeArgs& a, hipStream_t s) {
-    const dim3 grid(P.wgs), rows((uint32_t)cdiv((int64_t)a.B * a.n_q * a.H, 4));
-    tree_form<D, NARROW>(P.form, [&](auto form) {
-        using F = decltype(form);
-        using C = TreeCfg<KT, D, NARROW, F::MT, F::WR, F::NW>;
-        launch("fa_tree", fa_tree_kernel<KT, D, NARROW, F::MT, F::WR, F::NW>, grid, dim3(64 * F::NW), s, a);
-        launch("fa_tree_join", fa_tree_join<D, NARROW, C::PW, C::TR>, rows, dim3(256), s, a);
-    });
-}
-
-template <int KT>
-static void tree_launch_type(const TreePlan& P, const TreeArgs& a, int64_t D, bool narrow, hipStream_t s) {
-    if (D == 128) narrow ? tree_launch<KT, 128, true>(P, a, s) : tree_launch<KT, 128, false>(P, a, s);
-    else narrow ? tree_launch<KT, 256, true>(P, a, s) : tree_launch<KT, 256, false>(P, a, s);
 }
 
 }  // namespace xq
@@ -877,20 +979,28 @@ xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t
     a.q_nb1 = (int64_t)q->nb[1], a.q_nb2 = (int64_t)q->nb[2], a.q_nb3 = (int64_t)q->nb[3];
     a.dst = (uint8_t*)dst->data;
     a.d_nb1 = (int64_t)dst->nb[1], a.d_nb2 = (int64_t)dst->nb[2], a.d_nb3 = (int64_t)dst->nb[3];
+    a.k_page = (uint32_t)a.pg.k_page, a.k_row = (uint32_t)a.pg.k_row, a.v_page = (uint32_t)a.pg.v_page, a.v_row = (uint32_t)a.pg.v_row;
     a.lse = lse, a.parents = parents, a.n_tok = n_tok, a.scale = scale;
     a.n_q = (int32_t)q->ne[1], a.H = (int32_t)q->ne[2], a.B = (int32_t)q->ne[3];
     a.G = a.H / a.pg.n_head_kv;
-    a.d_g = UDivFlat((uint32_t)a.G), a.d_wgs = UDivFlat(P.wgs);
+    a.d_g = UDivFlat((uint32_t)a.G), a.d_wgs = UDivFlat(P.wgs), a.d_h = UDivFlat((uint32_t)a.H), a.d_q = UDivFlat((uint32_t)a.n_q);
+    a.least = P.least;
     a.max_ptiles = P.max_ptiles, a.part_pairs = P.part_pairs;
     a.part_o = (float*)workspace, a.part_ml = (float2*)((uint8_t*)workspace + P.ml_at);
     const bool narrow = q->type == XQ_TYPE_BF16;
     hipStream_t s = (hipStream_t)stream;
-    switch (cache->k.type) {
-    case XQ_TYPE_F16: tree_launch_type<XQ_TYPE_F16>(P, a, q->ne[0], narrow, s); break;
-    case XQ_TYPE_E5M2: tree_launch_type<XQ_TYPE_E5M2>(P, a, q->ne[0], narrow, s); break;
-    case XQ_TYPE_Q8_0: tree_launch_type<XQ_TYPE_Q8_0>(P, a, q->ne[0], narrow, s); break;
-    default: tree_launch_type<XQ_TYPE_Q4_0>(P, a, q->ne[0], narrow, s); break;
-    }
+    tree_variant(cache->k.type, q->ne[0], narrow, P.form, [&](auto k, auto d, auto nar, auto fm) {
+        using F = decltype(fm);
+        constexpr int KT = decltype(k)::value, D = decltype(d)::value;
+        constexpr bool NARROW = decltype(nar)::value;
+        using C = TreeCfg<KT, D, NARROW, F::MT, F::WR, F::NW>;
+        launch("fa_tree", fa_tree_kernel<KT, D, NARROW, F::MT, F::WR, F::NW>, dim3(P.wgs), dim3(64 * F::NW), s, a);
+        const uint32_t rows = (uint32_t)((int64_t)a.B * a.n_q * a.H);
+        if (rows <= 2048)
+            launch("fa_tree_join", fa_tree_join<D, NARROW, C::PW, C::TR, 4>, dim3(rows), dim3(256), s, a);
+        else
+            launch("fa_tree_join", fa_tree_join<D, NARROW, C::PW, C::TR, 1>, dim3((rows + 3) / 4), dim3(256), s, a);
+    });
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return failf(XQ_ERR_HIP, "fa_tree launch: %s", hipGetErrorString(e));
     return done_ok();
