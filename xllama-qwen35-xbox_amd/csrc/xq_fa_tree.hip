@@ -153,7 +153,12 @@ XQ_DEV void products_done() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Work of sequence b: its rows, tokens, row tiles and (KV head, pair tile, row tile) units.
+// A segment is one (sequence, KV head, pair tile); its units of work are its row tiles after
+// kStart units that stand for what a workgroup spends on it before its first tile (three
+// dependent loads, Q, and the state written at the end: the time of about two tiles).
+constexpr uint32_t kStart = 2;
+
+// Work of sequence b: its rows, tokens, row tiles, pair tiles and units.
 struct SeqWork {
     int32_t held, n_tok, end;
     uint32_t tiles, ptiles, units;
@@ -166,7 +171,7 @@ XQ_DEV SeqWork seq_work(const TreeArgs& a, int b) {
     s.end = (int32_t)min((uint32_t)s.held + (uint32_t)s.n_tok, (uint32_t)a.pg.row_limit);
     s.tiles = s.n_tok ? ((uint32_t)s.end + TR - 1) / TR : 0u;
     s.ptiles = (uint32_t)(s.n_tok * a.G + PW - 1) / PW;
-    s.units = s.tiles * s.ptiles * (uint32_t)a.pg.n_head_kv;
+    s.units = s.tiles ? (kStart + s.tiles) * s.ptiles * (uint32_t)a.pg.n_head_kv : 0u;
     return s;
 }
 
@@ -242,6 +247,12 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
     uint8_t* const imgK = img;
     uint8_t* const imgV = img + PARTS * C::PB;
 
+    // every argument the prologue needs, asked for at once: left to their uses, the scalar
+    // loads go out one dependent group after another
+    asm volatile("" ::"s"(a.pg.rows), "s"(a.n_tok), "s"(a.pg.table), "s"(a.parents), "s"(a.q), "s"(a.pg.k), "s"(a.pg.v), "s"(a.pg.k_head),
+                 "s"(a.pg.v_head), "s"(a.q_nb1), "s"(a.q_nb2), "s"(a.q_nb3), "s"(a.pg.table_cols), "s"(a.pg.n_pages), "s"(a.pg.row_limit),
+                 "s"(a.pg.n_head_kv), "s"(a.pg.d_page.m), "s"(a.n_q), "s"(a.G), "s"(a.B), "s"(a.scale), "s"(a.k_page), "s"(a.v_row),
+                 "s"(a.d_g.m), "s"(a.d_wgs.m), "s"(a.least));
     const uint32_t w = xcd_remap(blockIdx.x, a.d_wgs.d);
     SeqChunk<PW, TR> seqs;
     const Deal deal(seqs.total(a), a.d_wgs, a.least);
@@ -256,9 +267,12 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
         const int end = (int)lane_get((uint32_t)seqs.mine.end, sl);
         const uint32_t tiles = lane_get(seqs.mine.tiles, sl), ptiles = lane_get(seqs.mine.ptiles, sl);
         const uint32_t in_b = u - (lane_get(seqs.upto, sl) - lane_get(seqs.mine.units, sl));
-        const uint32_t seg = uniform(in_b / tiles), t_first = in_b - seg * tiles;
+        const uint32_t seg_units = kStart + tiles, seg = uniform(in_b / seg_units), v0 = in_b - seg * seg_units;
+        const uint32_t v1 = min(seg_units, v0 + (u_end - u));
+        u += v1 - v0;
+        if (v1 <= kStart) continue;  // no tile of it
+        const uint32_t t_first = max(v0, kStart) - kStart, t_last = v1 - kStart;
         const int hk = (int)uniform(seg / ptiles), pt = (int)(seg - (uint32_t)hk * ptiles);
-        const uint32_t t_last = min(tiles, t_first + (u_end - u));
         const bool whole = t_first == 0 && t_last == tiles;
         const int n_pairs = n_tok * a.G;
         const int p0 = pt * PW + pg * 16 * MT;  // this wave's first pair
@@ -497,7 +511,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 }
             }
 #pragma unroll 1
-            for (int sub = 0; sub < C::RW / (16 * RT); ++sub) {
+            for (int sub = 0; sub < (p0 < n_pairs ? C::RW / (16 * RT) : 0); ++sub) {  // (a wave without pairs only brings tiles)
                 const int row0 = C::RW * wr + 16 * RT * sub;  // the first of the wave's rows at this step
                 f4t s[MT][RT];
 #pragma unroll
@@ -669,7 +683,6 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 if (t + 1 < t_last) tile(t + 1, std::integral_constant<int, 1>{});
             }
         }
-        u += t_last - t_first;
         if (u < u_end) seqs.load(a, seqs.b0, seqs.before);  // again: not held in registers meanwhile
 
         // ---- the segment's result, or this workgroup's part of it
@@ -775,7 +788,7 @@ __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
     const bool live = real && t < lane_get((uint32_t)seqs.mine.n_tok, sl);
     const uint32_t tiles = lane_get(seqs.mine.tiles, sl), ptiles = lane_get(seqs.mine.ptiles, sl);
     const uint32_t hk = a.d_g.quot(h), pair = t * a.G + h - hk * a.G, pt = pair / PW;
-    const uint32_t u0 = lane_get(seqs.upto, sl) - lane_get(seqs.mine.units, sl) + (hk * ptiles + pt) * tiles;
+    const uint32_t u0 = lane_get(seqs.upto, sl) - lane_get(seqs.mine.units, sl) + (hk * ptiles + pt) * (kStart + tiles) + kStart;  // its first tile
     // (one part: its workgroup has written the row)
     const uint32_t w0 = live ? deal.owner(u0) : 0u, n = live ? deal.owner(u0 + tiles - 1) - w0 + 1 : 1u;
     const bool on = n > 1;
@@ -931,10 +944,10 @@ static TreePlan tree_plan(const xq_tensor* q, const xq_kv_pages* c) {
     P.max_ptiles = (int32_t)cdiv(pairs, P.pw);
     P.part_pairs = (int32_t)(pairs < P.pw ? pairs : P.pw);
     const int64_t segs = B * Hkv * P.max_ptiles;
-    // tiles that the table could hold, at most
-    const int64_t tiles = cdiv((int64_t)c->table_cols * c->k.ne[1], P.tr) * segs;
+    // units that the table could hold, at most
+    const int64_t units = (cdiv((int64_t)c->table_cols * c->k.ne[1], P.tr) + kStart) * segs;
     int64_t wgs = 256 * per_cu;
-    if (wgs > tiles) wgs = tiles;
+    if (wgs > units) wgs = units;
     P.wgs = (uint32_t)wgs;
     P.least = 1;
     P.parts = wgs + segs;
