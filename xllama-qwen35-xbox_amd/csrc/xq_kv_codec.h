@@ -117,4 +117,16 @@ XQ_DEV void kv_put4(const f4u x, uint32_t lane, uint32_t el, int32_t q8_variant,
     }
 }
 
+// The same with the type known at run time (the same for the whole wave).
+XQ_DEV void kv_put4_any(int32_t kt, const f4u x, uint32_t lane, uint32_t el, int32_t q8_variant, uint8_t* y, bool live) {
+    switch (kt) {
+    case XQ_TYPE_F32: kv_put4<XQ_TYPE_F32>(x, lane, el, q8_variant, y, live); break;
+    case XQ_TYPE_F16: kv_put4<XQ_TYPE_F16>(x, lane, el, q8_variant, y, live); break;
+    case XQ_TYPE_BF16: kv_put4<XQ_TYPE_BF16>(x, lane, el, q8_variant, y, live); break;
+    case XQ_TYPE_E5M2: kv_put4<XQ_TYPE_E5M2>(x, lane, el, q8_variant, y, live); break;
+    case XQ_TYPE_Q8_0: kv_put4<XQ_TYPE_Q8_0>(x, lane, el, q8_variant, y, live); break;
+    default: kv_put4<XQ_TYPE_Q4_0>(x, lane, el, q8_variant, y, live); break;
+    }
+}
+
 }  // namespace xq

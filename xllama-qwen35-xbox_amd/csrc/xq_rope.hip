@@ -19,17 +19,19 @@ namespace xq {
 
 struct RopeArgs {
     const uint8_t *q, *k, *v;
-    int64_t q_nb1, q_nb2, q_nb3, k_nb1, k_nb2, k_nb3, v_nb1, v_nb2, v_nb3;  // token, head, sequence
+    int64_t q_nb1, q_nb3, k_nb1, k_nb3, v_nb1, v_nb3;  // token, sequence
+    uint32_t q_nb2, k_nb2, v_nb2, o_nb2;               // head, below 2^32
     uint8_t* out;
-    int64_t o_nb1, o_nb2, o_nb3;
+    int64_t o_nb1, o_nb3;
     const int32_t* positions;
     const int32_t* n_tok;
     const float *qw, *kw, *ff;
     PagesView pg;
     int32_t kt, q8_variant, mode, n_rot, n_q, H, Hkv;
     int32_t units_q, units_kv;    // 256-element units of a token's queries; of its keys
-    int32_t parts, units_part;    // waves per token, units per wave
-    int64_t n_waves;
+    int32_t units_part;           // units of a wave
+    uint32_t n_waves;
+    UDivFlat d_parts, d_q;        // by the waves per token; by the tokens per sequence
     double rev0, rate;            // revolutions per position of index 0; factor from an index to the next
     double log2_rate;
     float attn, eps;
@@ -40,16 +42,18 @@ constexpr int kRopeBatch = 4;  // units whose loads a wave has in flight
 typedef uint16_t u16e __attribute__((aligned(2)));
 typedef uint32_t u32x2e __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f4e __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4f __attribute__((ext_vector_type(4), aligned(4)));
 
+// Four neighbouring elements as they lie in memory, and as f32.
+template <int T> struct Quad;
+template <> struct Quad<XQ_TYPE_F32> { using Raw = u32x4f; static constexpr int W = 4; };
+template <> struct Quad<XQ_TYPE_BF16> { using Raw = u32x2e; static constexpr int W = 2; };
 template <int T>
-XQ_DEV f4e load4(const uint8_t* p) {
-    if constexpr (T == XQ_TYPE_F32) {
-        return *(const f4e*)p;
-    } else {
-        const u32x2e w = *(const u32x2e*)p;
-        return f4e{bf16_bits_to_f32(w.x & 0xffffu), __uint_as_float(w.x & 0xffff0000u), bf16_bits_to_f32(w.y & 0xffffu),
-                   __uint_as_float(w.y & 0xffff0000u)};
-    }
+XQ_DEV f4e quad_f32(const typename Quad<T>::Raw w) {
+    if constexpr (T == XQ_TYPE_F32)
+        return __builtin_bit_cast(f4e, w);
+    else
+        return f4e{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
 }
 
 template <int T>
@@ -57,8 +61,10 @@ XQ_DEV void store4(uint8_t* p, f4e x) {
     if constexpr (T == XQ_TYPE_F32) {
         *(f4e*)p = x;
     } else {
-        *(u32x2e*)p = u32x2e{f32_to_bf16_bits(x[0]) | (f32_to_bf16_bits(x[1]) << 16),
-                             f32_to_bf16_bits(x[2]) | (f32_to_bf16_bits(x[3]) << 16)};
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        *(u32x2e*)p = u32x2e{__builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x[0], x[1]}), b2)),
+                             __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x[2], x[3]}), b2))};
     }
 }
 
@@ -80,117 +86,136 @@ XQ_DEV float head_sum(float x) {
 template <int TI, int TO, int D>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
     constexpr int RPU = 256 / D, LPR = D / 4, ES = TI == XQ_TYPE_F32 ? 4 : 2, EO = TO == XQ_TYPE_F32 ? 4 : 2;
-    const int64_t w = (int64_t)blockIdx.x * 4 + wave_id();
+    using Raw = typename Quad<TI>::Raw;
+    constexpr int W = Quad<TI>::W;
+    const uint32_t w = blockIdx.x * 4u + wave_id();
     if (w >= a.n_waves) return;
-    const int64_t tok = w / a.parts;
-    const int part = (int)(w - tok * a.parts);
-    const int b = (int)(tok / a.n_q), t = (int)(tok - (int64_t)b * a.n_q);
+    const uint32_t tok = a.d_parts.quot(w);
+    const int part = (int)(w - tok * a.d_parts.d);
+    const int b = (int)a.d_q.quot(tok), t = (int)(tok - b * a.d_q.d);
     if (a.n_tok && t >= a.n_tok[b]) return;
     const int lane = lane_id(), sub = lane / LPR, e0 = 4 * (lane % LPR);
-    const int u_end = min((part + 1) * a.units_part, a.units_q + 2 * a.units_kv);
-
-    // the row of the cache that takes this token's key and value
+    const int u_first = part * a.units_part, u_end = min(u_first + a.units_part, a.units_q + 2 * a.units_kv);
+    const int32_t position = a.positions[(int64_t)b * a.n_q + t];
     const int64_t row = (int64_t)a.pg.rows[b] + t;
-    const bool in = row >= 0 && row < a.pg.row_limit;
-    const uint32_t r = in ? (uint32_t)row : 0u;
-    const uint32_t page = a.pg.page(b, r), off = r - a.pg.d_page.quot(r) * (uint32_t)a.pg.page_rows;
-    const bool kept = in && page < (uint32_t)a.pg.n_pages;
 
-    // cos and sin of this lane's four elements (an element past n_rot is not turned)
-    const int half = a.n_rot / 2;
-    const bool halves = a.mode == XQ_ROPE_HALVES;
-    const bool turned = e0 < a.n_rot;
-    float cs[4], sn[4];
-    {
-        const int i0 = halves ? (e0 >= half ? e0 - half : e0) : e0 / 2;  // first index of the lane
-        const double pos = (double)a.positions[(int64_t)b * a.n_q + t];
-        double rev = pos * a.rev0 * exp2(a.log2_rate * i0);
+    // A kind's units [u0, u1) in batches: every load of a batch before its first use.
+    auto stream = [&](const uint8_t* base, uint32_t nb2, int heads, int u0, int u1, auto use) {
+        for (int u = u0; u < u1; u += kRopeBatch) {
+            Raw x[kRopeBatch];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!halves && j >= 2) break;
-            const int i = i0 + j;
-            double x = rev;
-            if (a.ff && i < half) x /= (double)a.ff[i];
-            x -= rint(x);
-            float s, c;
-            sincospif(2.0f * (float)x, &s, &c);
-            cs[j] = c * a.attn;
-            sn[j] = s * a.attn;
-            rev *= a.rate;
+            for (int i = 0; i < kRopeBatch; ++i) {
+                const uint32_t h = (uint32_t)min(min(u + i, u1 - 1) * RPU + sub, heads - 1);
+                // read once: past the caches (8194 tokens of 24 + 8 heads of 256 bf16: 65.7 us, with
+                // ordinary loads 71.9)
+                x[i] = __builtin_nontemporal_load((const Raw*)(base + (uint64_t)h * nb2 + e0 * ES));
+            }
+#pragma unroll
+            for (int i = 0; i < kRopeBatch; ++i)
+                if (u + i < u1) use(x[i], (u + i) * RPU + sub);
         }
-    }
-    const int shift = half / 4;  // lanes from an element to its partner
-    const bool low = e0 < half;
-    const int partner = !turned ? lane : low ? lane + shift : lane - shift;
+    };
+    const int uq1 = min(u_end, a.units_q), uk0 = max(u_first, a.units_q), uk1 = min(u_end, a.units_q + a.units_kv);
+    const int uv0 = max(u_first, a.units_q + a.units_kv);
 
-    f4e wq = {1.0f, 1.0f, 1.0f, 1.0f}, wk = wq;
-    if (a.qw) wq = *(const f4e*)(a.qw + e0);
-    if (a.kw) wk = *(const f4e*)(a.kw + e0);
-
-    for (int u0 = part * a.units_part; u0 < u_end; u0 += kRopeBatch) {
-        f4e x[kRopeBatch];
-        int head[kRopeBatch];
+    if (u_first < a.units_q + a.units_kv) {
+        // cos and sin of this lane's four elements: an element past n_rot does not turn
+        const int half = a.n_rot / 2;
+        const bool halves = a.mode == XQ_ROPE_HALVES;
+        const bool turned = e0 < a.n_rot, low = e0 < half;
+        f4e cs = {1.0f, 1.0f, 1.0f, 1.0f}, sn = {0.0f, 0.0f, 0.0f, 0.0f};
+        {
+            const int i0 = halves ? (low ? e0 : e0 - half) : e0 / 2;  // first index of the lane
+            double rev = (double)position * a.rev0 * exp2(a.log2_rate * i0);
 #pragma unroll
-        for (int i = 0; i < kRopeBatch; ++i) {
-            const int u = min(u0 + i, u_end - 1);
-            const bool is_q = u < a.units_q, is_k = u < a.units_q + a.units_kv;
-            head[i] = (u - (is_q ? 0 : is_k ? a.units_q : a.units_q + a.units_kv)) * RPU + sub;
-            const uint8_t* p = is_q ? a.q + b * a.q_nb3 + t * a.q_nb1 : is_k ? a.k + b * a.k_nb3 + t * a.k_nb1 : a.v + b * a.v_nb3 + t * a.v_nb1;
-            const int64_t nb2 = is_q ? a.q_nb2 : is_k ? a.k_nb2 : a.v_nb2;
-            const int last = (is_q ? a.H : a.Hkv) - 1;
-            x[i] = load4<TI>(p + min(head[i], last) * nb2 + e0 * ES);
-        }
-#pragma unroll
-        for (int i = 0; i < kRopeBatch; ++i) {
-            const int u = u0 + i;
-            if (u >= u_end) break;
-            const bool is_q = u < a.units_q, is_v = u >= a.units_q + a.units_kv;
-            f4e y = x[i];
-            if (!is_v) {
-                if (is_q ? a.qw : a.kw) {
-                    const float ss = head_sum<D>(fmaf(y[3], y[3], fmaf(y[2], y[2], fmaf(y[1], y[1], y[0] * y[0]))));
-                    const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-                    const f4e g = is_q ? wq : wk;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y[j] = y[j] * inv * g[j];
-                }
+            for (int j = 0; j < 4; ++j) {
+                if (!halves && j >= 2) break;
+                double x = rev;
+                if (a.ff && i0 + j < half) x /= (double)a.ff[i0 + j];
+                x -= rint(x);
+                float s, c;
+                sincospif(2.0f * (float)x, &s, &c);
+                c *= a.attn;
+                s *= a.attn;
                 if (halves) {
-                    f4e z;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) z[j] = __shfl(y[j], partner);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float turn = low ? fmaf(y[j], cs[j], -(z[j] * sn[j])) : fmaf(y[j], cs[j], z[j] * sn[j]);
-                        y[j] = turned ? turn : y[j];
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float p = y[2 * j], q = y[2 * j + 1];
-                        if (e0 + 2 * j < a.n_rot) {
-                            y[2 * j] = fmaf(p, cs[j], -(q * sn[j]));
-                            y[2 * j + 1] = fmaf(p, sn[j], q * cs[j]);
-                        }
-                    }
+                    cs[j] = turned ? c : 1.0f;
+                    sn[j] = turned ? (low ? -s : s) : 0.0f;
+                } else if (e0 + 2 * j < a.n_rot) {
+                    cs[2 * j] = cs[2 * j + 1] = c;
+                    sn[2 * j] = -s;
+                    sn[2 * j + 1] = s;
                 }
-            }
-            if (is_q) {
-                if (head[i] < a.H) store4<TO>(a.out + b * a.o_nb3 + t * a.o_nb1 + head[i] * a.o_nb2 + e0 * EO, y);
-                continue;
-            }
-            const bool live = kept && head[i] < a.Hkv;
-            uint8_t* y0 = is_v ? a.pg.v + page * a.pg.v_page + off * a.pg.v_row + head[i] * a.pg.v_head
-                               : a.pg.k + page * a.pg.k_page + off * a.pg.k_row + head[i] * a.pg.k_head;
-            const f4u yy = {y[0], y[1], y[2], y[3]};
-            switch (a.kt) {
-            case XQ_TYPE_F32: kv_put4<XQ_TYPE_F32>(yy, lane, e0, a.q8_variant, y0, live); break;
-            case XQ_TYPE_F16: kv_put4<XQ_TYPE_F16>(yy, lane, e0, a.q8_variant, y0, live); break;
-            case XQ_TYPE_BF16: kv_put4<XQ_TYPE_BF16>(yy, lane, e0, a.q8_variant, y0, live); break;
-            case XQ_TYPE_E5M2: kv_put4<XQ_TYPE_E5M2>(yy, lane, e0, a.q8_variant, y0, live); break;
-            case XQ_TYPE_Q8_0: kv_put4<XQ_TYPE_Q8_0>(yy, lane, e0, a.q8_variant, y0, live); break;
-            default: kv_put4<XQ_TYPE_Q4_0>(yy, lane, e0, a.q8_variant, y0, live); break;
+                rev *= a.rate;
             }
         }
+        const int shift = half / 4;  // lanes from an element to its partner
+        const int partner = low ? lane + shift : lane - shift;
+        // y cos +- z sin with y = x w / norm, z = the partner: x (w cos) / norm + x' (w' sin) / norm
+        f4e qc = cs, qs = sn, kc = cs, ks = sn;
+        auto weigh = [&](const float* g, f4e& c, f4e& s) {
+            if (!g) return;
+            const f4e own = *(const f4e*)(g + e0);
+            f4e other = own;
+            if (halves) {
+                if (turned) other = *(const f4e*)(g + (low ? e0 + half : e0 - half));
+            } else {
+                other = f4e{own[1], own[0], own[3], own[2]};
+            }
+            c *= own;
+            s *= other;
+        };
+        weigh(a.qw, qc, qs);
+        weigh(a.kw, kc, ks);
+        auto turn = [&](const Raw x, const f4e c, const f4e s, bool norm) -> f4e {
+            const f4e y = quad_f32<TI>(x);
+            f4e z;
+            if (halves) {
+                Raw other;
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const uint32_t o = (uint32_t)__shfl((int)x[j], partner);
+                    other[j] = turned ? o : 0u;  // what does not turn takes nothing, whatever is there
+                }
+                z = quad_f32<TI>(other);
+            } else {
+                z = f4e{e0 < a.n_rot ? y[1] : 0.0f, e0 < a.n_rot ? y[0] : 0.0f, e0 + 2 < a.n_rot ? y[3] : 0.0f, e0 + 2 < a.n_rot ? y[2] : 0.0f};
+            }
+            f4e r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = fmaf(y[j], c[j], z[j] * s[j]);
+            if (norm) {
+                const float ss = head_sum<D>(fmaf(y[3], y[3], fmaf(y[2], y[2], fmaf(y[1], y[1], y[0] * y[0]))));
+                r *= __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / D, a.eps));  // 1 ulp
+            }
+            return r;
+        };
+        uint8_t* const out = a.out + b * a.o_nb3 + t * a.o_nb1;
+        stream(a.q + b * a.q_nb3 + t * a.q_nb1, a.q_nb2, a.H, u_first, uq1, [&](const Raw x, int head) {
+            const f4e y = turn(x, qc, qs, a.qw != nullptr);
+            if (head < a.H) store4<TO>(out + (uint64_t)(uint32_t)head * a.o_nb2 + e0 * EO, y);
+        });
+        // the row of the cache that takes this token's key
+        const bool in = row >= 0 && row < a.pg.row_limit;
+        const uint32_t r = in ? (uint32_t)row : 0u;
+        const uint32_t page = a.pg.page(b, r), off = r - a.pg.d_page.quot(r) * a.pg.d_page.d;
+        const bool kept = in && page < (uint32_t)a.pg.n_pages;
+        uint8_t* const to = a.pg.k + page * a.pg.k_page + off * a.pg.k_row;
+        stream(a.k + b * a.k_nb3 + t * a.k_nb1, a.k_nb2, a.Hkv, uk0 - a.units_q, uk1 - a.units_q, [&](const Raw x, int head) {
+            const f4e y = turn(x, kc, ks, a.kw != nullptr);
+            kv_put4_any(a.kt, f4u{y[0], y[1], y[2], y[3]}, lane, e0, a.q8_variant, to + head * a.pg.k_head, kept && head < a.Hkv);
+        });
+    }
+    if (uv0 < u_end) {
+        const bool in = row >= 0 && row < a.pg.row_limit;
+        const uint32_t r = in ? (uint32_t)row : 0u;
+        const uint32_t page = a.pg.page(b, r), off = r - a.pg.d_page.quot(r) * a.pg.d_page.d;
+        const bool kept = in && page < (uint32_t)a.pg.n_pages;
+        uint8_t* const to = a.pg.v + page * a.pg.v_page + off * a.pg.v_row;
+        const int before = a.units_q + a.units_kv;
+        stream(a.v + b * a.v_nb3 + t * a.v_nb1, a.v_nb2, a.Hkv, uv0 - before, u_end - before, [&](const Raw x, int head) {
+            const f4e y = quad_f32<TI>(x);
+            kv_put4_any(a.kt, f4u{y[0], y[1], y[2], y[3]}, lane, e0, a.q8_variant, to + head * a.pg.v_head, kept && head < a.Hkv);
+        });
     }
 }
 
@@ -215,6 +240,7 @@ static xq_status rope_check(const xq_tensor* q, const xq_tensor* k, const xq_ten
         const size_t es = type_size(t->type);
         if (t->nb[0] != es) return failf(XQ_ERR_UNSUPPORTED, "elements must be contiguous");
         if (!elem_aligned(t, es, 1) || !aligned(t->data, es)) return failf(XQ_ERR_UNSUPPORTED, "misaligned tensor");
+        if (t->nb[2] >> 32) return failf(XQ_ERR_UNSUPPORTED, "head strides must be below 2^32 bytes");
     }
     if (p->mode != XQ_ROPE_HALVES && p->mode != XQ_ROPE_PAIRS) return failf(XQ_ERR_BAD_ARG, "bad rope mode %d", p->mode);
     if (p->n_rot < 0 || p->n_rot > D || p->n_rot % 2) return failf(XQ_ERR_BAD_ARG, "n_rot must be even and in [0, head dim]");
@@ -228,7 +254,7 @@ static xq_status rope_check(const xq_tensor* q, const xq_tensor* k, const xq_ten
 
 template <int TI, int TO>
 static hipError_t rope_launch(const RopeArgs& a, int64_t D, hipStream_t stream) {
-    const dim3 grid((uint32_t)((a.n_waves + 3) / 4)), block(256);
+    const dim3 grid((a.n_waves + 3) / 4), block(256);
     switch (D) {
     case 64: launch("qk_norm_rope", qk_norm_rope_kernel<TI, TO, 64>, grid, block, stream, a); break;
     case 128: launch("qk_norm_rope", qk_norm_rope_kernel<TI, TO, 128>, grid, block, stream, a); break;
@@ -261,11 +287,11 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
         if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
     const int64_t D = q->ne[0], rpu = 256 / D;
     a.q = (const uint8_t*)q->data, a.k = (const uint8_t*)k->data, a.v = (const uint8_t*)v->data;
-    a.q_nb1 = (int64_t)q->nb[1], a.q_nb2 = (int64_t)q->nb[2], a.q_nb3 = (int64_t)q->nb[3];
-    a.k_nb1 = (int64_t)k->nb[1], a.k_nb2 = (int64_t)k->nb[2], a.k_nb3 = (int64_t)k->nb[3];
-    a.v_nb1 = (int64_t)v->nb[1], a.v_nb2 = (int64_t)v->nb[2], a.v_nb3 = (int64_t)v->nb[3];
+    a.q_nb1 = (int64_t)q->nb[1], a.q_nb2 = (uint32_t)q->nb[2], a.q_nb3 = (int64_t)q->nb[3];
+    a.k_nb1 = (int64_t)k->nb[1], a.k_nb2 = (uint32_t)k->nb[2], a.k_nb3 = (int64_t)k->nb[3];
+    a.v_nb1 = (int64_t)v->nb[1], a.v_nb2 = (uint32_t)v->nb[2], a.v_nb3 = (int64_t)v->nb[3];
     a.out = (uint8_t*)q_out->data;
-    a.o_nb1 = (int64_t)q_out->nb[1], a.o_nb2 = (int64_t)q_out->nb[2], a.o_nb3 = (int64_t)q_out->nb[3];
+    a.o_nb1 = (int64_t)q_out->nb[1], a.o_nb2 = (uint32_t)q_out->nb[2], a.o_nb3 = (int64_t)q_out->nb[3];
     a.positions = positions, a.n_tok = n_tok, a.qw = q_weight, a.kw = k_weight, a.ff = freq_factors;
     a.kt = cache->k.type, a.q8_variant = p->q8_variant, a.mode = p->mode, a.n_rot = p->n_rot;
     a.n_q = (int32_t)q->ne[1], a.H = (int32_t)q->ne[2], a.Hkv = (int32_t)k->ne[2];
@@ -276,9 +302,10 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
     if (upw < 1) upw = 1;
     if (upw > units) upw = units;
     a.units_part = (int32_t)upw;
-    a.parts = (int32_t)cdiv(units, upw);
-    a.n_waves = tokens * a.parts;
-    if (a.n_waves > (int64_t)0x7fffffff) return failf(XQ_ERR_UNSUPPORTED, "too many tokens for one call");
+    const int64_t parts = cdiv(units, upw);
+    if (tokens * parts > 0x7ffffff0) return failf(XQ_ERR_UNSUPPORTED, "too many tokens for one call");
+    a.n_waves = (uint32_t)(tokens * parts);
+    a.d_parts = UDivFlat((uint32_t)parts), a.d_q = UDivFlat((uint32_t)a.n_q);
     a.log2_rate = p->n_rot ? -2.0 / p->n_rot * log2((double)p->freq_base) : 0.0;
     a.rate = exp2(a.log2_rate);
     a.rev0 = (double)p->freq_scale / 6.283185307179586476925286766559;
