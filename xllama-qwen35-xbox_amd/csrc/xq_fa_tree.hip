@@ -45,7 +45,12 @@ constexpr float kTreeOff = -7.0f;      // weights are 2^(x - max + 7), in (0, 2^
 template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 struct TreeCfg {
     static constexpr bool QUANT = KT == XQ_TYPE_Q8_0 || KT == XQ_TYPE_Q4_0;
-    static constexpr int PARTS = QUANT && !NARROW ? 2 : 1;                  // f16 parts of a cached value
+    // f32 Q on quantized K and V. Where few pairs share a row: the image holds the integers (exact
+    // in f16), the block scales join in f32 (scores, and weights before their split in two).
+    // That takes 5 vector instructions per weight and block, so where the waves share
+    // the pairs the image holds d * q in two f16 parts instead, at three products for two.
+    static constexpr bool SCALED = QUANT && !NARROW && WR > 1;
+    static constexpr int PARTS = QUANT && !NARROW && !SCALED ? 2 : 1;       // f16 parts of a cached value
     static constexpr int QP = NARROW ? 1 : 2;                               // f16 parts of Q and of the weights
     static constexpr int EL = KT == XQ_TYPE_F16 ? 8 : KT == XQ_TYPE_Q4_0 ? 32 : 16;  // elements of a 16-byte piece
     static constexpr int PPR = D / EL;                                      // pieces per row
@@ -61,9 +66,10 @@ struct TreeCfg {
     static constexpr int MS = D + 4;                                        // merge row stride, floats
     static constexpr int MERGE = WR > 1 ? NW * 16 * MS * 4 : 0;
     static constexpr int SMEM = IMG > MERGE ? IMG : MERGE;
-    // tiles whose loads are in flight while one is computed: two where their registers allow it
-    static constexpr int DEPTH = NPT * 2 * (QUANT ? 5 : 4) <= 20 ? 2 : 1;
-    static constexpr int WAVES = D == 256 || MT == 2 || PARTS == 2 ? 2 : 3;  // per SIMD, that the registers allow
+    // Waves per SIMD: two (256 registers each); three where the form fits 168 registers without
+    // spills (32 fp8 chats of up to 8000 rows: 32.4 us against 34.2; 32 f16 chats, whose form
+    // spills there, 70.1 against 59.4)
+    static constexpr int WAVES = NARROW && D == 128 && WR == 4 && (KT == XQ_TYPE_E5M2 || KT == XQ_TYPE_Q4_0) ? 3 : 2;
     // workgroups that a CU holds
     static constexpr int BY_LDS = 160 * 1024 / (SMEM + 2048), BY_WAVES = WAVES * 4 / NW;
     static constexpr int PER_CU = BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES;
@@ -155,8 +161,8 @@ XQ_DEV void products_done() {
 
 // A segment is one (sequence, KV head, pair tile); its units of work are its row tiles after
 // kStart units that stand for what a workgroup spends on it before its first tile (three
-// dependent loads, Q, and the state written at the end: the time of about two tiles).
-constexpr uint32_t kStart = 2;
+// dependent loads, Q, and the state written at the end: the time of two to four tiles).
+constexpr uint32_t kStart = 3;
 
 // Work of sequence b: its rows, tokens, row tiles, pair tiles and units.
 struct SeqWork {
@@ -234,12 +240,13 @@ template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES)) void fa_tree_kernel(TreeArgs a) {
     using C = TreeCfg<KT, D, NARROW, MT, WR, NW>;
     constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW, TR = C::TR, RT = C::RT;
-    constexpr bool QUANT = C::QUANT;
+    constexpr bool QUANT = C::QUANT, SCALED = C::SCALED;
     constexpr int KC = PARTS == 2 ? 2 : 4;  // 32-element chunks of K read at once
-    constexpr int VC = PARTS == 2 ? 4 : 8;  // 16-element columns of V
+    constexpr int VC = PARTS == 2 ? 2 : 4;  // 16-element columns of V
     __shared__ __attribute__((aligned(16))) uint8_t img[C::SMEM];
     __shared__ float sM[WR > 1 ? NW : 1][16 * MT], sL[WR > 1 ? NW : 1][16 * MT];
-    __shared__ int sEk[PARTS == 2 ? TR : 1], sEv[PARTS == 2 ? TR : 1];
+    __shared__ __attribute__((aligned(16))) int sEk[PARTS == 2 ? TR : 4], sEv[PARTS == 2 || SCALED ? TR : 4];
+    __shared__ __attribute__((aligned(16))) float sDk[SCALED ? NB : 1][SCALED ? TR : 4], sDv[SCALED ? NB : 1][SCALED ? TR : 4];
     __shared__ unsigned long long sBad[2];
     const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x, lr = lane & 15, lg = lane >> 4;
     const int wr = wave % WR, pg = wave / WR;  // the wave's rows and pairs of a tile
@@ -294,7 +301,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
             u4t k[NPT], v[NPT];
             uint32_t dk[QUANT ? NPT : 1], dv[QUANT ? NPT : 1];
         };
-        Raw raw[C::DEPTH];
+        Raw raw;  // the next tile's pieces, in flight while a tile is computed
         auto fetch = [&](Raw& set, uint32_t page, uint32_t in) {
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
@@ -319,37 +326,44 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
             }
         };
         // raw pieces -> image
-        auto put = [&](uint8_t* image, int rs, int part_bytes, const u4t raw, uint32_t d, int r, int c, int* exps, bool clean, uint32_t t) {
+        auto put = [&](uint8_t* image, int rs, int part_bytes, const u4t raw, uint32_t d, int r, int c, int* exps, float* scales, bool clean, uint32_t t) {
             constexpr int WORDS = C::EL / 2;
             uint32_t o[WORDS], lo[WORDS];
             piece_f16<KT, WORDS>(raw, o);
-            if constexpr (QUANT && PARTS == 1) {
+            if constexpr (QUANT && NARROW) {
                 const uint32_t dd = d | (d << 16);
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i) o[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2t, o[i]) * __builtin_bit_cast(h2t, dd));
             } else if constexpr (QUANT) {
-                // the row's power of two: its largest finite block scale to [2^7, 2^8), over the
-                // row's PPR (4, 8 or 16) lanes. Then d q = hi + lo exactly: hi its rounding, lo
-                // the remainder of at most 8 bits
+                // the exponent of the row's largest finite block scale, over the row's PPR (4, 8
+                // or 16) lanes
                 const float df = f16_bits_to_f32(d);
                 int e = (int)((__float_as_uint(df) >> 23) & 255u);
-                if (e == 255 || e == 0) e = 1;
+                if (e == 255 || e < 103) e = 103;  // 2^-24, the smallest f16: a zero scale asks for no larger power
                 e = max(e, dpp_i<0xB1>(e));
                 e = max(e, dpp_i<0x4E>(e));
                 if constexpr (PPR >= 8) e = max(e, dpp_i<0x141>(e));
                 if constexpr (PPR >= 16) e = max(e, dpp_i<0x140>(e));
-                e -= 127 + 7;
-                const _Float16 f = (_Float16)ldexpf(df, -e);
-                if (c == 0) exps[r] = e;
+                if constexpr (SCALED) {
+                    constexpr int PB = 32 / C::EL;  // pieces of a block
+                    if (c % PB == 0) scales[(c / PB) * TR + r] = df;
+                    if (exps && c == 0) exps[r] = e - 126;  // d 2^-e below 1
+                } else {
+                    // to [2^7, 2^8); then d q = hi + lo exactly: hi its rounding, lo the remainder
+                    // of at most 8 bits
+                    e -= 127 + 7;
+                    const _Float16 f = (_Float16)ldexpf(df, -e);
+                    if (c == 0) exps[r] = e;
 #pragma unroll
-                for (int i = 0; i < WORDS; ++i) {
-                    const h2t q = __builtin_bit_cast(h2t, o[i]), ff = {f, f};
-                    const h2t hi = q * ff;
-                    o[i] = __builtin_bit_cast(uint32_t, hi);
-                    lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(q, ff, -hi));
+                    for (int i = 0; i < WORDS; ++i) {
+                        const h2t q = __builtin_bit_cast(h2t, o[i]), ff = {f, f};
+                        const h2t hi = q * ff;
+                        o[i] = __builtin_bit_cast(uint32_t, hi);
+                        lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(q, ff, -hi));
+                    }
                 }
             }
-            if (clean) {
+            if (!SCALED && clean) {
                 uint32_t bad = 0;
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i) {
@@ -372,8 +386,8 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
             for (int j = 0; j < NPT; ++j) {
                 const int r = r0 + 64 * NW / PPR * j, c = c0;
                 if (C::PIECES % (64 * NW) && tid + 64 * NW * j >= C::PIECES) break;  // (whole waves: PIECES is a multiple of 64)
-                put(imgK, C::RS, C::PB, set.k[j], QUANT ? set.dk[j] : 0u, r, c, sEk, false, t);
-                put(imgV, C::RS, C::PB, set.v[j], QUANT ? set.dv[j] : 0u, r, c, sEv, clean, t);
+                put(imgK, C::RS, C::PB, set.k[j], QUANT ? set.dk[j] : 0u, r, c, SCALED ? nullptr : sEk, &sDk[0][0], false, t);
+                put(imgV, C::RS, C::PB, set.v[j], QUANT ? set.dv[j] : 0u, r, c, sEv, &sDv[0][0], clean, t);
             }
         };
 
@@ -434,15 +448,9 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     }
             }
         }
-        fetch(raw[0], page, in);
-        uint64_t valid[C::DEPTH];  // rows that have a page, of the tile in each register set
-        valid[0] = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+        fetch(raw, page, in);
+        uint64_t valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);  // rows of raw's tile that have a page
         lookup(t_first + 1, page, in);
-        if constexpr (C::DEPTH == 2) {
-            fetch(raw[1], page, in);
-            valid[1] = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
-            lookup(t_first + 2, page, in);
-        }
 
         f4t acc[MT][ND];
         float m_run[MT], l_run[MT];
@@ -453,19 +461,18 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 #pragma unroll
             for (int n = 0; n < ND; ++n) acc[m][n] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        int e_run = -1000;  // PARTS 2: the accumulators hold their sums times 2^-e_run
+        int e_run = -1000;  // PARTS 2, SCALED: the accumulators hold their sums times 2^-e_run
         if (tid < 2) sBad[tid] = 0;
 
-        auto tile = [&](uint32_t t, auto set_tag) {
-            constexpr int SET = decltype(set_tag)::value;
+        for (uint32_t t = t_first; t < t_last; ++t) {
             __syncthreads();  // the image is free, the flags are zero
-            commit(raw[SET], t);
+            commit(raw, t);
             __syncthreads();
-            const uint64_t now = valid[SET];
-            if (t + C::DEPTH < t_last) {
-                fetch(raw[SET], page, in);
-                valid[SET] = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
-                lookup(t + C::DEPTH + 1, page, in);
+            const uint64_t now = valid;
+            if (t + 1 < t_last) {
+                fetch(raw, page, in);
+                valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);
+                lookup(t + 2, page, in);
             }
             if (tid == 0) sBad[(t + 1) & 1] = 0;
 
@@ -496,7 +503,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     sees[m] = s & now;
                 }
             }
-            if constexpr (PARTS == 2) {
+            if constexpr (PARTS == 2 || SCALED) {
                 int e = sEv[lane % TR];
 #pragma unroll
                 for (int s = 1; s < 64; s *= 2) e = max(e, __shfl_xor(e, s));
@@ -518,6 +525,27 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int r = 0; r < RT; ++r) s[m][r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (SCALED) {
+                    // a block's integer products, times its scales of the lane's rows
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const uint8_t* const k = imgK + (row0 + 16 * r + lr) * C::RS + 16 * lg;
+                        f4t z[NB];
+#pragma unroll
+                        for (int c = 0; c < NB; ++c) {
+                            const h8t kh = *(const h8t*)(k + 64 * c);
+                            z[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[0][c][0], f4t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                            z[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[0][c][QP - 1], z[c], 0, 0, 0);
+                        }
+                        products_done();
+#pragma unroll
+                        for (int c = 0; c < NB; ++c) {
+                            const f4t d = *(const f4t*)&sDk[c][row0 + 16 * r + 4 * lg];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[0][r][i] = fmaf(z[c][i], d[i], s[0][r][i]);
+                        }
+                    }
+                } else {
                 // K rows, a batch of chunks at a time: all of its reads before its products
                 const uint8_t* const krow = imgK + (row0 + lr) * C::RS + 16 * lg;
 #pragma unroll
@@ -542,6 +570,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                                 if constexpr (QP == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][r], qo[m][c0 + c][1], s[m][r], 0, 0, 0);
                                 if constexpr (PARTS == 2) s[m][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[c][r], qo[m][c0 + c][0], s[m][r], 0, 0, 0);
                             }
+                }
                 }
                 // the first V columns come while the softmax runs
                 const uint8_t* const vrow = imgV + (row0 + 4 * lg + (lr >> 2)) * C::RS + 8 * (lr & 3);
@@ -604,6 +633,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 }
                 // weights
                 h4t ph[MT][RT], pl[QP == 2 ? MT : 1][QP == 2 ? RT : 1];
+                f4t pw[SCALED ? RT : 1];  // SCALED: the weights times 2^-e_run
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     const float mu = m_run[m] == -INFINITY ? 0.0f : -(m_run[m] + kTreeOff);
@@ -614,6 +644,10 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                         for (int i = 0; i < 4; ++i) {
                             p[i] = __builtin_amdgcn_exp2f(fmaf(s[m][r][i], qf[m], mu));
                             l_run[m] += p[i];
+                        }
+                        if constexpr (SCALED) {
+                            pw[r] = f4t{ldexpf(p[0], -e_run), ldexpf(p[1], -e_run), ldexpf(p[2], -e_run), ldexpf(p[3], -e_run)};
+                            continue;
                         }
                         if constexpr (PARTS == 2) {
                             const int4 e = *(const int4*)(sEv + row0 + 16 * r + 4 * lg);
@@ -640,18 +674,39 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     if (n0 + VC < ND) columns(n0 + VC, 1 - x);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int n = 0; n < VC; ++n)
+                    for (int n = 0; n < VC; ++n) {
+                        if constexpr (SCALED) {
+                            // the weights times the block's scales, as f16 high and low parts
+                            if (n % 2 == 0) {
+#pragma unroll
+                                for (int r = 0; r < RT; ++r) {
+                                    const f4t d = *(const f4t*)&sDv[(n0 + n) / 2][row0 + 16 * r + 4 * lg];
+                                    f4t w = pw[r] * d;
+                                    if (careful) {  // (an unseen row's scale may be anything)
+                                        const uint32_t bits = (uint32_t)(sees[0] >> (row0 + 16 * r + 4 * lg));
+#pragma unroll
+                                        for (int i = 0; i < 4; ++i) w[i] = (bits >> i) & 1u ? w[i] : 0.0f;
+                                    }
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        ph[0][r][i] = (_Float16)w[i];
+                                        pl[0][r][i] = (_Float16)(w[i] - (float)ph[0][r][i]);
+                                    }
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int m = 0; m < MT; ++m) {
                             product(vh[x][n], ph[m], acc[m][n0 + n]);
                             if constexpr (QP == 2) product(vh[x][n], pl[m], acc[m][n0 + n]);
                             if constexpr (PARTS == 2) product(vl[x][n], ph[m], acc[m][n0 + n]);
                         }
+                    }
                 }
             }
             products_done();
             // non-finite values of rows that not every token sees: to the tokens that do
-            if (careful) {
+            if (!SCALED && careful) {
                 uint64_t bad = sBad[t & 1];
                 if constexpr (WR > 1) bad &= (~0ull >> (64 - C::RW)) << (C::RW * wr);
                 bad = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(bad >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)bad);
@@ -676,17 +731,11 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                         }
                 }
             }
-        };
-        for (uint32_t t = t_first; t < t_last; t += C::DEPTH) {
-            tile(t, std::integral_constant<int, 0>{});
-            if constexpr (C::DEPTH == 2) {
-                if (t + 1 < t_last) tile(t + 1, std::integral_constant<int, 1>{});
-            }
         }
         if (u < u_end) seqs.load(a, seqs.b0, seqs.before);  // again: not held in registers meanwhile
 
         // ---- the segment's result, or this workgroup's part of it
-        if constexpr (PARTS == 2) {
+        if constexpr (PARTS == 2 || SCALED) {
             const float f = ldexpf(1.0f, max(e_run, -126));
 #pragma unroll
             for (int m = 0; m < MT; ++m)
