@@ -34,6 +34,7 @@ typedef _Float16 h8t __attribute__((ext_vector_type(8)));
 typedef float f4t __attribute__((ext_vector_type(4)));
 typedef uint32_t u4t __attribute__((ext_vector_type(4)));
 typedef uint32_t u4any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u4dw __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16any __attribute__((aligned(1)));
 typedef uint32_t u4half __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f4el __attribute__((ext_vector_type(4), aligned(4)));
@@ -299,28 +300,42 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
         };
         struct Raw {
             u4t k[NPT], v[NPT];
-            uint32_t dk[QUANT ? NPT : 1], dv[QUANT ? NPT : 1];
+            // quantized: the fifth dword of each piece's window, and the bytes (0, 2 or 4, in
+            // halves, two bits each) that the piece starts into its window
+            uint32_t k5[QUANT ? NPT : 1], v5[QUANT ? NPT : 1], shift;
         };
         Raw raw;  // the next tile's pieces, in flight while a tile is computed
+        // A quantized piece (16 bytes behind a 2-byte scale in 34- or 18-byte blocks) by whole
+        // aligned dwords: 16-byte loads at 2-byte addresses took twice the time of a decode.
+        // The window starts at the dword of the block's scale, or (q8_0's second pieces) of the
+        // piece; every dword read holds a byte of the two.
+        auto window = [&](const uint8_t* rec, u4t& x, uint32_t& x5) -> uint32_t {
+            constexpr int BB = KT == XQ_TYPE_Q8_0 ? 34 : 18;
+            const bool first = KT == XQ_TYPE_Q4_0 || c0 % 2 == 0;
+            const uint8_t* q = rec + (KT == XQ_TYPE_Q8_0 ? c0 / 2 * BB + 2 + c0 % 2 * 16 : c0 * BB + 2);
+            const uint32_t odd = (uint32_t)(uintptr_t)q & 2u, shift = first && !odd ? 4u : odd;
+            const uint8_t* w = q - shift;
+            x = *(const u4dw*)w;
+            x5 = *(const uint32_t*)(w + (shift ? 16 : 12));
+            return shift / 2;
+        };
         auto fetch = [&](Raw& set, uint32_t page, uint32_t in) {
+            if constexpr (QUANT) set.shift = 0;
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
                 const int r = (r0 + 64 * NW / PPR * j) % TR;
                 const uint32_t p = (uint32_t)__shfl((int)page, r), x = (uint32_t)__shfl((int)in, r);
                 set.k[j] = u4t{0, 0, 0, 0};
                 set.v[j] = u4t{0, 0, 0, 0};
-                if constexpr (QUANT) set.dk[j] = set.dv[j] = 0u;
+                if constexpr (QUANT) set.k5[j] = set.v5[j] = 0u;
                 if (p < (uint32_t)a.pg.n_pages && (C::PIECES % (64 * NW) == 0 || tid + 64 * NW * j < C::PIECES)) {
                     const uint8_t* k = kb + (uint64_t)p * a.k_page + (uint64_t)x * a.k_row;
                     const uint8_t* v = vb + (uint64_t)p * a.v_page + (uint64_t)x * a.v_row;
-                    constexpr int BB = KT == XQ_TYPE_Q8_0 ? 34 : 18;
-                    const int blk = KT == XQ_TYPE_Q8_0 ? c0 / 2 : c0;
-                    const int at = QUANT ? blk * BB + 2 + (KT == XQ_TYPE_Q8_0 ? c0 % 2 * 16 : 0) : 16 * c0;
-                    set.k[j] = *(const u4any*)(k + at);
-                    set.v[j] = *(const u4any*)(v + at);
                     if constexpr (QUANT) {
-                        set.dk[j] = *(const u16any*)(k + blk * BB);
-                        set.dv[j] = *(const u16any*)(v + blk * BB);
+                        set.shift |= window(k, set.k[j], set.k5[j]) << (4 * j) | window(v, set.v[j], set.v5[j]) << (4 * j + 2);
+                    } else {
+                        set.k[j] = *(const u4any*)(k + 16 * c0);
+                        set.v[j] = *(const u4any*)(v + 16 * c0);
                     }
                 }
             }
@@ -380,14 +395,29 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 if constexpr (PARTS == 2) *(u4t*)(y + part_bytes + 4 * i) = u4t{lo[i], lo[i + 1], lo[i + 2], lo[i + 3]};
             }
         };
+        // the piece from its window; returns its block's scale
+        auto realign = [&](u4t& x, uint32_t x5, uint32_t half) -> uint32_t {
+            const uint32_t sel = 0x03020100u + half * 0x02020202u;
+            const uint32_t d = half == 2 ? x[0] >> 16 : x[0] & 0xffffu;
+            x = u4t{__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[2], x[1], sel),
+                    __builtin_amdgcn_perm(x[3], x[2], sel), __builtin_amdgcn_perm(x5, x[3], sel)};
+            // q8_0: the odd lane's scale is its even neighbour's (quad_perm 0, 0, 2, 2)
+            return KT == XQ_TYPE_Q8_0 ? (uint32_t)dpp_i<0xA0>((int)d) : d;
+        };
         auto commit = [&](const Raw& set, uint32_t t) {
             const bool clean = (t + 1) * TR > (uint32_t)held;  // holds rows that only some tokens see
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
                 const int r = r0 + 64 * NW / PPR * j, c = c0;
                 if (C::PIECES % (64 * NW) && tid + 64 * NW * j >= C::PIECES) break;  // (whole waves: PIECES is a multiple of 64)
-                put(imgK, C::RS, C::PB, set.k[j], QUANT ? set.dk[j] : 0u, r, c, SCALED ? nullptr : sEk, &sDk[0][0], false, t);
-                put(imgV, C::RS, C::PB, set.v[j], QUANT ? set.dv[j] : 0u, r, c, sEv, &sDv[0][0], clean, t);
+                u4t k = set.k[j], v = set.v[j];
+                uint32_t dk = 0u, dv = 0u;
+                if constexpr (QUANT) {
+                    dk = realign(k, set.k5[j], (set.shift >> (4 * j)) & 3u);
+                    dv = realign(v, set.v5[j], (set.shift >> (4 * j + 2)) & 3u);
+                }
+                put(imgK, C::RS, C::PB, k, dk, r, c, SCALED ? nullptr : sEk, &sDk[0][0], false, t);
+                put(imgV, C::RS, C::PB, v, dv, r, c, sEv, &sDv[0][0], clean, t);
             }
         };
 
