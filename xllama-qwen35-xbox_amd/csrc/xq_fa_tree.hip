@@ -106,6 +106,16 @@ XQ_DEV float across_rows_sum(float x) {
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
+// The largest over the wave, in a scalar register.
+XQ_DEV int wave_max_int(int x) {
+    x = max(x, dpp_i<0xB1>(x));
+    x = max(x, dpp_i<0x4E>(x));
+    x = max(x, dpp_i<0x141>(x));
+    x = max(x, dpp_i<0x140>(x));
+    const int a = max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
+    return max(a, max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+
 // Nonzero halves (0x8000 each) of w that are Inf or NaN.
 XQ_DEV uint32_t bad_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
 XQ_DEV uint32_t without_bad(uint32_t w) { return w & ~((bad_halves(w) >> 15) * 0xffffu); }
@@ -323,8 +333,8 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
             if constexpr (QUANT) set.shift = 0;
 #pragma unroll
             for (int j = 0; j < NPT; ++j) {
-                const int r = (r0 + 64 * NW / PPR * j) % TR;
-                const uint32_t p = (uint32_t)__shfl((int)page, r), x = (uint32_t)__shfl((int)in, r);
+                const int r4 = 4 * (r0 + 64 * NW / PPR * j);  // (modulo 64 lanes)
+                const uint32_t p = (uint32_t)__builtin_amdgcn_ds_bpermute(r4, (int)page), x = (uint32_t)__builtin_amdgcn_ds_bpermute(r4, (int)in);
                 set.k[j] = u4t{0, 0, 0, 0};
                 set.v[j] = u4t{0, 0, 0, 0};
                 if constexpr (QUANT) set.k5[j] = set.v5[j] = 0u;
@@ -386,7 +396,11 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     if constexpr (PARTS == 2) lo[i] &= ~((bad_halves(o[i]) >> 15) * 0xffffu);
                     o[i] = without_bad(o[i]);
                 }
-                if (bad) atomicOr(&sBad[t & 1], 1ull << r);
+                if (bad) {
+                    int row = r;
+                    asm volatile("" : "+v"(row));  // (its bit is formed here, not kept over the tiles)
+                    atomicOr(&sBad[t & 1], 1ull << row);
+                }
             }
             uint8_t* y = image + r * rs + c * (2 * C::EL);
 #pragma unroll
@@ -534,10 +548,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 }
             }
             if constexpr (PARTS == 2 || SCALED) {
-                int e = sEv[lane % TR];
-#pragma unroll
-                for (int s = 1; s < 64; s *= 2) e = max(e, __shfl_xor(e, s));
-                e = __builtin_amdgcn_readfirstlane(e);
+                const int e = wave_max_int(sEv[lane % TR]);
                 if (e > e_run) {
                     const float f = ldexpf(1.0f, e_run - e);
 #pragma unroll
@@ -560,19 +571,22 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
                         const uint8_t* const k = imgK + (row0 + 16 * r + lr) * C::RS + 16 * lg;
-                        f4t z[NB];
 #pragma unroll
-                        for (int c = 0; c < NB; ++c) {
-                            const h8t kh = *(const h8t*)(k + 64 * c);
-                            z[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[0][c][0], f4t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                            z[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[0][c][QP - 1], z[c], 0, 0, 0);
-                        }
-                        products_done();
+                        for (int c0 = 0; c0 < NB; c0 += 4) {
+                            f4t z[4];
 #pragma unroll
-                        for (int c = 0; c < NB; ++c) {
-                            const f4t d = *(const f4t*)&sDk[c][row0 + 16 * r + 4 * lg];
+                            for (int c = 0; c < 4; ++c) {
+                                const h8t kh = *(const h8t*)(k + 64 * (c0 + c));
+                                z[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[0][c0 + c][0], f4t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                                z[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qo[0][c0 + c][QP - 1], z[c], 0, 0, 0);
+                            }
+                            products_done();
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[0][r][i] = fmaf(z[c][i], d[i], s[0][r][i]);
+                            for (int c = 0; c < 4; ++c) {
+                                const f4t d = *(const f4t*)&sDk[c0 + c][row0 + 16 * r + 4 * lg];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) s[0][r][i] = fmaf(z[c][i], d[i], s[0][r][i]);
+                            }
                         }
                     }
                 } else {
