@@ -191,6 +191,47 @@ def test_kv_pages_refusals():
     assert lib.xq_kv_pages_release(None, None, None, 4, 3, 10, None, 0, None) == OK
 
 
+def test_limits_of_strides_and_counts():
+    """Sizes whose products the kernels hold in 32 bits, at and past their bounds."""
+    lib = xqattn.load()
+
+    def tree(want, q, c, d):
+        assert call_tree(q, c, d) == want and lib.xq_last_error(), lib.xq_last_error()
+        assert lib.xq_supports_fa_tree(ctypes.byref(q), ctypes.byref(c), ctypes.byref(d)) == 0
+
+    for i in (1, 3):  # row, page
+        for name in "kv":
+            tree(UNSUPPORTED, *tree_args(c=cache(**{name: with_nb(tensor(wl.F16, (128, 16, 4, 10)), i, 1 << 32)})))
+    tree(UNSUPPORTED, *tree_args(T=64, H=32, B=4096, c=cache(n_seq=4096)))                                 # 2^23 query rows
+    big = (1 << 31) - 1
+    tree(UNSUPPORTED, *tree_args(T=64, H=big, B=big, c=cache(n_seq=big, k=tensor(wl.F16, (128, 16, big, 10)), v=tensor(wl.F16, (128, 16, big, 10)))))
+    tree(UNSUPPORTED, *tree_args(T=1, H=8, B=1024, c=cache(n_seq=1024, P=1 << 20, cols=2000, Hkv=8)))         # 2^25 tiles of 8192 segments
+    q, c, d = tree_args(T=1, H=8, B=4, c=cache(n_seq=4, P=1 << 20, cols=2000, Hkv=8))
+    assert lib.xq_supports_fa_tree(ctypes.byref(q), ctypes.byref(c), ctypes.byref(d)) == 1
+
+    def rope(ok, T=4, B=2, H=8, nb=None):
+        a = [tensor(wl.F32, (128, T, h, B), nb=(4, 512 * h, 512, 512 * h * T)) for h in (H, 4, 4, H)]  # a token's heads together
+        if nb:
+            a[nb[0]].nb[2] = nb[1]
+        c, p = cache(n_seq=B), xqattn.rope_params(64, 1e4)
+        r = [ctypes.byref(x) for x in a]
+        assert lib.xq_supports_qk_norm_rope(r[0], r[1], r[2], ctypes.byref(p), r[3], ctypes.byref(c)) == ok
+        if not ok:
+            assert lib.xq_qk_norm_rope(r[0], r[1], r[2], DATA, None, None, None, None, ctypes.byref(p), r[3], ctypes.byref(c), None) == UNSUPPORTED
+
+    for i in range(4):
+        rope(0, nb=(i, 1 << 32))
+        rope(1, nb=(i, (1 << 32) - 4))
+    rope(1, T=(1 << 25) - 1)
+    rope(0, T=1 << 25)
+    rope(0, T=(1 << 31) - 1, B=(1 << 31) - 1)
+    two = (xqattn.XqTensor * 2)(tensor(wl.F16, (128, 16, 4, 10)), tensor(wl.F16, (128, 16, 4, 10)))
+    assert lib.xq_kv_pages_compact(two, 2, DATA, DATA, 2, 3, DATA, DATA, 4, DATA + 4096, None) == BAD_ARG   # one pool twice
+    many = (xqattn.XqTensor * 1025)(*[tensor(wl.F16, (128, 16, 4, 10), data=DATA + 4096 * i) for i in range(1025)])
+    assert lib.xq_kv_pages_copy(many, 1025, DATA, DATA, 1, None) == BAD_ARG
+    assert lib.xq_kv_pages_copy(many, 1024, DATA, DATA, 0, None) == OK
+
+
 def test_binding_refuses_tensors_that_do_not_fit():
     import torch
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731

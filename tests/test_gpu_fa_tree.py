@@ -335,3 +335,49 @@ def test_fa_tree_many_sequences(torch_gpu):
     q = bf16(q)
     got, lse = on_gpu(torch_gpu, q, c, parents, n_tok, 0.09, True)
     check(got, lse, tree_f64(q, c, parents, n_tok, 0.09, True))
+
+
+@pytest.mark.parametrize("kt", list(TYPES))
+@pytest.mark.parametrize("narrow", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("D,H,Hkv,rows,T", [(128, 8, 4, [3, 1500], 2), (256, 8, 4, [1, 400], 12), (128, 8, 4, [2, 90], 30)])
+def test_fa_tree_nan_queries_and_keys(torch_gpu, D, H, Hkv, rows, T, narrow, kt):
+    """A NaN query makes its own row of dst and lse NaN; a NaN key (or block scale) those of the
+    tokens that see it; the others stay as they were."""
+    rng, c, q, parents, n_tok = setup(40 + T, TYPES[kt], D, H, Hkv, 16, rows, T)
+    q = bf16(q)
+    parents[:] = np.arange(T) - 1
+    want = tree_f64(q, c, parents, n_tok, 0.08, narrow)
+    hit = np.zeros((len(rows), T, H), bool)
+    for b, t, h in ((0, 0, 1), (1, T - 1, H - 1), (1, 0, 4)):
+        q[b, t, h, rng.integers(D)] = np.nan
+        hit[b, t, h] = True
+    p, i = c.place(0, rows[0] + T // 2)  # sequence 0, KV head 2: seen from token T / 2 on
+    c.view(c.k)[p, i, 2, :2] = (0x7F, 0x7F) if kt == "e5m2" else (0x01, 0x7E)
+    hit[0, T // 2:, 4:6] = True
+    got, lse = on_gpu(torch_gpu, q, c, parents, n_tok, 0.08, narrow)
+    assert np.isnan(got[hit]).all() and np.isnan(lse[hit]).all()
+    assert np.all(np.abs(got - want[0])[~hit] <= want[2][~hit]) and np.all(np.abs(lse - want[1])[~hit] <= want[3][~hit])
+
+
+@pytest.mark.parametrize("narrow", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("kt", ["f16", "q4_0"])
+def test_fa_tree_infinite_values_in_many_segments(torch_gpu, kt, narrow):
+    """More segments than workgroups, each with an infinite value of a token's own row: a
+    workgroup goes from one to the next with its flags set."""
+    B, T = 96, 40
+    rng, c, q, parents, n_tok = setup(50, TYPES[kt], 128, 8, 8, 16, [(7 * b) % 40 for b in range(B)], T)
+    q = bf16(q)
+    parents[:] = np.arange(T) - 1
+    want = tree_f64(q, c, parents, n_tok, 0.08, narrow)
+    hit = np.zeros(want[0].shape, bool)
+    dims = slice(40, 41) if kt == "f16" else slice(32, 64)
+    o = {"f16": 80, "q4_0": 18}[kt]
+    for b in range(B):
+        for h in range(8):
+            t = int(rng.integers(1, T))
+            p, i = c.place(b, int(c.rows[b]) + t)
+            c.view(c.v)[p, i, h, o:o + 2] = (0x00, 0x7C)
+            hit[b, t:, h, dims] = True
+    got, _ = on_gpu(torch_gpu, q, c, parents, n_tok, 0.08, narrow)
+    assert not np.isfinite(got[hit]).any()
+    assert np.all(np.abs(got - want[0])[~hit] <= want[2][~hit])

@@ -21,7 +21,6 @@ struct TreeArgs {
     float scale;
     uint32_t k_page, k_row, v_page, v_row;  // strides, below 2^32
     UDivFlat d_g, d_wgs, d_h, d_q;  // by the group, the workgroups, the heads, the tokens
-    uint32_t least;           // tiles that a workgroup takes at least
     int32_t max_ptiles;       // pair tiles of a sequence with n_q tokens
     int32_t part_pairs;       // pairs of a part
     float* part_o;            // [parts][part_pairs][D]
@@ -198,7 +197,7 @@ XQ_DEV uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirs
 // The units of all sequences dealt to the workgroups in order, `per` each.
 struct Deal {
     uint32_t units, per;
-    XQ_DEV Deal(uint32_t n, const UDivFlat& d_wgs, uint32_t least) : units(n), per(uniform(max(d_wgs.quot(n + d_wgs.d - 1), least))) {}
+    XQ_DEV Deal(uint32_t n, const UDivFlat& d_wgs) : units(n), per(uniform(max(d_wgs.quot(n + d_wgs.d - 1), 1u))) {}
     XQ_DEV uint32_t first(uint32_t w) const { return uniform((uint32_t)min((uint64_t)w * per, (uint64_t)units)); }
     XQ_DEV uint32_t owner(uint32_t u) const { return u / per; }  // the workgroup that has unit u
 };
@@ -270,10 +269,10 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
     asm volatile("" ::"s"(a.pg.rows), "s"(a.n_tok), "s"(a.pg.table), "s"(a.parents), "s"(a.q), "s"(a.pg.k), "s"(a.pg.v), "s"(a.pg.k_head),
                  "s"(a.pg.v_head), "s"(a.q_nb1), "s"(a.q_nb2), "s"(a.q_nb3), "s"(a.pg.table_cols), "s"(a.pg.n_pages), "s"(a.pg.row_limit),
                  "s"(a.pg.n_head_kv), "s"(a.pg.d_page.m), "s"(a.n_q), "s"(a.G), "s"(a.B), "s"(a.scale), "s"(a.k_page), "s"(a.v_row),
-                 "s"(a.d_g.m), "s"(a.d_wgs.m), "s"(a.least));
+                 "s"(a.d_g.m), "s"(a.d_wgs.m));
     const uint32_t w = xcd_remap(blockIdx.x, a.d_wgs.d);
     SeqChunk<PW, TR> seqs;
-    const Deal deal(seqs.total(a), a.d_wgs, a.least);
+    const Deal deal(seqs.total(a), a.d_wgs);
     uint32_t u = deal.first(w);
     const uint32_t u_end = deal.first(w + 1);
     while (u < u_end) {
@@ -302,7 +301,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
             const uint32_t r = t * TR + lane;
             page = ~0u;
             in = 0;
-            if (t < t_last && r < (uint32_t)end && (TR == 64 || lane < TR)) {
+            if (t < t_last && r < (uint32_t)end) {
                 const uint32_t c = a.pg.d_page.quot(r);
                 page = (uint32_t)a.pg.table[(int64_t)b * a.pg.table_cols + c];
                 in = r - c * a.pg.d_page.d;
@@ -521,7 +520,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
             if (tid == 0) sBad[(t + 1) & 1] = 0;
 
             // which of the tile's rows each pair sees
-            const bool careful = (t + 1) * TR > (uint32_t)held || now != ~0ull >> (64 - TR);
+            const bool careful = (t + 1) * TR > (uint32_t)held || now != ~0ull;
             uint64_t sees[MT];
             if (careful) {
                 // ancestors by doubling: lane i is token i
@@ -548,7 +547,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 }
             }
             if constexpr (PARTS == 2 || SCALED) {
-                const int e = wave_max_int(sEv[lane % TR]);
+                const int e = wave_max_int(sEv[lane]);
                 if (e > e_run) {
                     const float f = ldexpf(1.0f, e_run - e);
 #pragma unroll
@@ -840,7 +839,8 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                         f4t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int x = g * WR; x < g * WR + WR; ++x) {
-                            if (sM[x][q] != -INFINITY) l = fmaf(sL[x][q], __builtin_amdgcn_exp2f(sM[x][q] - mm), l);
+                            // (a wave without a maximum: its sum is 0, or NaN by a NaN score)
+                            l = fmaf(sL[x][q], sM[x][q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[x][q] - mm), l);
                             o += *(const f4t*)(mg + (16 * x + p) * C::MS + d);
                         }
                         emit(pair, d, o, mm, l, d == 0);
@@ -858,6 +858,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     for (int n = 0; n < ND; ++n) emit(p, 16 * n + 4 * lg, acc[m][n], m_run[m], l, n == 0 && lg == 0);
                 }
             }
+            __syncthreads();  // every wave has read the last tile's flags before the next segment clears them
         }
     }
 }
@@ -874,7 +875,7 @@ __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
     const uint32_t bt = a.d_h.quot(row), h = row - bt * a.d_h.d;
     const uint32_t b = a.d_q.quot(bt), t = bt - b * a.d_q.d;
     SeqChunk<PW, TR> seqs;
-    const Deal deal(seqs.total(a), a.d_wgs, a.least);
+    const Deal deal(seqs.total(a), a.d_wgs);
     const bool real = b < (uint32_t)a.B;
     while (real && (uint32_t)seqs.b0 + 64 <= b) seqs.load(a, seqs.b0 + 64, seqs.last());
     const int sl = real ? (int)b - seqs.b0 : 0;
@@ -897,7 +898,10 @@ __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
             const int64_t at = part0 + (int64_t)min(x0 + NG * i, n - 1) * a.part_pairs;
             ml[i] = a.part_ml[at];
             y[i] = *(const f4t*)(a.part_o + at * D + d);
-            if (x0 + NG * i >= n) ml[i].x = -INFINITY;
+            if (x0 + NG * i >= n) {  // not a part: no weight, and nothing that a product could make NaN
+                ml[i] = make_float2(-INFINITY, 0.0f);
+                y[i] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+            }
         }
         float top = m;
 #pragma unroll
@@ -908,8 +912,7 @@ __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
         m = top;
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
-            if (ml[i].x == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
+            const float w = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - top);
             l = fmaf(ml[i].y, w, l);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(y[i][e], w, o[e]);
@@ -947,41 +950,13 @@ __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
     }
 }
 
-static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, PagesView* pg) {
-    if (!q || !cache || !dst) return failf(XQ_ERR_BAD_ARG, "null argument");
-    if (q->type != XQ_TYPE_F32 && q->type != XQ_TYPE_BF16) return failf(XQ_ERR_UNSUPPORTED, "q must be F32 or BF16");
-    if (dst->type != q->type) return failf(XQ_ERR_UNSUPPORTED, "dst must have q's type");
-    const int64_t D = q->ne[0];
-    if (D != 128 && D != 256) return failf(XQ_ERR_UNSUPPORTED, "head dim %lld not in {128, 256}", (long long)D);
-    for (int i = 1; i < 4; ++i)
-        if (q->ne[i] < 1 || q->ne[i] > 0x7fffffff) return failf(XQ_ERR_BAD_SHAPE, "bad ne");
-    const int64_t T = q->ne[1], H = q->ne[2], B = q->ne[3];
-    if (T > kTreeMax) return failf(XQ_ERR_UNSUPPORTED, "more than 64 tokens of a sequence");
-    if (dst->ne[0] != D || dst->ne[1] != H || dst->ne[2] != T || dst->ne[3] != B)
-        return failf(XQ_ERR_BAD_SHAPE, "dst must be [D, n_head, n_q, n_seq]");
-    const size_t es = type_size(q->type);
-    if (q->nb[0] != es || dst->nb[0] != es) return failf(XQ_ERR_UNSUPPORTED, "q/dst elements must be contiguous");
-    if (!elem_aligned(q, es, 1) || !aligned(q->data, es)) return failf(XQ_ERR_UNSUPPORTED, "misaligned q");
-    if (!elem_aligned(dst, 16, 1) || !aligned(dst->data, 16))
-        return failf(XQ_ERR_UNSUPPORTED, "dst strides and pointer must be multiples of 16 bytes");
-    const xq_status st = pages_check(cache, D, 0, B, kF16 | kE5M2 | kQ8 | kQ4, pg);
-    if (st != XQ_OK) return st;
-    for (const xq_tensor* t : {&cache->k, &cache->v})
-        if (t->nb[1] >> 32 || t->nb[3] >> 32) return failf(XQ_ERR_UNSUPPORTED, "row and page strides must be below 2^32 bytes");
-    const int64_t Hkv = cache->k.ne[2];
-    if (H % Hkv) return failf(XQ_ERR_BAD_SHAPE, "n_head %% n_head_kv != 0");
-    if (H / Hkv > 32) return failf(XQ_ERR_UNSUPPORTED, "GQA group above 32");
-    if (B * T * H >= (int64_t)1 << 23) return failf(XQ_ERR_UNSUPPORTED, "2^23 query rows or more");
-    return XQ_OK;
-}
-
 // The kernel variant, workgroups and workspace of a call: of its shapes alone.
 struct TreePlan {
     int form;                 // index into the forms below
     int pw, tr;               // pairs of a workgroup, KV rows of a tile
-    uint32_t wgs, least;
+    uint32_t wgs;
     int32_t max_ptiles, part_pairs;
-    int64_t parts;
+    int64_t units, parts;     // units: those that the table could hold, at most
     size_t ml_at, bytes;
 };
 // Forms by the pairs (tokens x group) of a KV head: up to 16, 32: the waves share the rows;
@@ -1037,17 +1012,46 @@ static TreePlan tree_plan(const xq_tensor* q, const xq_kv_pages* c) {
     P.max_ptiles = (int32_t)cdiv(pairs, P.pw);
     P.part_pairs = (int32_t)(pairs < P.pw ? pairs : P.pw);
     const int64_t segs = B * Hkv * P.max_ptiles;
-    // units that the table could hold, at most
-    const int64_t units = (cdiv((int64_t)c->table_cols * c->k.ne[1], P.tr) + kStart) * segs;
+    const int64_t limit = (int64_t)c->table_cols * c->k.ne[1];
+    P.units = (cdiv(limit < 0x7fffff00 ? limit : 0x7fffff00, P.tr) + kStart) * segs;
     int64_t wgs = 256 * per_cu;
-    if (wgs > units) wgs = units;
+    if (wgs > P.units) wgs = P.units;
     P.wgs = (uint32_t)wgs;
-    P.least = 1;
     P.parts = wgs + segs;
     const size_t o = (size_t)P.parts * P.part_pairs * D * 4;
     P.ml_at = (o + 255) / 256 * 256;
     P.bytes = P.ml_at + (size_t)P.parts * P.part_pairs * 8;
     return P;
+}
+
+static xq_status tree_check(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, PagesView* pg) {
+    if (!q || !cache || !dst) return failf(XQ_ERR_BAD_ARG, "null argument");
+    if (q->type != XQ_TYPE_F32 && q->type != XQ_TYPE_BF16) return failf(XQ_ERR_UNSUPPORTED, "q must be F32 or BF16");
+    if (dst->type != q->type) return failf(XQ_ERR_UNSUPPORTED, "dst must have q's type");
+    const int64_t D = q->ne[0];
+    if (D != 128 && D != 256) return failf(XQ_ERR_UNSUPPORTED, "head dim %lld not in {128, 256}", (long long)D);
+    for (int i = 1; i < 4; ++i)
+        if (q->ne[i] < 1 || q->ne[i] > 0x7fffffff) return failf(XQ_ERR_BAD_SHAPE, "bad ne");
+    const int64_t T = q->ne[1], H = q->ne[2], B = q->ne[3];
+    if (T > kTreeMax) return failf(XQ_ERR_UNSUPPORTED, "more than 64 tokens of a sequence");
+    if (dst->ne[0] != D || dst->ne[1] != H || dst->ne[2] != T || dst->ne[3] != B)
+        return failf(XQ_ERR_BAD_SHAPE, "dst must be [D, n_head, n_q, n_seq]");
+    const size_t es = type_size(q->type);
+    if (q->nb[0] != es || dst->nb[0] != es) return failf(XQ_ERR_UNSUPPORTED, "q/dst elements must be contiguous");
+    if (!elem_aligned(q, es, 1) || !aligned(q->data, es)) return failf(XQ_ERR_UNSUPPORTED, "misaligned q");
+    if (!elem_aligned(dst, 16, 1) || !aligned(dst->data, 16))
+        return failf(XQ_ERR_UNSUPPORTED, "dst strides and pointer must be multiples of 16 bytes");
+    const xq_status st = pages_check(cache, D, 0, B, kF16 | kE5M2 | kQ8 | kQ4, pg);
+    if (st != XQ_OK) return st;
+    for (const xq_tensor* t : {&cache->k, &cache->v})
+        if (t->nb[1] >> 32 || t->nb[3] >> 32) return failf(XQ_ERR_UNSUPPORTED, "row and page strides must be below 2^32 bytes");
+    const int64_t Hkv = cache->k.ne[2];
+    if (H % Hkv) return failf(XQ_ERR_BAD_SHAPE, "n_head %% n_head_kv != 0");
+    if (H / Hkv > 32) return failf(XQ_ERR_UNSUPPORTED, "GQA group above 32");
+    if (B >> 23 || H >> 23 || B * T * H >= (int64_t)1 << 23) return failf(XQ_ERR_UNSUPPORTED, "2^23 query rows or more");
+    // numbers of units are 32-bit (and divided as 31-bit ones)
+    if (tree_plan(q, cache).units >= (int64_t)1 << 30) return failf(XQ_ERR_UNSUPPORTED, "a table of 2^30 tiles of work or more");
+    return XQ_OK;
 }
 
 }  // namespace xq
@@ -1090,7 +1094,6 @@ xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t
     a.n_q = (int32_t)q->ne[1], a.H = (int32_t)q->ne[2], a.B = (int32_t)q->ne[3];
     a.G = a.H / a.pg.n_head_kv;
     a.d_g = UDivFlat((uint32_t)a.G), a.d_wgs = UDivFlat(P.wgs), a.d_h = UDivFlat((uint32_t)a.H), a.d_q = UDivFlat((uint32_t)a.n_q);
-    a.least = P.least;
     a.max_ptiles = P.max_ptiles, a.part_pairs = P.part_pairs;
     a.part_o = (float*)workspace, a.part_ml = (float2*)((uint8_t*)workspace + P.ml_at);
     const bool narrow = q->type == XQ_TYPE_BF16;

@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256) void pages_release_kernel(int32_t* table, int3
 
 static xq_status pools_check(const xq_tensor* pools, int32_t n_pools, int32_t* page_rows, int32_t* n_pages) {
     if (!pools) return failf(XQ_ERR_BAD_ARG, "null pools");
-    if (n_pools < 1 || n_pools > 65535) return failf(XQ_ERR_BAD_ARG, "n_pools must be in [1, 65535]");
+    if (n_pools < 1 || n_pools > 1024) return failf(XQ_ERR_BAD_ARG, "n_pools must be in [1, 1024]");
     for (int32_t i = 0; i < n_pools; ++i) {
         const xq_tensor& t = pools[i];
         const size_t ts = type_size(t.type);
@@ -424,6 +424,10 @@ xq_status xq_kv_pages_compact(const xq_tensor* pools, int32_t n_pools, const int
     if (rows_out == rows) return failf(XQ_ERR_BAD_ARG, "rows_out must not be rows");
     for (const void* x : {(const void*)table, (const void*)rows, (const void*)path, (const void*)n_path, (const void*)rows_out})
         if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
+    // (its rows would be moved twice, by waves that do not wait for each other)
+    for (int32_t i = 0; i < n_pools; ++i)
+        for (int32_t j = 0; j < i; ++j)
+            if (pools[i].data == pools[j].data) return failf(XQ_ERR_BAD_ARG, "pools %d and %d are one", j, i);
     const int64_t lim = (int64_t)table_cols * page_rows;
     for (int32_t i0 = 0; i0 < n_pools; i0 += kPoolsPerLaunch) {
         const int32_t m = n_pools - i0 < kPoolsPerLaunch ? n_pools - i0 : kPoolsPerLaunch;

@@ -39,7 +39,6 @@ struct RopeArgs {
 
 constexpr int kRopeBatch = 4;  // units whose loads a wave has in flight
 
-typedef uint16_t u16e __attribute__((aligned(2)));
 typedef uint32_t u32x2e __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f4e __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4f __attribute__((ext_vector_type(4), aligned(4)));
@@ -231,6 +230,8 @@ static xq_status rope_check(const xq_tensor* q, const xq_tensor* k, const xq_ten
         if (q->ne[i] < 1 || q->ne[i] > 0x7fffffff) return failf(XQ_ERR_BAD_SHAPE, "bad ne");
     const int64_t T = q->ne[1], H = q->ne[2], B = q->ne[3], Hkv = k->ne[2];
     if (Hkv < 1 || Hkv > 0x7fffff || H > 0x7fffff) return failf(XQ_ERR_BAD_SHAPE, "bad head counts");
+    // (a wave each at least; a grid holds below 2^32 threads)
+    if (T * B >= (int64_t)1 << 26) return failf(XQ_ERR_UNSUPPORTED, "2^26 tokens or more");
     for (const xq_tensor* t : {k, v})
         if (t->ne[0] != D || t->ne[1] != T || t->ne[2] != Hkv || t->ne[3] != B)
             return failf(XQ_ERR_BAD_SHAPE, "k/v must be [D, n_q, n_head_kv, n_seq]");
@@ -303,7 +304,6 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
     if (upw > units) upw = units;
     a.units_part = (int32_t)upw;
     const int64_t parts = cdiv(units, upw);
-    if (tokens * parts > 0x7ffffff0) return failf(XQ_ERR_UNSUPPORTED, "too many tokens for one call");
     a.n_waves = (uint32_t)(tokens * parts);
     a.d_parts = UDivFlat((uint32_t)parts), a.d_q = UDivFlat((uint32_t)a.n_q);
     a.log2_rate = p->n_rot ? -2.0 / p->n_rot * log2((double)p->freq_base) : 0.0;

@@ -111,8 +111,9 @@ def _on(stream, *tensors):
         raise ValueError(f"device tensors are needed, got {dev}")
     if stream is not None and stream.device != dev:
         raise ValueError(f"stream of {stream.device}, tensors on {dev}")
-    with torch.cuda.device(dev):
-        yield ctypes.c_void_p((stream or torch.cuda.current_stream(dev)).cuda_stream)
+    # (a workspace made inside belongs to the stream that uses it)
+    with torch.cuda.device(dev), torch.cuda.stream(stream):
+        yield ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _space(nbytes, workspace, like):
