@@ -1,4 +1,34 @@
 // xq_fa_tree.hip — attention of drafted tokens (a tree, a chain, one token) over the paged cache.
+//
+// Pair p of a KV head is (token p / G, query head p % G of the group): all pairs of a sequence
+// and KV head read the same rows, so one workgroup takes up to 16..256 of them and a row leaves
+// HBM once. With x = scale log2(e) q.k over the rows that a pair sees and any m near their
+// maximum,
+//   O = sum_r 2^(x_r - m) v_r / sum_r 2^(x_r - m),    lse = (m + log2 sum) / log2(e):
+// the sums run over the rows tile by tile, and sums with another m join by the factor 2^(m' - m).
+//
+// A tile is 64 rows. Its pieces (16 bytes a thread) are asked for one tile ahead into registers,
+// become f16 in an LDS image [row][D], and go through 16x16x32 matrix products: scores as
+// K Q^T (a lane then holds four rows of one pair, as the second product wants its weights),
+// O^T as V^T P^T with V's columns read transposed from the image. The visible own rows are a
+// 64-bit ancestor mask per token, formed by pointer doubling in the tiles that hold own rows;
+// all other tiles carry no mask. A sequence's tiles are dealt to a fixed number of workgroups
+// (SeqWork, Deal: from the device's rows and token counts, so a captured graph follows them); a
+// segment that several workgroups shared leaves parts that fa_tree_join adds up.
+//
+// Bound by: HBM while few pairs share a row (decode of 32 x up to 8000 f16 rows, 16/8 heads of
+// 128: 59 us, 4.7 TB/s of the 4.9 of a large copy); vector issue (conversion, softmax) between;
+// matrix and vector issue together at 256 pairs (64 tokens, 4 x 32000 f16 rows, 32/8 heads: 187 us,
+// 3.1 TB/s and 0.74 PFLOP/s of the 1.22 of a large f16 matrix product). A second LDS image, so that
+// one barrier per tile is enough, gave nothing there (188 us; f32 Q 102 against 92), nor did
+// wave priorities that hold the waves of a SIMD apart (188). Small calls cost 14 us: two launches
+// and the five dependent reads (arguments, rows, table with Q, K with V, parts) of a lone tile.
+//
+// Roundings: scores, maxima, sums, accumulators f32. The matrix cores take f16 operands: BF16 Q
+// goes in exactly (8 bits, scaled into range by a power of two per row), F16 and E5M2 rows
+// exactly; beside BF16 Q, d * q of q8_0 / q4_0 rows and the weights are rounded to f16's 11 bits
+// (2^-12 relative each, below the 2^-9 of the bf16 result, for half or a third of the products);
+// beside F32 Q every operand is a high and a low f16, 22 bits.
 #include <type_traits>
 
 #include "xq_kv_codec.h"
@@ -59,7 +89,7 @@ struct TreeCfg {
     static constexpr int RT = RW >= 32 ? 2 : 1;                             // 16-row score tiles of a wave at a time
     static constexpr int PIECES = TR * PPR;                                 // of a tile and tensor
     static constexpr int NPT = (PIECES + 64 * NW - 1) / (64 * NW);          // per thread
-    static constexpr int RS = 2 * D + 32;                                   // image rows, bytes: 8 banks of 64 apart
+    static constexpr int RS = 2 * D + 32;                                   // image rows, bytes: 8 banks of 64 apart, so that 16 rows' operand reads meet no bank twice at a time
     static constexpr int PB = TR * RS;                                      // one part of K or V
     static constexpr int IMG = 2 * PARTS * PB;
     static constexpr int PW = 16 * MT * (NW / WR);                          // pairs of a workgroup
@@ -172,6 +202,8 @@ XQ_DEV void products_done() {
 // A segment is one (sequence, KV head, pair tile); its units of work are its row tiles after
 // kStart units that stand for what a workgroup spends on it before its first tile (three
 // dependent loads, Q, and the state written at the end: the time of two to four tiles).
+// Dealing by tiles alone (0): 32 fp8 chats 37.7 us against 32.4, 16 sequences of 25 tokens 79
+// against 66; 2, 4 and 5 are within 1 % of 3 over 40 calls of all sizes.
 constexpr uint32_t kStart = 3;
 
 // Work of sequence b: its rows, tokens, row tiles, pair tiles and units.
@@ -866,6 +898,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 // Joins the parts of the segments that more than one workgroup had. NWR waves per row
 // (sequence, token, head): D / 4 lanes read a part's dims, NG parts at a time and
 // four of those in flight, each group of lanes with a running maximum of its own.
+// Bound by the launch and two memory round trips (4 us of a small call).
 template <int D, bool NARROW, int PW, int TR, int NWR>
 __global__ __launch_bounds__(256) void fa_tree_join(TreeArgs a) {
     constexpr int L = D / 4, NG = 64 * NWR / L, UN = 4, RB = 4 / NWR;
@@ -960,7 +993,11 @@ struct TreePlan {
     size_t ml_at, bytes;
 };
 // Forms by the pairs (tokens x group) of a KV head: up to 16, 32: the waves share the rows;
-// above: they share the pairs, up to 64, 128, 256 of a workgroup.
+// above: they share the pairs, up to 64, 128, 256 of a workgroup. The smallest that holds the
+// pairs, as products of absent pairs cost as much as others, and the most that share a row.
+// Decode of 24/4 heads of 256, 8 x 16000 q8_0 rows: 73 us in the form of 16, 81 in that of 64
+// (f32 Q, 4 x 32000 rows: 118; 175 in that of 32; 194); 64 pairs over f16 rows: 36 us, 40 in the
+// form of 128 (f32 Q over q4_0: 52, 69); 256 pairs: 186 us, 218 in two tiles of 128.
 template <int MT_, int WR_, int NW_> struct TreeForm { static constexpr int MT = MT_, WR = WR_, NW = NW_; };
 template <int D, bool NARROW, typename F>
 static void tree_form(int form, F f) {
@@ -1104,6 +1141,8 @@ xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t
         constexpr bool NARROW = decltype(nar)::value;
         using C = TreeCfg<KT, D, NARROW, F::MT, F::WR, F::NW>;
         launch("fa_tree", fa_tree_kernel<KT, D, NARROW, F::MT, F::WR, F::NW>, dim3(P.wgs), dim3(64 * F::NW), s, a);
+        // four waves per row while those find room together: 768 rows of 256 38.7 us (one wave each
+        // 42.5), 1024 rows of 128 alike, 4096 rows 20.2 (16.2), 12800 rows 75 (66)
         const uint32_t rows = (uint32_t)((int64_t)a.B * a.n_q * a.H);
         if (rows <= 2048)
             launch("fa_tree_join", fa_tree_join<D, NARROW, C::PW, C::TR, 4>, dim3(rows), dim3(256), s, a);

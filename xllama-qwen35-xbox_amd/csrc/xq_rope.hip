@@ -298,8 +298,10 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
     a.n_q = (int32_t)q->ne[1], a.H = (int32_t)q->ne[2], a.Hkv = (int32_t)k->ne[2];
     a.units_q = (int32_t)cdiv(a.H, rpu), a.units_kv = (int32_t)cdiv(a.Hkv, rpu);
     const int64_t tokens = q->ne[1] * q->ne[3], units = a.units_q + 2 * (int64_t)a.units_kv;
-    // one unit per wave while that leaves CUs without a wave, then up to all of a token's
-    int64_t upw = tokens * units / 8192;
+    // one unit per wave while that leaves CUs without a wave, then up to all of a token's: a wave
+    // forms the angles once, but needs company. 2 x 4097 bf16 prompt tokens of 24/4 heads of 256, shared
+    // out to about 8192 waves 65.7 us, 16384 64.4, 32768 70.2, 65536 84.3
+    int64_t upw = tokens * units / 16384;
     if (upw < 1) upw = 1;
     if (upw > units) upw = units;
     a.units_part = (int32_t)upw;
