@@ -400,7 +400,8 @@ typedef struct xq_rope_params {
  * and turned by its token's position; queries go to q_out, keys and values to the
  * rows rows[b] + i of their sequence's pages.
  *   q      F32|BF16 [D, n_q, n_head, n_seq], k, v the same type [D, n_q, n_head_kv, n_seq];
- *          elements contiguous, other strides free
+ *          elements contiguous, other strides free (head strides below 2^32 bytes); fewer
+ *          than 2^26 tokens in all
  *   positions I32 [n_seq][n_q] (device): the position that token i of sequence b turns by
  *   n_tok  I32 [n_seq] (device), or NULL: all n_q. Tokens from n_tok[b] on are padding:
  *          neither read nor written
@@ -431,9 +432,13 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
  *   dst     q's type [D, n_head, n_q, n_seq], strides multiples of 16 bytes
  *   lse     F32 [n_seq][n_q][n_head], natural logarithm of the softmax sum, or NULL
  *   scale   on the scores; finite
+ * Fewer than 2^23 query rows (n_q * n_head * n_seq); row and page strides of the pools below
+ * 2^32 bytes; a table of fewer than 2^30 tiles of 64 rows over all sequences and KV heads.
  * Scores and values are those of the decoded cache, sums in f32. F32 q: operands enter
- * the matrix cores as f16 hi + lo, about 22 bits. BF16 q: as one f16 (weights, and
- * q8_0 / q4_0 values d * q, rounded to 11 bits; such a value beyond 65504 is infinite).
+ * the matrix cores as f16 hi + lo, about 22 bits (q8_0 / q4_0 as exact integers, or as d * q in
+ * both parts). BF16 q: as one f16 (weights, and q8_0 / q4_0 values d * q, rounded to 11 bits;
+ * such a value beyond 65504 is infinite). dst is not q's memory. Calls that may run at the same
+ * time need a workspace each.
  * A row that a token does not see has no part in its result, whatever it holds; a
  * non-finite element of a row that it sees makes what it reaches non-finite.
  * A sink joins by xq_fa_lse_merge, as a part with OUT 0 and LSE the sink. */
@@ -442,8 +447,9 @@ xq_status xq_fa_tree_workspace(const xq_tensor* q, const xq_kv_pages* cache, con
 xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t* parents, const int32_t* n_tok,
                      xq_tensor* dst, float* lse, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* The pages themselves. `pools` are the pools (K and V of every layer, host array)
- * that one table addresses; all have the same page_rows and n_pages. All other
+/* The pages themselves. `pools` are the pools (K and V of every layer, host array, at most
+ * 1024, head dim a multiple of 32, pages below 2^31 bytes) that one table addresses; all have
+ * the same page_rows and n_pages. All other
  * arrays are device memory. refs[p] is the number of sequences that hold page p: 0 is
  * free. Entries of a table that hold no page are -1.
  *
@@ -455,7 +461,8 @@ xq_status xq_kv_pages_copy(const xq_tensor* pools, int32_t n_pools, const int32_
 /* compact: after a tree's verify the rows of the accepted path move to the front:
  * row rows[b] + path[b * path_cols + j] of sequence b becomes row rows[b] + j, for
  * j < min(n_path[b], path_cols), and rows_out[b] = rows[b] + that number. A path rises
- * (path[j] < path[j + 1]); an entry below j is skipped. rows_out is not rows. */
+ * (path[j] < path[j + 1]); an entry below j is skipped. rows_out is not rows; no pool is
+ * given twice; at most 65535 sequences. */
 xq_status xq_kv_pages_compact(const xq_tensor* pools, int32_t n_pools, const int32_t* table, const int32_t* rows,
                               int32_t n_seq, int32_t table_cols, const int32_t* path, const int32_t* n_path,
                               int32_t path_cols, int32_t* rows_out, void* stream);
@@ -481,7 +488,8 @@ xq_status xq_kv_pages_fork(const xq_tensor* pools, int32_t n_pools, int32_t* tab
                            int32_t* done, void* workspace, size_t workspace_bytes, void* stream);
 
 /* release: the sequences seqs[0..n) hold no page and no rows any more; refs of each of
- * their pages falls by one. An id out of range, or named again, releases nothing. */
+ * their pages falls by one. An id out of range, or named again, releases nothing; n at most
+ * 65535. */
 xq_status xq_kv_pages_release(int32_t* table, int32_t* rows, int32_t* refs, int32_t n_seq, int32_t table_cols,
                               int32_t n_pages, const int32_t* seqs, int32_t n, void* stream);
 
