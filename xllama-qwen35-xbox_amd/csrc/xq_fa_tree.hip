@@ -17,7 +17,7 @@
 // segment that several workgroups shared leaves parts that fa_tree_join adds up.
 //
 // Bound by: HBM while few pairs share a row (decode of 32 x up to 8000 f16 rows, 16/8 heads of
-// 128: 59 us, 4.7 TB/s of the 4.9 of a large copy); vector issue (conversion, softmax) between;
+// 128, two input sets in turn: 59 us, 4.7 TB/s of the 4.9 of a large copy); vector issue (conversion, softmax) between;
 // matrix and vector issue together at 256 pairs (64 tokens, 4 x 32000 f16 rows, 32/8 heads: 187 us,
 // 3.1 TB/s and 0.74 PFLOP/s of the 1.22 of a large f16 matrix product). A second LDS image, so that
 // one barrier per tile is enough, gave nothing there (188 us; f32 Q 102 against 92), nor did
