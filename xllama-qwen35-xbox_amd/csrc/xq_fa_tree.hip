@@ -27,7 +27,7 @@
 // Roundings: scores, maxima, sums, accumulators f32. The matrix cores take f16 operands: BF16 Q
 // goes in exactly (8 bits, scaled into range by a power of two per row), F16 and E5M2 rows
 // exactly; beside BF16 Q, d * q of q8_0 / q4_0 rows and the weights are rounded to f16's 11 bits
-// (2^-12 relative each, below the 2^-9 of the bf16 result, for half or a third of the products);
+// (2^-11 relative each, below the 2^-8 of the bf16 result, for half or a third of the products);
 // beside F32 Q every operand is a high and a low f16, 22 bits.
 #include <type_traits>
 
