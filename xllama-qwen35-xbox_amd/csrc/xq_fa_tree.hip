@@ -71,6 +71,8 @@ typedef float f4el __attribute__((ext_vector_type(4), aligned(4)));
 constexpr float kTreeLog2e = 1.4426950408889634f, kTreeLn2 = 0.6931471805599453f;
 constexpr float kTreeLazy = 8.0f;      // base-2 headroom before the running maximum moves
 constexpr float kTreeOff = -7.0f;      // weights are 2^(x - max + 7), in (0, 2^15]: f16 keeps small ones normal
+constexpr float kTreeHigh = 6.0f;      // and where block scales take part, the largest lies above 2^11 (SCALED) or 2^12:
+                                       // the reference stays this far below the maximum it was taken from
 
 template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 struct TreeCfg {
@@ -82,6 +84,11 @@ struct TreeCfg {
     static constexpr bool SCALED = QUANT && !NARROW && WR > 1;
     static constexpr int PARTS = QUANT && !NARROW && !SCALED ? 2 : 1;       // f16 parts of a cached value
     static constexpr int QP = NARROW ? 1 : 2;                               // f16 parts of Q and of the weights
+    // The weights become f16 parts times a power of two of V's row, that of its largest block scale. The
+    // reference that keeps them in f16's range is then a maximum of x plus that power over the rows that
+    // the pair sees: a row of which it sees nothing, or next to nothing, costs the others no bits,
+    // whatever its scales.
+    static constexpr bool BY_V = PARTS == 2 || SCALED;
     static constexpr int EL = KT == XQ_TYPE_F16 ? 8 : KT == XQ_TYPE_Q4_0 ? 32 : 16;  // elements of a 16-byte piece
     static constexpr int PPR = D / EL;                                      // pieces per row
     static constexpr int TR = 64;                                           // KV rows of a tile (a lane per row)
@@ -133,16 +140,6 @@ XQ_DEV float across_rows_sum(float x) {
     x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(q[0]) + __uint_as_float(q[1]);
-}
-
-// The largest over the wave, in a scalar register.
-XQ_DEV int wave_max_int(int x) {
-    x = max(x, dpp_i<0xB1>(x));
-    x = max(x, dpp_i<0x4E>(x));
-    x = max(x, dpp_i<0x141>(x));
-    x = max(x, dpp_i<0x140>(x));
-    const int a = max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16));
-    return max(a, max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
 
 // Nonzero halves (0x8000 each) of w that are Inf or NaN.
@@ -282,7 +279,7 @@ template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES)) void fa_tree_kernel(TreeArgs a) {
     using C = TreeCfg<KT, D, NARROW, MT, WR, NW>;
     constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW, TR = C::TR, RT = C::RT;
-    constexpr bool QUANT = C::QUANT, SCALED = C::SCALED;
+    constexpr bool QUANT = C::QUANT, SCALED = C::SCALED, BY_V = C::BY_V;
     constexpr int KC = PARTS == 2 ? 2 : 4;  // 32-element chunks of K read at once
     constexpr int VC = PARTS == 2 ? 2 : 4;  // 16-element columns of V
     __shared__ __attribute__((aligned(16))) uint8_t img[C::SMEM];
@@ -536,7 +533,6 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 #pragma unroll
             for (int n = 0; n < ND; ++n) acc[m][n] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        int e_run = -1000;  // PARTS 2, SCALED: the accumulators hold their sums times 2^-e_run
         if (tid < 2) sBad[tid] = 0;
 
         for (uint32_t t = t_first; t < t_last; ++t) {
@@ -576,17 +572,6 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                     const uint64_t x = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(anc >> 32), tok[m]) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, tok[m]);
                     uint64_t s = sh >= 64 ? ~0ull : sh >= 0 ? (x << sh) | ((1ull << sh) - 1) : sh > -64 ? x >> -sh : 0ull;
                     sees[m] = s & now;
-                }
-            }
-            if constexpr (PARTS == 2 || SCALED) {
-                const int e = wave_max_int(sEv[lane]);
-                if (e > e_run) {
-                    const float f = ldexpf(1.0f, e_run - e);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int n = 0; n < ND; ++n) acc[m][n] *= f;
-                    e_run = e;
                 }
             }
 #pragma unroll 1
@@ -685,20 +670,27 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 bool over = false;
                 float top[MT];
 #pragma unroll
+                for (int m = 0; m < MT; ++m) top[m] = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    int4 e;
+                    if constexpr (BY_V) e = *(const int4*)(sEv + row0 + 16 * r + 4 * lg);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            top[m] = fmaxf(top[m], BY_V ? fmaf(s[m][r][i], qf[m], (float)(i == 0 ? e.x : i == 1 ? e.y : i == 2 ? e.z : e.w)) : s[m][r][i]);
+                }
+#pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    top[m] = -INFINITY;
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top[m] = fmaxf(top[m], s[m][r][i]);
-                    top[m] *= qf[m];
+                    if constexpr (!BY_V) top[m] *= qf[m];
                     over |= top[m] > m_run[m] + kTreeLazy;
                 }
                 if (__builtin_amdgcn_ballot_w64(over)) {
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const float mt = across_rows_max(top[m]);
-                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) : m_run[m];
+                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) - (BY_V ? kTreeHigh : 0.0f) : m_run[m];
                         const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
                         l_run[m] *= f;
 #pragma unroll
@@ -708,7 +700,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                 }
                 // weights
                 h4t ph[MT][RT], pl[QP == 2 ? MT : 1][QP == 2 ? RT : 1];
-                f4t pw[SCALED ? RT : 1];  // SCALED: the weights times 2^-e_run
+                f4t pw[SCALED ? RT : 1];  // SCALED: the weights, before their block scales
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     const float mu = m_run[m] == -INFINITY ? 0.0f : -(m_run[m] + kTreeOff);
@@ -721,12 +713,12 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
                             l_run[m] += p[i];
                         }
                         if constexpr (SCALED) {
-                            pw[r] = f4t{ldexpf(p[0], -e_run), ldexpf(p[1], -e_run), ldexpf(p[2], -e_run), ldexpf(p[3], -e_run)};
+                            pw[r] = p;
                             continue;
                         }
                         if constexpr (PARTS == 2) {
                             const int4 e = *(const int4*)(sEv + row0 + 16 * r + 4 * lg);
-                            p = f4t{ldexpf(p[0], e.x - e_run), ldexpf(p[1], e.y - e_run), ldexpf(p[2], e.z - e_run), ldexpf(p[3], e.w - e_run)};
+                            p = f4t{ldexpf(p[0], e.x), ldexpf(p[1], e.y), ldexpf(p[2], e.z), ldexpf(p[3], e.w)};
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -810,13 +802,6 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
         if (u < u_end) seqs.load(a, seqs.b0, seqs.before);  // again: not held in registers meanwhile
 
         // ---- the segment's result, or this workgroup's part of it
-        if constexpr (PARTS == 2 || SCALED) {
-            const float f = ldexpf(1.0f, max(e_run, -126));
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < ND; ++n) acc[m][n] *= f;
-        }
         const uint32_t piece = w + (uint32_t)((b * a.pg.n_head_kv + hk) * a.max_ptiles + pt);
         auto emit = [&](int p, int d, f4t o, float mm, float l, bool first) {  // pair p of the segment's tile, dims d..d+3
             if (whole) {
