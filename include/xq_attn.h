@@ -435,9 +435,12 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
  * Fewer than 2^23 query rows (n_q * n_head * n_seq); row and page strides of the pools below
  * 2^32 bytes; a table of fewer than 2^30 tiles of 64 rows over all sequences and KV heads.
  * Scores and values are those of the decoded cache, sums in f32. F32 q: operands enter
- * the matrix cores as f16 hi + lo, about 22 bits (q8_0 / q4_0 as exact integers, or as d * q in
- * both parts). BF16 q: as one f16 (weights, and q8_0 / q4_0 values d * q, rounded to 11 bits;
- * such a value beyond 65504 is infinite). dst is not q's memory. Calls that may run at the same
+ * the matrix cores as f16 hi + lo, 22 bits (q8_0 / q4_0 as exact integers, or as d * q in
+ * both parts); what is far smaller than its like keeps fewer: a weight (on q8_0 / q4_0 pools a
+ * weight times its block scale) is off by up to 2^-36 of the largest that the token has, an
+ * element of q by 2^-39 of its row's largest, a block scale by 2^-32 of its row's largest. BF16 q:
+ * as one f16 (weights, and q8_0 / q4_0 values d * q, rounded to 11 bits; a weight by up to 2^-31
+ * of the largest; a value d * q beyond 65504 is infinite). dst is not q's memory. Calls that may run at the same
  * time need a workspace each.
  * A row that a token does not see has no part in its result, whatever it holds; a
  * non-finite element of a row that it sees makes what it reaches non-finite.

@@ -117,3 +117,23 @@ def test_a_large_scale_of_next_to_no_weight(torch_gpu, form, kt, value, power):
 
     got, lse = on_gpu(torch_gpu, q, c, parents, None, D**-0.5, False)
     check_f32(c, q, parents, D**-0.5, got, lse, unit)
+
+
+@pytest.mark.parametrize("power", [28, 30, 32, 34])
+@pytest.mark.parametrize("kt", ["f16", "e5m2"])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_large_values_of_little_weight(torch_gpu, form, kt, power):
+    """Values of 2^15 and more at a weight of about 2^-power, the others near 2^-6: what they add up
+    to keeps its bits.
+
+    A weight is an f16 high and low part at 2^12 or more for the largest: one is off by 2^-25 / 2^12 of
+    the largest at least, and that is at most the sum of all."""
+    D, H, Hkv, T = FORMS[form]
+    case_note(f"large values {FORMS[form]} {kt} 2^-{power}")
+    c, q, parents = spread_case(80 + form, kt, D, H, Hkv, T, 130, power, 2.0**-6)
+    p, i = c.place(0, 37)
+    big = np.random.default_rng(form).choice([-57344.0, -32768.0, 32768.0, 57344.0], (Hkv, D)).astype(np.float32)
+    c.view(c.v)[p, i] = oracle.quantize(c.kv_type, big).reshape(Hkv, c.rec)
+    v = np.abs(c.values(c.v, 0, 130 + T))
+    got, lse = on_gpu(torch_gpu, q, c, parents, None, D**-0.5, False)
+    check_f32(c, q, parents, D**-0.5, got, lse, lambda w, rows, hk: 2.0**-37 * v[rows, hk].sum(0))

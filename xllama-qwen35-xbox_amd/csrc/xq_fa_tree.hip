@@ -27,8 +27,11 @@
 // Roundings: scores, maxima, sums, accumulators f32. The matrix cores take f16 operands: BF16 Q
 // goes in exactly (8 bits, scaled into range by a power of two per row), F16 and E5M2 rows
 // exactly; beside BF16 Q, d * q of q8_0 / q4_0 rows and the weights are rounded to f16's 11 bits
-// (2^-11 relative each, below the 2^-8 of the bf16 result, for half or a third of the products);
-// beside F32 Q every operand is a high and a low f16, 22 bits.
+// (2^-11 relative each, below the 2^-8 of the bf16 result, for half or a third of the products;
+// d * q below f16's normal range is exact, as d is a multiple of 2^-24);
+// beside F32 Q every operand is a high and a low f16, 22 bits. f16's subnormal step, 2^-24, is
+// what a small operand loses: the powers of two that bring Q's rows, block scales and weights into
+// range set how far below the largest that begins.
 #include <type_traits>
 
 #include "xq_kv_codec.h"
@@ -71,8 +74,9 @@ typedef float f4el __attribute__((ext_vector_type(4), aligned(4)));
 constexpr float kTreeLog2e = 1.4426950408889634f, kTreeLn2 = 0.6931471805599453f;
 constexpr float kTreeLazy = 8.0f;      // base-2 headroom before the running maximum moves
 constexpr float kTreeOff = -7.0f;      // weights are 2^(x - max + 7), in (0, 2^15]: f16 keeps small ones normal
-constexpr float kTreeHigh = 6.0f;      // and where block scales take part, the largest lies above 2^11 (SCALED) or 2^12:
-                                       // the reference stays this far below the maximum it was taken from
+constexpr float kTreeHigh = 6.0f;      // and beside f32 Q the largest lies above 2^12 (SCALED, with its block scale: 2^11):
+                                       // the reference stays this far below the maximum it was taken from, so that
+                                       // a weight's two parts are off by 2^-37 of the largest, or 2^-22 of itself
 
 template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 struct TreeCfg {
@@ -690,7 +694,7 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const float mt = across_rows_max(top[m]);
-                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) - (BY_V ? kTreeHigh : 0.0f) : m_run[m];
+                        const float mn = mt > m_run[m] + kTreeLazy ? ceilf(mt) - (QP == 2 ? kTreeHigh : 0.0f) : m_run[m];
                         const float f = mn == m_run[m] ? 1.0f : __builtin_amdgcn_exp2f(m_run[m] - mn);
                         l_run[m] *= f;
 #pragma unroll
