@@ -6,7 +6,7 @@ import pytest
 import oracle
 from conftest import case_note
 from paged_cases import Cache, ancestors, bf16, tree_f64
-from test_gpu_fa_tree import TYPES, on_gpu, setup
+from test_gpu_fa_tree import TYPES, check, on_gpu, setup
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,21 @@ def test_large_values_of_little_weight(torch_gpu, form, kt, power):
     v = np.abs(c.values(c.v, 0, 130 + T))
     got, lse = on_gpu(torch_gpu, q, c, parents, None, D**-0.5, False)
     check_f32(c, q, parents, D**-0.5, got, lse, lambda w, rows, hk: 2.0**-37 * v[rows, hk].sum(0))
+
+
+@pytest.mark.parametrize("narrow", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("kt", ["f16", "q8_0"])
+@pytest.mark.parametrize("scale,power", [(3e38, -123), (-3e38, -123), (1e-40, 126), (-1e-40, 126), (3e38, 100)])
+def test_scales_at_the_ends_of_f32(torch_gpu, kt, narrow, scale, power):
+    """Scales whose product with log2(e) leaves f32's normal range, and queries that bring the scores
+    back; where nothing can (the last), keys of zeros still score 0."""
+    rng = np.random.default_rng(90)
+    c = Cache(rng, TYPES[kt], 128, 4, 16, [100], [5])
+    x = rng.standard_normal((c.n_pages, 16, 4, 128)).astype(np.float32) * {-123: 2.0**-8, 126: 2.0**5, 100: 0.0}[power]
+    c.view(c.k)[...] = oracle.quantize(c.kv_type, x.astype(np.float32)).reshape(c.n_pages, 16, 4, c.rec)
+    q = bf16((rng.standard_normal((1, 5, 8, 128)) * 2.0**power).astype(np.float32))
+    assert np.isfinite(q).all()
+    parents = (np.arange(5, dtype=np.int32) - 1)[None]
+    scale = float(np.float32(scale))
+    got, lse = on_gpu(torch_gpu, q, c, parents, None, scale, narrow)
+    check(got, lse, tree_f64(q, c, parents, [5], scale, narrow))

@@ -511,8 +511,8 @@ __global__ __launch_bounds__(64 * NW, (TreeCfg<KT, D, NARROW, MT, WR, NW>::WAVES
 #pragma unroll
                     for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(xq[m][c][j]));
                 const int lift = 141 - min((int)(__float_as_uint(across_rows_max(big)) >> 23), 254);
-                // (not below the smallest normal: an unseen score's -inf stays one)
-                qf[m] = fmaxf(ldexpf(fabsf(a.scale) * kTreeLog2e, -lift), 1.17549435e-38f);
+                // (a normal number: an unseen score's -inf stays one, and a score of 0 too)
+                qf[m] = fminf(fmaxf(ldexpf(fabsf(a.scale), -lift) * kTreeLog2e, 1.17549435e-38f), 3.40282347e38f);
 #pragma unroll
                 for (int c = 0; c < NB; ++c)
 #pragma unroll
