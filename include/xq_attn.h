@@ -473,7 +473,8 @@ xq_status xq_kv_pages_compact(const xq_tensor* pools, int32_t n_pools, const int
 /* reserve: each sequence is given pages for rows [0, want[b]) where its table has
  * none, sequence after sequence and column after column, the lowest free page
  * first, until none is left; refs of a page given is 1. got[b] is the number of rows, up
- * to table_cols * page_rows, that the sequence's unbroken first pages hold then. */
+ * to table_cols * page_rows, that the sequence's unbroken first pages hold then. A table has
+ * fewer than 2^32 entries. */
 xq_status xq_kv_pages_reserve_workspace(int32_t n_seq, int32_t n_pages, size_t* bytes);
 xq_status xq_kv_pages_reserve(int32_t* table, int32_t* refs, int32_t n_seq, int32_t table_cols, int32_t n_pages,
                               int32_t page_rows, const int32_t* want, int32_t* got, void* workspace,

@@ -467,6 +467,8 @@ xq_status xq_kv_pages_reserve(int32_t* table, int32_t* refs, int32_t n_seq, int3
     if (st == XQ_OK) st = table_check(n_seq, table_cols);
     if (st != XQ_OK) return st;
     if (page_rows < 1) return failf(XQ_ERR_BAD_ARG, "page_rows must be at least 1");
+    // (the pages that all sequences miss are counted in 32 bits)
+    if ((int64_t)n_seq * table_cols >> 32) return failf(XQ_ERR_UNSUPPORTED, "a table of 2^32 entries or more");
     if (!table || !refs || !want || !got) return failf(XQ_ERR_BAD_ARG, "null pointer");
     for (const void* x : {(const void*)table, (const void*)refs, (const void*)want, (const void*)got})
         if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
