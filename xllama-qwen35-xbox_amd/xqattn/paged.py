@@ -123,7 +123,14 @@ def _space(nbytes, workspace, like):
     return workspace, *_aligned_ptr(workspace)
 
 
+def _memory(pools):
+    return [None if isinstance(p, XqTensor) else p.t for p in pools]
+
+
 def _pools(pools):
+    """Descriptors of the pools; one may be given as its descriptor, its memory is the caller's then."""
+    if not pools:
+        raise ValueError("at least one pool is needed")
     return (XqTensor * len(pools))(*[p if isinstance(p, XqTensor) else p.desc() for p in pools]), len(pools)
 
 
@@ -188,7 +195,7 @@ def kv_pages_copy(pools, src, dst, stream=None):
     _i32("dst", dst)
     _size("dst", dst, src.numel())
     arr, n = _pools(pools)
-    with _on(stream, src, dst, *[p.t for p in pools]) as s:
+    with _on(stream, src, dst, *_memory(pools)) as s:
         _check(load().xq_kv_pages_copy(arr, n, _ptr(src), _ptr(dst), src.numel(), s), "kv_pages_copy")
 
 
@@ -201,7 +208,7 @@ def kv_pages_compact(pools, table, rows, path, n_path, rows_out, stream=None):
     if path.shape[0] != table.shape[0]:
         raise ValueError("path must have one row per sequence")
     arr, n = _pools(pools)
-    with _on(stream, table, rows, path, n_path, rows_out, *[p.t for p in pools]) as s:
+    with _on(stream, table, rows, path, n_path, rows_out, *_memory(pools)) as s:
         _check(load().xq_kv_pages_compact(arr, n, _ptr(table), _ptr(rows), *table.shape, _ptr(path), _ptr(n_path), path.shape[1],
                                           _ptr(rows_out), s), "kv_pages_compact")
 
@@ -234,7 +241,7 @@ def kv_pages_fork(pools, table, rows, refs, parents, children, done, workspace=N
         raise ValueError("refs must hold one number per page")
     n = ctypes.c_size_t(0)
     _check(load().xq_kv_pages_fork_workspace(count, ctypes.byref(n)), "kv_pages_fork_workspace")
-    with _on(stream, table, rows, refs, parents, children, done, workspace, *[p.t for p in pools]) as s:
+    with _on(stream, table, rows, refs, parents, children, done, workspace, *_memory(pools)) as s:
         ws, wp, wn = _space(n.value, workspace, table)
         _check(load().xq_kv_pages_fork(arr, m, _ptr(table), _ptr(rows), _ptr(refs), *table.shape, _ptr(parents), _ptr(children), count,
                                        _ptr(done), ctypes.c_void_p(wp), wn, s), "kv_pages_fork")
