@@ -155,3 +155,32 @@ def test_scales_at_the_ends_of_f32(torch_gpu, kt, narrow, scale, power):
     scale = float(np.float32(scale))
     got, lse = on_gpu(torch_gpu, q, c, parents, None, scale, narrow)
     check(got, lse, tree_f64(q, c, parents, [5], scale, narrow))
+
+
+SMALL = {"f16": -12, "q8_0": -12, "q4_0": -12, "e5m2": -10}
+
+
+def small_case(kt, narrow):
+    """K and V at a power of two where elements or block scales still hold several bits, queries that
+    bring the scores back to 1; the bounds of tree_f64 without its absolute 2^-24."""
+    rng = np.random.default_rng(95)
+    c = Cache(rng, TYPES[kt], 128, 4, 16, [150], [6])
+    for n, buf in enumerate((c.k, c.v)):
+        x = np.random.default_rng(96 + n).standard_normal((c.n_pages, 16, 4, 128)) * 2.0**SMALL[kt]
+        c.view(buf)[...] = oracle.quantize(c.kv_type, x.astype(np.float32)).reshape(c.n_pages, 16, 4, c.rec)
+    q = bf16((rng.standard_normal((1, 6, 8, 128)) * 2.0**-SMALL[kt]).astype(np.float32))
+    parents = (np.arange(6, dtype=np.int32) - 1)[None]
+    out, lse, tol, tol_lse = tree_f64(q, c, parents, [6], 0.09, narrow)
+    if not narrow:
+        tol = tol - 2.0**-24 + 2.0**-24 * (np.abs(out) + tol)
+    return c, q, parents, (out, lse, tol, tol_lse)
+
+
+@pytest.mark.parametrize("kt", list(TYPES))
+@pytest.mark.parametrize("narrow", [False, True], ids=["f32", "bf16"])
+def test_small_values_and_keys(torch_gpu, kt, narrow):
+    c, q, parents, want = small_case(kt, narrow)
+    # (an output of zeros would not pass)
+    assert np.mean(np.abs(want[0]) > want[2]) > (0.6 if narrow else 0.99)
+    got, lse = on_gpu(torch_gpu, q, c, parents, None, 0.09, narrow)
+    check(got, lse, want)
