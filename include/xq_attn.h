@@ -443,7 +443,8 @@ xq_status xq_qk_norm_rope(const xq_tensor* q, const xq_tensor* k, const xq_tenso
  * of the largest; a value d * q beyond 65504 is infinite). dst is not q's memory. Calls that may run at the same
  * time need a workspace each.
  * A row that a token does not see has no part in its result, whatever it holds; a
- * non-finite element of a row that it sees makes what it reaches non-finite.
+ * non-finite element of a row that it sees makes what it reaches non-finite (but a score of
+ * -inf, as BF16 q and a key of -inf give it, is a weight of 0).
  * A sink joins by xq_fa_lse_merge, as a part with OUT 0 and LSE the sink. */
 int xq_supports_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst);
 xq_status xq_fa_tree_workspace(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, size_t* bytes);

@@ -184,3 +184,20 @@ def test_small_values_and_keys(torch_gpu, kt, narrow):
     assert np.mean(np.abs(want[0]) > want[2]) > (0.6 if narrow else 0.99)
     got, lse = on_gpu(torch_gpu, q, c, parents, None, 0.09, narrow)
     check(got, lse, want)
+
+
+@pytest.mark.parametrize("T", [5, 40])
+def test_a_score_of_minus_infinity_is_no_weight(torch_gpu, T):
+    """bf16 Q and a key with an infinite element: where its score is -inf the row has no part, where it
+    is +inf the result is NaN."""
+    _, c, q, parents, n_tok = setup(99, TYPES["f16"], 128, 8, 4, 1, [100], T)
+    q = bf16(q)
+    assert np.all(q[..., 9] != 0)
+    p, i = c.place(0, 37)
+    c.view(c.k)[p, i, :, 18:20] = np.array([np.inf], np.float16).view(np.uint8)
+    got, lse = on_gpu(torch_gpu, q, c, parents, n_tok, 0.08, True)
+    c.table[0, 37] = -1  # (a page of that row alone) for the reference: not seen
+    out, wlse, tol, tol_lse = tree_f64(q, c, parents, n_tok, 0.08, True)
+    minus = q[..., 9] < 0
+    assert np.all(np.abs(got - out)[minus] <= tol[minus]) and np.all(np.abs(lse - wlse)[minus] <= tol_lse[minus])
+    assert np.isnan(got[~minus]).all() and np.isnan(lse[~minus]).all()
