@@ -17,10 +17,10 @@
 // segment that several workgroups shared leaves parts that fa_tree_join adds up.
 //
 // Bound by: HBM while few pairs share a row (decode of 32 x up to 8000 f16 rows, 16/8 heads of
-// 128, two input sets in turn: 59 us, 4.7 TB/s of the 4.9 of a large copy); vector issue (conversion, softmax) between;
-// matrix and vector issue together at 256 pairs (64 tokens, 4 x 32000 f16 rows, 32/8 heads: 187 us,
-// 3.1 TB/s and 0.74 PFLOP/s of the 1.22 of a large f16 matrix product). A second LDS image, so that
-// one barrier per tile is enough, gave nothing there (188 us; f32 Q 102 against 92), nor did
+// 128, 281 MB, two input sets in turn: 61 us, 4.6 TB/s of the 4.9 of a large copy); vector issue (conversion, softmax) between;
+// matrix and vector issue together at 256 pairs (64 tokens, 4 x 32768 f16 rows, 32/8 heads, 541 MB and 138 GFLOP: 184 us,
+// 2.9 TB/s and 0.75 PFLOP/s of the 1.22 of a large f16 matrix product). A second LDS image, so that
+// one barrier per tile is enough, gave nothing there (188 us for 188; f32 Q 102 for 92), nor did
 // wave priorities that hold the waves of a SIMD apart (188). Small calls cost 14 us: two launches
 // and the five dependent reads (arguments, rows, table with Q, K with V, parts) of a lone tile.
 //
@@ -107,9 +107,15 @@ struct TreeCfg {
     static constexpr int MS = D + 4;                                        // merge row stride, floats
     static constexpr int MERGE = WR > 1 ? NW * 16 * MS * 4 : 0;
     static constexpr int SMEM = IMG > MERGE ? IMG : MERGE;
-    // Waves per SIMD: two (256 registers each); three where the form fits 168 registers without
-    // spills (32 fp8 chats of up to 8000 rows: 32.4 us against 34.2; 32 f16 chats, whose form
-    // spills there, 70.1 against 59.4)
+    // Waves per SIMD: two (256 registers each); three for the E5M2 and Q4_0 forms that fit 168 registers
+    // (32 fp8 chats of up to 8000 rows: 32.2 us, with two 32.5; 32 q4_0 chats 34.8, 37.9; 4 x 32000 q4_0
+    // rows 52, 62). 32 f16 chats, whose form spills there, take 70.1 with three, 59.4 with two. Q8_0's form
+    // fits too (163 registers) and is left at two: three take 47.1 for 49.3 (32 chats), 73.5 for 84.3
+    // (4 x 32000 rows).
+    // Spills: 29 of the 72 forms keep 3 to 74 registers in scratch, some of them read in the tile loop:
+    // of f32 Q, all at head dim 256 but the two of one wave per SIMD (139 KB of LDS), and those of 128
+    // and 256 pairs at 128; of bf16 Q, f16 rows at 256, E5M2 and Q8_0 rows of 64 pairs at 256, f16 rows of
+    // 128 pairs at 128.
     static constexpr int WAVES = NARROW && D == 128 && WR == 4 && (KT == XQ_TYPE_E5M2 || KT == XQ_TYPE_Q4_0) ? 3 : 2;
     // workgroups that a CU holds
     static constexpr int BY_LDS = 160 * 1024 / (SMEM + 2048), BY_WAVES = WAVES * 4 / NW;
@@ -191,9 +197,12 @@ XQ_DEV uint2 column4(const uint8_t* p) {
 }
 
 // Wait states between a group of matrix products and the first vector instruction that reads
-// them. The compiler inserts these itself, but leaves them out where that reader is the first
-// instruction of a block (seen as scores of one register in four from before the product);
-// nothing moves across this.
+// them (eight on gfx950); nothing moves across this. The compiler inserts such waits itself, but AMD
+// clang 22 (ROCm 7.2) once did so an instruction late: with the accumulators in AGPRs, the last
+// score product ended a block and a branch round the masking led to
+//     v_accvgpr_read_b32 v2, a27 / s_nop 5 / v_accvgpr_read_b32 v3, a26 ...
+// where a27 was the product's, so that one register in four held the score from before it. In the
+// present forms the compiler's own waits reach eight without this.
 XQ_DEV void products_done() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 7\n\ts_nop 1");

@@ -194,8 +194,9 @@ XQ_DEV void free_pages(const int32_t* refs, uint32_t n_pages, uint32_t want, int
 
 // One workgroup. Wave w counts the missing pages of sequences w, w + 16, ...; a scan over the
 // sequences gives each its place in the list of free pages; then the waves fill the tables.
-// One workgroup, since who gets which page depends on all before: bound by its dependent
-// reads, not by their bytes.
+// One workgroup, since who gets which page depends on all before. It reads every page's references on
+// every call, each thread a span of its own, whether a page is wanted or not, and that bounds it: 64
+// sequences, 1024 pages 8 us, 8192 13, 65536 62, 262144 215 (64 pages wanted: 9, 18, 73, 227).
 // list: [n_pages] free pages, then counts: [n_seq].
 __global__ __launch_bounds__(kScanThreads) void pages_reserve_kernel(int32_t* table, int32_t* refs, uint32_t n_seq, uint32_t cols,
                                                                      uint32_t n_pages, uint32_t page_rows, const int32_t* __restrict__ want,
