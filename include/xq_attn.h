@@ -451,6 +451,56 @@ xq_status xq_fa_tree_workspace(const xq_tensor* q, const xq_kv_pages* cache, con
 xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t* parents, const int32_t* n_tok,
                      xq_tensor* dst, float* lse, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* How a chunk of new tokens meets the paged cache: the scores are scale q.k, then (logit_softcap
+ * above 0) logit_softcap * tanh(./logit_softcap), then (max_bias above 0) slope_h * (row - the token's
+ * row), with ggml's ALiBi slopes. window above 0: a token sees its own row and the window - 1 before
+ * it, 0: all before it. scale finite, the others finite and not negative, reserved 0. */
+typedef struct xq_chunk_params {
+    float scale;
+    float max_bias;
+    float logit_softcap;
+    int32_t window;
+    int32_t reserved[4];
+} xq_chunk_params;
+
+/* Attention of a chunk of new tokens (a prompt, a part of one, one token) over the paged cache:
+ * token t of sequence b stands at row at = rows[b] + t and sees the rows [lo, hi) of its sequence,
+ *   lo = max(0, at + 1 - window, first[b][t]),  hi = max(at + 1, min(prefix[b], rows[b] + n_tok[b])).
+ *   q       F32|BF16 [D, n_q, n_head, n_seq], any n_q >= 1, D 128 or 256; elements contiguous, other
+ *           strides free
+ *   cache   as xq_fa_tree takes it; the tokens' own rows are in it (xq_qk_norm_rope)
+ *   first   I32 [n_seq][n_q] (device), or NULL: the first row that a token may see (of its document)
+ *   prefix  I32 [n_seq] (device), or NULL: rows below it are seen by all tokens, earlier ones too
+ *   n_tok   I32 [n_seq] (device), or NULL: all n_q. Rows of dst and lse from n_tok[b] on
+ *           are left as they were
+ *   dst     q's type [D, n_head, n_q, n_seq], strides multiples of 16 bytes; not q's memory
+ *   lse     F32 [n_seq][n_q][n_head], natural logarithm of the softmax sum, or NULL
+ * A token that sees no row gets O = 0, LSE = -inf. Fewer than 2^25 query rows (n_q * n_head * n_seq) and
+ * 2^22 workgroups (of at least 64 of a KV head's n_q * group rows); row and page strides of the pools below 2^32 bytes. Roundings and non-finite values are
+ * xq_fa_tree's. The workspace may be of 0 bytes; calls that may run at the same time need one each. */
+int xq_supports_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst);
+xq_status xq_fa_chunk_workspace(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, size_t* bytes);
+xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chunk_params* params, const int32_t* first,
+                      const int32_t* prefix, const int32_t* n_tok, xq_tensor* dst, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Accumulated attention weights: what the cached rows have got of the tokens' attention so far.
+ *   scores_out[b][r] = c scores[b][r] + sum over the chunk's tokens t that see r, and the heads h,
+ *                      of e^(score of (t, h, r) - lse[b][t][h]),
+ * for the rows r below rows[b] + n_tok[b] and score_cols; rows from there on are left as they were. c
+ * is `decay`; with `fresh` 1 it is 0 for the tokens' own rows (of the first layer of a step; the other
+ * layers' calls add to them: decay 1, fresh 0).
+ *   q, cache, params, first, prefix, n_tok  as for xq_fa_chunk (V is not read). A view of a chunk's last
+ *           tokens, with rows moved up by those left out, gives the weights of these alone
+ *   lse     F32 [n_seq][n_q][n_head] (device), of xq_fa_chunk or xq_fa_tree; -inf: a token without weight
+ *   scores  F32 [n_seq][score_cols] (device), or NULL: zeros; scores_out the same, and may be scores
+ * Scores are those of the decoded cache at 22 bits and more whatever q's type, sums in f32, in an order
+ * that depends on the shapes alone. decay finite. */
+xq_status xq_kv_weights_workspace(const xq_tensor* q, const xq_kv_pages* cache, size_t* bytes);
+xq_status xq_kv_weights(const xq_tensor* q, const xq_kv_pages* cache, const xq_chunk_params* params, const int32_t* first,
+                        const int32_t* prefix, const int32_t* n_tok, const float* lse, const float* scores, float* scores_out,
+                        int32_t score_cols, float decay, int32_t fresh, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The pages themselves. `pools` are the pools (K and V of every layer, host array, at most
  * 1024, head dim a multiple of 32, pages below 2^31 bytes) that one table addresses; all have
  * the same page_rows and n_pages. All other
@@ -497,6 +547,55 @@ xq_status xq_kv_pages_fork(const xq_tensor* pools, int32_t n_pools, int32_t* tab
  * 65535. */
 xq_status xq_kv_pages_release(int32_t* table, int32_t* rows, int32_t* refs, int32_t n_seq, int32_t table_cols,
                               int32_t n_pages, const int32_t* seqs, int32_t n, void* stream);
+
+/* evict: rows of least accumulated weight (xq_kv_weights) leave the cache. Of a sequence with n =
+ * rows[b] rows above keep[b] (below 0 counts as 0) that many stay: first those that are protected, then those of larger
+ * scores[b][r] (NaN the least), then those of lower index. Protected are rows whose position is below
+ * first_rows, or above the newest position held less last_rows; positions[b][r] is row r's, NULL: r.
+ * Rows that stay and lie at index keep[b] or behind move, in order, into the places below it that others
+ * leave, in order: in every pool, in scores_out and positions_out (as wide as scores; the same arrays, others,
+ * or NULL; written for the rows that are held after the call). rows_out[b] is the number of rows held then. A cache of which rows have been moved
+ * needs positions from then on (its rows' order says nothing about their age, and xq_fa_chunk's window,
+ * first and max_bias go by rows).
+ * refs NULL: no page of a sequence is another's too, and none is given back. refs given: pages without rows
+ * are given back (the table's entry -1, refs less 1), and a sequence of which a page to be written has refs
+ * above 1 is left as it was. So is one
+ * with a row to be moved from or to a page that is none, or with rows below 0, above score_cols or
+ * past the table's columns. At most 65535 sequences, score_cols up to 2^30; rows_out is not rows, no pool is given twice. */
+xq_status xq_kv_pages_evict_workspace(int32_t n_seq, int32_t score_cols, size_t* bytes);
+xq_status xq_kv_pages_evict(const xq_tensor* pools, int32_t n_pools, int32_t* table, const int32_t* rows, int32_t* refs,
+                            int32_t n_seq, int32_t table_cols, const int32_t* keep, int32_t first_rows, int32_t last_rows,
+                            const float* scores, const int32_t* positions, int32_t score_cols, float* scores_out,
+                            int32_t* positions_out, int32_t* rows_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Drafted tokens against the target's logits, from given random numbers: which of them stand, and the
+ * token after them. Token 0 of a sequence is decided (the last one it has); token i's row of logits is
+ * the target's answer after it. From token 0 on, the children of the token reached are tried in order
+ * of index; p = softmax(logits / temperature) after that token:
+ *   draft NULL   a child with token x stands if uniform[b][c] * R < p(x), R = 1 less the p of its rejected
+ *                siblings' tokens; a token tried twice has no mass left;
+ *   draft given  (a chain: parents NULL) it stands if uniform[b][c] * q(x) < p(x), q the draft's distribution
+ *                after the same token (the probabilities that x was drawn from).
+ * The next token is the lowest v whose running sum of what is left (p without the rejected tokens; max(p - q, 0)
+ * where a child was rejected) exceeds uniform[b][n_q] times its whole; p's where nothing is left. A
+ * temperature of 0 or less: the child that is the largest logit (the lowest index of equal ones) stands,
+ * and that one is next.
+ *   logits  F32|BF16 [V, n_q, n_seq], n_q <= 64, V <= 2^24, elements contiguous, other strides free; NaN counts as -inf, and
+ *           of +inf each has the same mass
+ *   draft   logits' type and shape (probabilities), or NULL
+ *   tokens  I32 [n_seq][n_q] (device); one outside [0, V) never stands
+ *   parents, n_tok  as for xq_fa_tree; a token that does not descend from token 0 is never reached
+ *   temperature  F32 [n_seq] (device), or NULL: 1
+ *   uniform F32 [n_seq][n_q + 1] (device) in [0, 1), or NULL: all greedy
+ *   path    I32 [n_seq][n_q]: the tokens that stand, token 0 first, then -1; n_path their number (what
+ *           xq_kv_pages_compact takes); next I32 [n_seq]: -1 where n_tok is 0 or the row holds nothing but -inf
+ *   logp    F32 [n_seq][n_q + 1], or NULL: ln p of each token with a parent after that parent, and of the next
+ *           one; 0 where there is none; greedy ones at temperature 1
+ * Sums of the next token's row are formed in f64. */
+xq_status xq_verify_tokens_workspace(const xq_tensor* logits, size_t* bytes);
+xq_status xq_verify_tokens(const xq_tensor* logits, const xq_tensor* draft, const int32_t* tokens, const int32_t* parents,
+                           const int32_t* n_tok, const float* temperature, const float* uniform, int32_t* path, int32_t* n_path,
+                           int32_t* next, float* logp, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Misc

@@ -1,0 +1,318 @@
+// xq_evict.hip — rows of least accumulated weight leave the paged cache.
+//
+// Per sequence with n rows and a budget k below n: the rows are ordered by (protected first, larger
+// weight, lower index) and the first k stay. Those of them that lie at index k or behind move, in
+// order, to the places below k that others leave, in order: no row is both read and written, so all
+// move at once, and no more bytes than have to. One workgroup per sequence selects (the weights are
+// read from L2 a few times: a radix search for the k-th key, then ranks by ballots), and writes a list
+// of (page, row) pairs; a second launch moves them in every pool and gives pages without rows back.
+#include "xq_pools.h"
+
+namespace xq {
+
+struct EvictArgs {
+    int32_t* table;
+    const int32_t* rows;
+    int32_t* refs;  // null: no page is shared, none is given back
+    const int32_t* keep;
+    int32_t cols, n_pages, page_rows, row_limit;
+    int64_t first_rows, last_rows;  // protected: by position
+    const float* scores;
+    const int32_t* positions;  // null: the rows' indexes
+    int32_t score_cols;
+    float* scores_out;      // null: not wanted
+    int32_t* positions_out;
+    int32_t* rows_out;
+    int32_t* count;  // [sequence] moves
+    int32_t* stay;   // [sequence] rows that stay, or -1 where nothing was done
+    int32_t* lists;  // [sequence][2][half] places to fill, rows that fill them
+    int4* moves;     // [sequence][half] page and row from, page and row to
+    int32_t half;
+    UDivFlat d_page;
+};
+
+// Larger weights have larger keys; NaN the least, -0 is 0.
+XQ_DEV uint32_t weight_key(float x) {
+    const uint32_t u = x == 0.0f ? 0u : __float_as_uint(x);
+    return x != x ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+
+// Exclusive sums over the 16 waves of each wave's number; the whole in *total.
+XQ_DEV uint32_t before_wave(uint32_t mine, uint32_t* lds, uint32_t* total) {
+    __syncthreads();
+    if (lane_id() == 0) lds[wave_id()] = mine;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kEvictWaves; ++i) {
+        before += i < wave_id() ? lds[i] : 0u;
+        all += lds[i];
+    }
+    *total = all;
+    return before;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
+    __shared__ uint32_t hist[256], lds[kEvictWaves], found[2];
+    const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wave = wave_id();
+    const int n = a.rows[b], k = max(a.keep[b], 0);
+    const float* const score = a.scores + (int64_t)b * a.score_cols;
+    const int32_t* const position = a.positions ? a.positions + (int64_t)b * a.score_cols : nullptr;
+    const bool held = n >= 0 && n <= a.score_cols && n <= a.row_limit;
+    const bool cut = held && n > k;
+    auto pos = [&](int r) { return position ? position[r] : r; };
+    // the newest position
+    int newest = -0x7fffffff - 1;
+    if (cut) {
+        for (int r = tid; r < n; r += kEvictThreads) newest = max(newest, pos(r));
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2) newest = max(newest, __shfl_xor(newest, s));
+        if (lane == 0) lds[wave] = (uint32_t)newest;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, (int)lds[i]);
+        __syncthreads();
+    }
+    auto safe = [&](int r) {
+        const int64_t p = pos(r);
+        return p < a.first_rows || (int64_t)newest - p < a.last_rows;
+    };
+    // rows [w0, w1) are this wave's, 64 at a time
+    const int span = ((n + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
+    const int w0 = min(n, wave * span), w1 = min(n, w0 + span);
+    uint32_t moves = 0;
+    bool done = cut;
+    if (cut) {
+        uint32_t mine = 0, n_safe;
+        for (int r0 = w0; r0 < w1; r0 += 64) mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r0 + lane < w1 && safe(r0 + lane)));
+        before_wave(mine, lds, &n_safe);
+        // the group that is cut: protected rows where those alone exceed the budget, else the others,
+        // of which `want` stay: all keys above `key`, and the first `ties` that equal it
+        const bool among_safe = n_safe > (uint32_t)k;
+        const uint32_t want = among_safe ? (uint32_t)k : (uint32_t)k - n_safe;
+        uint32_t key = 0, left = want;
+        if (want) {
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                __syncthreads();
+                if (tid < 256) hist[tid] = 0;
+                __syncthreads();
+                for (int r = tid; r < n; r += kEvictThreads) {
+                    const uint32_t x = weight_key(score[r]);
+                    if (safe(r) == among_safe && (shift == 24 || (x ^ key) >> (shift + 8) == 0)) atomicAdd(&hist[(x >> shift) & 255u], 1u);
+                }
+                __syncthreads();
+                if (wave == 0) {
+                    // lane l: bins 4l .. 4l + 3; how many lie in the bins above
+                    const uint32_t h0 = hist[4 * lane], h1 = hist[4 * lane + 1], h2 = hist[4 * lane + 2], h3 = hist[4 * lane + 3];
+                    uint32_t up = h0 + h1 + h2 + h3;
+#pragma unroll
+                    for (int s = 1; s < 64; s *= 2) {
+                        const uint32_t y = __shfl_down(up, s);
+                        if (lane + s < 64) up += y;
+                    }
+                    uint32_t above = up - (h0 + h1 + h2 + h3);
+                    const uint32_t h[4] = {h0, h1, h2, h3};
+#pragma unroll
+                    for (int i = 3; i >= 0; --i) {
+                        if (above < left && above + h[i] >= left) {
+                            found[0] = (uint32_t)(4 * lane + i);
+                            found[1] = left - above;
+                        }
+                        above += h[i];
+                    }
+                }
+                __syncthreads();
+                key |= found[0] << shift;
+                left = found[1];
+            }
+        }
+        const uint32_t ties = want ? left : 0u;
+        // ranks of the ties, in the rows' order
+        mine = 0;
+        for (int r0 = w0; r0 < w1; r0 += 64)
+            mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r0 + lane < w1 && safe(r0 + lane) == among_safe && weight_key(score[r0 + lane]) == key));
+        uint32_t total, tie0 = before_wave(mine, lds, &total);
+        // f(row, stays) for this wave's rows; all 64 lanes take part
+        auto rows = [&](auto f) {
+            uint32_t tie = tie0;
+            for (int r0 = w0; r0 < w1; r0 += 64) {
+                const int r = r0 + lane;
+                const bool on = r < w1, s = on && safe(r), group = on && s == among_safe;
+                const uint32_t x = on ? weight_key(score[r]) : 0u;
+                const uint64_t eq = __builtin_amdgcn_ballot_w64(group && x == key);
+                const uint32_t rank = tie + __builtin_popcountll(eq & (((uint64_t)1 << lane) - 1));
+                f(r, on, on && (group ? want && (x > key || (x == key && rank < ties)) : !among_safe && s));
+                tie += __builtin_popcountll(eq);
+            }
+        };
+        uint32_t holes = 0, tails = 0;
+        rows([&](int r, bool on, bool stays) {
+            holes += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && !stays && r < k));
+            tails += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && stays && r >= k));
+        });
+        uint32_t hole0 = before_wave(holes, lds, &moves), tail0 = before_wave(tails, lds, &total);
+        int32_t* const hole = a.lists + (int64_t)b * 2 * a.half;
+        int32_t* const tail = hole + a.half;
+        rows([&](int r, bool on, bool stays) {
+            const uint64_t below = ((uint64_t)1 << lane) - 1;
+            const uint64_t x = __builtin_amdgcn_ballot_w64(on && !stays && r < k), y = __builtin_amdgcn_ballot_w64(on && stays && r >= k);
+            if (x >> lane & 1) hole[hole0 + __builtin_popcountll(x & below)] = r;
+            if (y >> lane & 1) tail[tail0 + __builtin_popcountll(y & below)] = r;
+            hole0 += __builtin_popcountll(x);
+            tail0 += __builtin_popcountll(y);
+        });
+        __syncthreads();
+        // their places; a page that other sequences hold too is not written
+        bool ok = true;
+        for (uint32_t i = tid; i < moves; i += kEvictThreads) {
+            const uint32_t from = (uint32_t)tail[i], to = (uint32_t)hole[i];
+            const uint32_t fc = a.d_page.quot(from), tc = a.d_page.quot(to);
+            const uint32_t fp = (uint32_t)a.table[(int64_t)b * a.cols + fc], tp = (uint32_t)a.table[(int64_t)b * a.cols + tc];
+            ok = ok && fp < (uint32_t)a.n_pages && tp < (uint32_t)a.n_pages && (!a.refs || a.refs[tp] <= 1);
+            a.moves[(int64_t)b * a.half + i] = make_int4((int)fp, (int)(from - fc * a.d_page.d), (int)tp, (int)(to - tc * a.d_page.d));
+        }
+        done = __syncthreads_and(ok);
+    }
+    // weights and positions of the rows that are held now
+    const int32_t* const hole = a.lists + (int64_t)b * 2 * a.half;
+    const int rest = held ? (done ? k : n) : 0;
+    if (a.scores_out && a.scores_out != a.scores)
+        for (int r = tid; r < rest; r += kEvictThreads) a.scores_out[(int64_t)b * a.score_cols + r] = score[r];
+    if (a.positions_out && a.positions_out != a.positions)
+        for (int r = tid; r < rest; r += kEvictThreads) a.positions_out[(int64_t)b * a.score_cols + r] = pos(r);
+    __syncthreads();
+    if (done)
+        for (uint32_t i = tid; i < moves; i += kEvictThreads) {
+            const int64_t to = (int64_t)b * a.score_cols + hole[i];
+            const int from = hole[a.half + i];
+            if (a.scores_out) a.scores_out[to] = score[from];
+            if (a.positions_out) a.positions_out[to] = pos(from);
+        }
+    if (tid == 0) {
+        a.rows_out[b] = done ? k : n;
+        a.count[b] = done ? (int32_t)moves : 0;
+        a.stay[b] = done ? k : -1;
+    }
+}
+
+// A workgroup moves kMoveRows rows of a sequence in one pool at a time: a thread takes every 256th
+// 16-byte piece of them, four loads before the first store.
+constexpr int kMoveRows = 16;
+
+__global__ __launch_bounds__(256) void evict_move_kernel(PoolSet set, EvictArgs a, int32_t chunks, int32_t gives) {
+    __shared__ int64_t from[kMoveRows], to[kMoveRows];
+    const uint32_t chunk = blockIdx.x, pool = blockIdx.y, b = blockIdx.z;
+    const int n = a.count[b], k = a.stay[b];
+    if (gives && a.refs && chunk == 0 && pool == 0 && k >= 0) {
+        // pages behind the last row: the exchange hands each entry to one thread
+        const uint32_t c0 = k ? a.d_page.quot((uint32_t)k - 1u) + 1u : 0u;
+        for (uint32_t c = c0 + threadIdx.x; c < (uint32_t)a.cols; c += 256) {
+            const uint32_t p = (uint32_t)atomicExch(&a.table[(int64_t)b * a.cols + c], -1);
+            if (p < (uint32_t)a.n_pages) atomicSub(&a.refs[p], 1);
+        }
+    }
+    const Pool p = set.p[pool];
+    const uint32_t per_line = (p.line + 15u) / 16u, units = per_line * p.heads;
+    for (int i0 = (int)chunk * kMoveRows; i0 < n; i0 += chunks * kMoveRows) {
+        const int m = min(kMoveRows, n - i0);
+        __syncthreads();
+        if ((int)threadIdx.x < m) {
+            const int4 e = a.moves[(int64_t)b * a.half + i0 + threadIdx.x];
+            from[threadIdx.x] = (int64_t)e.x * p.page + (int64_t)e.y * p.row;
+            to[threadIdx.x] = (int64_t)e.z * p.page + (int64_t)e.w * p.row;
+        }
+        __syncthreads();
+        const uint32_t total = units * (uint32_t)m;
+        for (uint32_t u0 = threadIdx.x; u0 < total; u0 += 1024) {
+            u32x4p v[4];
+            uint8_t* y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t u = u0 + 256u * j;
+                if (u < total) {
+                    const uint32_t r = u / units, x = u - r * units, h = x / per_line;
+                    const int64_t off = (int64_t)h * p.head + piece_at(x - h * per_line, p.line);
+                    v[j] = *(const u32x4p*)(p.base + from[r] + off);
+                    y[j] = p.base + to[r] + off;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (u0 + 256u * j < total) *(u32x4p*)y[j] = v[j];
+        }
+    }
+}
+
+static size_t evict_space(int32_t n_seq, int32_t score_cols, size_t* moves_at, size_t* lists_at) {
+    const size_t half = (size_t)score_cols / 2 + 1;
+    *moves_at = ((size_t)n_seq * 8 + 15) / 16 * 16;
+    *lists_at = *moves_at + (size_t)n_seq * half * 16;
+    return *lists_at + (size_t)n_seq * half * 8;
+}
+
+}  // namespace xq
+
+using namespace xq;
+
+extern "C" {
+
+xq_status xq_kv_pages_evict_workspace(int32_t n_seq, int32_t score_cols, size_t* bytes) {
+    if (!bytes || n_seq < 1 || score_cols < 1) return failf(XQ_ERR_BAD_ARG, "bad evict arguments");
+    size_t m, l;
+    *bytes = evict_space(n_seq, score_cols, &m, &l);
+    return done_ok();
+}
+
+xq_status xq_kv_pages_evict(const xq_tensor* pools, int32_t n_pools, int32_t* table, const int32_t* rows, int32_t* refs,
+                            int32_t n_seq, int32_t table_cols, const int32_t* keep, int32_t first_rows, int32_t last_rows,
+                            const float* scores, const int32_t* positions, int32_t score_cols, float* scores_out,
+                            int32_t* positions_out, int32_t* rows_out, void* workspace, size_t workspace_bytes, void* stream) {
+    int32_t page_rows, n_pages;
+    xq_status st = pools_check(pools, n_pools, &page_rows, &n_pages);
+    if (st == XQ_OK) st = table_check(n_seq, table_cols);
+    if (st == XQ_OK) st = pools_differ(pools, n_pools);
+    if (st != XQ_OK) return st;
+    if (n_seq > 65535) return failf(XQ_ERR_UNSUPPORTED, "more than 65535 sequences");
+    if (score_cols < 1) return failf(XQ_ERR_BAD_ARG, "score_cols must be at least 1");
+    if (score_cols > (1 << 30)) return failf(XQ_ERR_UNSUPPORTED, "score_cols above 2^30");
+    if (first_rows < 0 || last_rows < 0) return failf(XQ_ERR_BAD_ARG, "first_rows and last_rows must not be negative");
+    if (!table || !rows || !keep || !scores || !rows_out) return failf(XQ_ERR_BAD_ARG, "null pointer");
+    if (rows_out == rows) return failf(XQ_ERR_BAD_ARG, "rows_out must not be rows");
+    for (const void* x : {(const void*)table, (const void*)rows, (const void*)refs, (const void*)keep, (const void*)scores, (const void*)positions,
+                          (const void*)scores_out, (const void*)positions_out, (const void*)rows_out})
+        if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
+    EvictArgs a{};
+    size_t moves_at, lists_at;
+    const size_t need = evict_space(n_seq, score_cols, &moves_at, &lists_at);
+    if (!workspace || workspace_bytes < need) return failf(XQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    if (!aligned(workspace, 256)) return failf(XQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    const int64_t lim = (int64_t)table_cols * page_rows;
+    a.table = table, a.rows = rows, a.refs = refs, a.keep = keep;
+    a.cols = table_cols, a.n_pages = n_pages, a.page_rows = page_rows, a.row_limit = (int32_t)(lim < 0x7fffff00 ? lim : 0x7fffff00);
+    a.first_rows = first_rows, a.last_rows = last_rows;
+    a.scores = scores, a.positions = positions, a.score_cols = score_cols;
+    a.scores_out = scores_out, a.positions_out = positions_out, a.rows_out = rows_out;
+    a.count = (int32_t*)workspace, a.stay = a.count + n_seq;
+    a.moves = (int4*)((uint8_t*)workspace + moves_at);
+    a.lists = (int32_t*)((uint8_t*)workspace + lists_at);
+    a.half = score_cols / 2 + 1;
+    a.d_page = UDivFlat((uint32_t)page_rows);
+    hipStream_t s = (hipStream_t)stream;
+    launch("kv_pages_evict", evict_select_kernel, dim3((uint32_t)n_seq), dim3(kEvictThreads), s, a);
+    for (int32_t i0 = 0; i0 < n_pools; i0 += kPoolsPerLaunch) {
+        const int32_t m = n_pools - i0 < kPoolsPerLaunch ? n_pools - i0 : kPoolsPerLaunch;
+        PoolSet set{};
+        for (int32_t i = 0; i < m; ++i) set.p[i] = pool_of(pools[i0 + i]);
+        // workgroups for half of the rows, up to 4096 in all
+        int64_t chunks = 4096 / ((int64_t)m * n_seq), most = cdiv(a.half, kMoveRows);
+        chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
+        launch("kv_pages_move", evict_move_kernel, dim3((uint32_t)chunks, (uint32_t)m, (uint32_t)n_seq), dim3(256), s, set, a, (int32_t)chunks, i0 == 0 ? 1 : 0);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return failf(XQ_ERR_HIP, "kv_pages_evict launch: %s", hipGetErrorString(e));
+    return done_ok();
+}
+
+}  // extern "C"

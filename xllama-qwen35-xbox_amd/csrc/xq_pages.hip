@@ -5,29 +5,11 @@
 // tables change. Pool records may lie anywhere (free row, head and page strides), so a
 // page is `runs` of contiguous bytes: one where the page is one block, one per row or head,
 // or one per record.
-#include "xq_paged.h"
+#include "xq_pools.h"
 
 namespace xq {
 
-constexpr int kPoolsPerLaunch = 40;  // 40 bytes each: kernel arguments stay below 2 KiB
 constexpr int kMaxForks = 1024;
-
-typedef uint32_t u32x4p __attribute__((ext_vector_type(4), aligned(1)));
-typedef uint16_t u16p __attribute__((aligned(1)));
-
-struct Pool {
-    uint8_t* base;
-    int64_t page, row, head;  // strides, bytes
-    uint32_t line;            // contiguous bytes: a record, or a row's n_head_kv records (heads 1)
-    uint32_t heads;           // lines per row
-};
-
-struct PoolSet {
-    Pool p[kPoolsPerLaunch];
-};
-
-// 16 bytes of the run at byte off (the last piece of a run is moved up to end with it).
-XQ_DEV uint32_t piece_at(uint32_t i, uint32_t run) { return min(i * 16u, run - 16u); }
 
 // ---------------------------------------------------------------- copy
 
@@ -331,40 +313,6 @@ __global__ __launch_bounds__(256) void pages_release_kernel(int32_t* table, int3
 
 // ---------------------------------------------------------------- host
 
-static xq_status pools_check(const xq_tensor* pools, int32_t n_pools, int32_t* page_rows, int32_t* n_pages) {
-    if (!pools) return failf(XQ_ERR_BAD_ARG, "null pools");
-    if (n_pools < 1 || n_pools > 1024) return failf(XQ_ERR_BAD_ARG, "n_pools must be in [1, 1024]");
-    for (int32_t i = 0; i < n_pools; ++i) {
-        const xq_tensor& t = pools[i];
-        const size_t ts = type_size(t.type);
-        if (!ts) return failf(XQ_ERR_UNSUPPORTED, "pool %d: type %d", i, t.type);
-        for (int j = 0; j < 4; ++j)
-            if (t.ne[j] < 1 || t.ne[j] > 0x7fffffff) return failf(XQ_ERR_BAD_SHAPE, "pool %d: bad ne", i);
-        if (t.ne[0] % 32 || t.ne[0] > 65536) return failf(XQ_ERR_UNSUPPORTED, "pool %d: head dim must be a multiple of 32", i);
-        if (t.nb[0] != ts) return failf(XQ_ERR_UNSUPPORTED, "pool %d: records must be contiguous", i);
-        if (t.ne[1] != pools[0].ne[1] || t.ne[3] != pools[0].ne[3])
-            return failf(XQ_ERR_BAD_SHAPE, "pool %d: page_rows and n_pages must be those of pool 0", i);
-        if ((int64_t)record_bytes(t.type, t.ne[0]) * t.ne[2] > ((int64_t)1 << 24)) return failf(XQ_ERR_UNSUPPORTED, "pool %d: row above 2^24 bytes", i);
-        if ((int64_t)record_bytes(t.type, t.ne[0]) * t.ne[2] * t.ne[1] >= ((int64_t)1 << 31))
-            return failf(XQ_ERR_UNSUPPORTED, "pool %d: page of 2^31 bytes or more", i);
-        if (!t.data) return failf(XQ_ERR_BAD_ARG, "pool %d: null data pointer", i);
-    }
-    *page_rows = (int32_t)pools[0].ne[1];
-    *n_pages = (int32_t)pools[0].ne[3];
-    return XQ_OK;
-}
-
-static Pool pool_of(const xq_tensor& t) {
-    Pool p{};
-    const size_t rec = record_bytes(t.type, t.ne[0]);
-    p.base = (uint8_t*)t.data;
-    p.row = (int64_t)t.nb[1], p.head = (int64_t)t.nb[2], p.page = (int64_t)t.nb[3];
-    const bool one = t.ne[2] == 1 || t.nb[2] == rec;  // a row's records lie one after another
-    p.line = (uint32_t)(one ? rec * t.ne[2] : rec);
-    p.heads = one ? 1u : (uint32_t)t.ne[2];
-    return p;
-}
-
 // pieces of a page: a bound over the run forms (a run's last piece counts whole)
 static int64_t page_pieces(const xq_tensor& t) {
     const Pool p = pool_of(t);
@@ -393,11 +341,6 @@ static xq_status copy_launch(const xq_tensor* pools, int32_t n_pools, const int3
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return failf(XQ_ERR_HIP, "kv_pages_copy launch: %s", hipGetErrorString(e));
-    return XQ_OK;
-}
-
-static xq_status table_check(int32_t n_seq, int32_t table_cols) {
-    if (n_seq < 1 || table_cols < 1) return failf(XQ_ERR_BAD_ARG, "bad table sizes");
     return XQ_OK;
 }
 
@@ -432,10 +375,8 @@ xq_status xq_kv_pages_compact(const xq_tensor* pools, int32_t n_pools, const int
     if (rows_out == rows) return failf(XQ_ERR_BAD_ARG, "rows_out must not be rows");
     for (const void* x : {(const void*)table, (const void*)rows, (const void*)path, (const void*)n_path, (const void*)rows_out})
         if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
-    // (its rows would be moved twice, by waves that do not wait for each other)
-    for (int32_t i = 0; i < n_pools; ++i)
-        for (int32_t j = 0; j < i; ++j)
-            if (pools[i].data == pools[j].data) return failf(XQ_ERR_BAD_ARG, "pools %d and %d are one", j, i);
+    st = pools_differ(pools, n_pools);
+    if (st != XQ_OK) return st;
     const int64_t lim = (int64_t)table_cols * page_rows;
     for (int32_t i0 = 0; i0 < n_pools; i0 += kPoolsPerLaunch) {
         const int32_t m = n_pools - i0 < kPoolsPerLaunch ? n_pools - i0 : kPoolsPerLaunch;

@@ -1,0 +1,501 @@
+// xq_verify.hip — drafted tokens against the target's logits, from given random numbers.
+//
+// p_i = softmax(logits_i / temperature) is the target's distribution after token i. From token 0, which
+// is decided, the children of the token reached are tried in order of index: child c with token x is
+// accepted if u_c R < p(x), R = 1 - the p of the children's tokens rejected before (a token tried
+// twice has no mass left), or, along a chain drawn from a draft's distributions q, if u_c q(x) < p(x).
+// The next token is drawn from what is left: p without the rejected tokens, or max(p - q, 0): the lowest v
+// whose running sum exceeds u times the whole.
+//
+// Whether a child would be accepted if its parent were reached does not depend on the walk: all rows'
+// maxima and sums are formed at once (one pass over the logits, bound by HBM), then one wave has
+// the path by ballots and pointer doubling, a lane a token. Only the next token needs sums that hold
+// next to a border: those of one row per sequence, in f64 throughout. A row's sum over the tests is of
+// f32 exponentials (each off by 2^-22 of itself, the sum by less) joined in f64.
+#include "xq_tile.h"
+
+namespace xq {
+
+constexpr int kVerifyMax = 64;    // tokens of a sequence: a lane each
+constexpr int kVChunk = 8192;     // elements of a row that a workgroup takes
+constexpr float kVLog2e = 1.4426950408889634f;
+
+struct RowStat {
+    float max, sum;  // of a chunk; the sum relative to its maximum
+    int32_t arg;
+    int32_t pad;
+};
+struct Walk {
+    int32_t at, n;  // the last token of the path, its length; at -1: nothing left to draw
+    uint64_t kids;  // its children
+    double max, heat, whole;  // of row `at`; whole: the stats' sum
+};
+
+struct VerifyArgs {
+    const uint8_t* logits;
+    int64_t l_nb1, l_nb2;  // token, sequence
+    const uint8_t* draft;
+    int64_t q_nb1, q_nb2;
+    const int32_t *tokens, *parents, *n_tok;
+    const float *temperature, *uniform;
+    int32_t *path, *n_path, *next;
+    float* logp;
+    int32_t V, n_q, B, chunks;
+    RowStat* stats;  // [sequence][token][chunk]
+    Walk* walk;      // [sequence]
+    double* sums;    // [2][sequence][chunk]: of p's weights; of what is left
+
+    XQ_DEV int tokens_of(int b) const { return n_tok ? min(max(n_tok[b], 0), n_q) : n_q; }
+    // the temperature of a sequence; 0: greedy. (Any above 1e30 leaves all finite logits the same mass.)
+    XQ_DEV float heat(int b) const {
+        const float t = !uniform ? 0.0f : temperature ? temperature[b] : 1.0f;
+        return t > 0.0f ? fminf(t, 1e30f) : 0.0f;
+    }
+};
+
+template <bool WIDE>
+XQ_DEV float element(const uint8_t* row, int64_t v) {
+    const float x = WIDE ? *(const float*)(row + 4 * v) : bf16_bits_to_f32(*(const uint16_t*)(row + 2 * v));
+    return x == x ? x : -INFINITY;
+}
+// Elements v .. v + N - 1 (4 of f32, 8 of bf16); -inf from V on and for NaN.
+template <bool WIDE, int N>
+XQ_DEV void elements(const uint8_t* row, int v, int V, float (&x)[N]) {
+    static_assert(N == (WIDE ? 4 : 8));
+    if (v + N <= V) {
+        if constexpr (WIDE) {
+            const f4el y = *(const f4el*)(row + 4 * (int64_t)v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = y[i];
+        } else {
+            const u4half y = *(const u4half*)(row + 2 * (int64_t)v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = __uint_as_float(y[i] << 16);
+                x[2 * i + 1] = __uint_as_float(y[i] & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = v + i < V ? element<WIDE>(row, v + i) : -INFINITY;
+    }
+}
+
+// A weight relative to the maximum; +inf shares the mass where it is the maximum.
+XQ_DEV float weight_f32(float x, float max, float c) { return x == max ? 1.0f : __builtin_amdgcn_exp2f((x - max) * c); }
+XQ_DEV double weight_f64(double x, double max, double heat) { return x == max ? 1.0 : exp((x - max) / heat); }
+
+XQ_DEV float exponent_factor(float heat) { return fminf(kVLog2e / (heat > 0.0f ? heat : 1.0f), 3.40282347e38f); }
+
+// Maximum, first index of it and sum of exponentials of a chunk of a row.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
+    constexpr int N = WIDE ? 4 : 8, S = kVChunk / 256 / N;
+    __shared__ float sMax[4], sSum[4];
+    __shared__ int sArg[4];
+    const int j = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    if (i >= a.tokens_of(b)) return;
+    const uint8_t* row = a.logits + b * a.l_nb2 + i * a.l_nb1;
+    const float c = exponent_factor(a.heat(b));
+    float x[S][N];
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < S; ++s) elements<WIDE, N>(row, j * kVChunk + (s * 256 + tid) * N, a.V, x[s]);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = fmaxf(top, x[s][e]);
+    top = wave_max(top);
+    if (lane_id() == 0) sMax[wave_id()] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
+    float sum = 0.0f;
+    int arg = 0x7fffffff;
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s)
+#pragma unroll
+        for (int e = N - 1; e >= 0; --e) {
+            sum += weight_f32(x[s][e], top, c);
+            arg = x[s][e] == top ? j * kVChunk + (s * 256 + tid) * N + e : arg;
+        }
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) arg = min(arg, __shfl_xor(arg, s));
+    if (lane_id() == 0) {
+        sSum[wave_id()] = sum;
+        sArg[wave_id()] = arg;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        RowStat r;
+        r.max = top;
+        r.sum = top == -INFINITY ? 0.0f : (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
+        r.arg = min(min(sArg[0], sArg[1]), min(sArg[2], sArg[3]));
+        r.pad = 0;
+        a.stats[((int64_t)b * a.n_q + i) * a.chunks + j] = r;
+    }
+}
+
+XQ_DEV uint64_t shfl64(uint64_t x, int l) { return ((uint64_t)(uint32_t)__shfl((int)(x >> 32), l) << 32) | (uint32_t)__shfl((int)(uint32_t)x, l); }
+XQ_DEV double shfl_f64(double x, int l) { return __builtin_bit_cast(double, shfl64(__builtin_bit_cast(uint64_t, x), l)); }
+
+// Sum over the workgroup's 256 threads, the same in all; the order is fixed.
+XQ_DEV double block_sum(double x, double* lds) {
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) x += shfl_f64(x, lane_id() ^ s);
+    __syncthreads();
+    if (lane_id() == 0) lds[wave_id()] = x;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// The path, by one wave; a lane is a token. Every lane gets the same result.
+template <bool WIDE>
+XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
+    const int c = lane_id(), n = a.tokens_of(b);
+    const float heat = a.heat(b), f = exponent_factor(heat);
+    const double T = heat > 0.0f ? (double)heat : 1.0;
+    const bool live = c < n;
+    // row c's maximum, sum and first index of the maximum
+    float top = -INFINITY;
+    double whole = 0.0;
+    int arg = -1;
+    if (live) {
+        const RowStat* r = a.stats + ((int64_t)b * a.n_q + c) * a.chunks;
+        for (int j = 0; j < a.chunks; ++j) top = fmaxf(top, r[j].max);
+        if (top > -INFINITY)
+            for (int j = 0; j < a.chunks; ++j) {
+                const RowStat s = r[j];
+                whole += (double)s.sum * (double)weight_f32(s.max, top, f);
+                if (arg < 0 && s.max == top) arg = s.arg;
+            }
+    }
+    const int tok = live ? a.tokens[(int64_t)b * a.n_q + c] : -1;
+    int up = !live || c == 0 ? -1 : a.parents ? a.parents[(int64_t)b * a.n_q + c] : c - 1;
+    if (up < 0 || up >= c) up = -1;
+    const int from = up < 0 ? c : up;
+    const float p_top = __shfl(top, from);
+    const double p_whole = shfl_f64(whole, from);
+    const int p_arg = __shfl(arg, from);
+    const bool known = up >= 0 && tok >= 0 && tok < a.V && p_top > -INFINITY;
+    double p = 0.0, lp = -INFINITY;
+    if (known) {
+        const double x = element<WIDE>(a.logits + b * a.l_nb2 + up * a.l_nb1, tok);
+        p = weight_f64(x, p_top, T) / p_whole;
+        lp = (x == (double)p_top ? 0.0 : (x - (double)p_top) / T) - log(p_whole);
+    }
+    // earlier children of the same token: whether one has the same token; the mass of the others
+    bool twice = false;
+    double gone = 0.0;
+    uint64_t before = 0;
+    if (a.parents)
+        for (int i = 1; i < n - 1; ++i) {
+            const int iu = __shfl(up, i), it = __shfl(tok, i);
+            const double ip = shfl_f64(twice ? 0.0 : p, i);  // (lane i is through with its own: i' < i)
+            if (c > i && up >= 0 && iu == up) {
+                before |= 1ull << i;
+                gone += ip;
+                twice = twice || it == tok;
+            }
+        }
+    bool ok;
+    if (heat == 0.0f) {
+        ok = known && tok == p_arg;
+    } else {
+        const double u = live ? (double)a.uniform[(int64_t)b * (a.n_q + 1) + c] : 0.0;
+        if (a.draft)
+            ok = known && u * (double)element<WIDE>(a.draft + b * a.q_nb2 + up * a.q_nb1, tok) < p;
+        else
+            ok = known && !twice && u * (1.0 - gone) < p;
+    }
+    if (c == 0) ok = live;
+    const uint64_t oks = __builtin_amdgcn_ballot_w64(ok);
+    const uint64_t chosen = __builtin_amdgcn_ballot_w64(ok && !(before & oks));
+    // on the path: chosen, and so are all tokens above
+    uint64_t above = 1ull << c;
+    int at = up;
+#pragma unroll
+    for (int d = 0; d < 6; ++d) {
+        const int l = at < 0 ? c : at;
+        above |= shfl64(above, l);
+        const int q = __shfl(at, l);
+        at = at < 0 ? -1 : q;
+    }
+    const uint64_t on = __builtin_amdgcn_ballot_w64(live && (above & 1) && !(above & ~chosen));
+    const int len = __builtin_popcountll(on), last = on ? 63 - __builtin_clzll(on) : 0;
+    Walk w;
+    w.n = len;
+    w.at = len ? last : -1;
+    w.kids = __builtin_amdgcn_ballot_w64(live && up >= 0 && up == last) & (len ? ~0ull : 0ull);
+    w.max = (double)__shfl(top, last);
+    w.heat = T;
+    w.whole = shfl_f64(whole, last);
+    const int last_arg = __shfl(arg, last);
+    if (write) {
+        const int64_t r = (int64_t)b * a.n_q;
+        if (c < a.n_q) {
+            const int rank = __builtin_popcountll(on & ((1ull << c) - 1));
+            if (c >= len) a.path[r + c] = -1;
+            if (on >> c & 1) a.path[r + rank] = c;
+            if (a.logp) a.logp[(int64_t)b * (a.n_q + 1) + c] = live && up >= 0 ? (float)lp : 0.0f;
+        }
+        if (c == 0) a.n_path[b] = len;
+    }
+    if (heat == 0.0f || !len || !(w.max > -INFINITY)) {
+        // nothing is drawn
+        const int v = len && heat == 0.0f ? last_arg : -1;
+        if (write && c == 0) {
+            a.next[b] = v;
+            if (a.logp) a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = v >= 0 ? (float)-log(w.whole) : len ? -INFINITY : 0.0f;
+        }
+        w.at = -1;
+    }
+    return w;
+}
+
+// What is left of element v's weight; `sum`: of row at's weights.
+template <bool WIDE>
+XQ_DEV double left_over(const VerifyArgs& a, const Walk& w, double x, const uint8_t* q, int v, double sum, const uint32_t* hit, int v0) {
+    const double p = weight_f64(x, w.max, w.heat);
+    if (q) return fmax(p / sum - (double)element<WIDE>(q, v), 0.0);
+    return hit[(v - v0) >> 5] >> ((v - v0) & 31) & 1u ? 0.0 : p;
+}
+
+// The tokens of `kids` in the chunk from v0 on, as bits.
+XQ_DEV void mark_kids(const VerifyArgs& a, const Walk& w, int b, int v0, uint32_t* hit) {
+    for (int i = threadIdx.x; i < kVChunk / 32; i += blockDim.x) hit[i] = 0;
+    __syncthreads();
+    if (threadIdx.x < 64 && (w.kids >> threadIdx.x & 1)) {
+        const int64_t t = (int64_t)a.tokens[(int64_t)b * a.n_q + threadIdx.x] - v0;
+        if (t >= 0 && t < kVChunk) atomicOr(&hit[t >> 5], 1u << (t & 31));
+    }
+    __syncthreads();
+}
+
+// PART 0: the path, and the sums of a chunk of the row that the next token is drawn from: of its weights
+// and, without a draft, of what is left of them. PART 1: with a draft, the sum of what is left.
+template <bool WIDE, int PART>
+__global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
+    __shared__ Walk shared;
+    __shared__ double lds[4];
+    __shared__ uint32_t hit[kVChunk / 32];
+    const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, v0 = j * kVChunk;
+    if constexpr (PART == 0) {
+        if (wave_id() == 0) {
+            const Walk w = walk_path<WIDE>(a, b, j == 0);
+            if (tid == 0) shared = w;
+            if (tid == 0 && j == 0) a.walk[b] = w;
+        }
+    } else {
+        if (tid == 0) shared = a.walk[b];
+    }
+    __syncthreads();
+    const Walk w = shared;
+    if (w.at < 0) return;
+    const uint8_t* row = a.logits + b * a.l_nb2 + w.at * a.l_nb1;
+    const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
+    if (PART == 1 && !q) return;
+    double sum = 0.0;
+    if constexpr (PART == 1)
+        for (int i = 0; i < a.chunks; ++i) sum += a.sums[(int64_t)b * a.chunks + i];
+    else
+        mark_kids(a, w, b, v0, hit);
+    double all = 0.0, left = 0.0;
+    for (int v = v0 + tid; v < min(a.V, v0 + kVChunk); v += 256) {
+        const double x = element<WIDE>(row, v);
+        if constexpr (PART == 0) {
+            const double p = weight_f64(x, w.max, w.heat);
+            all += p;
+            left += hit[(v - v0) >> 5] >> ((v - v0) & 31) & 1u ? 0.0 : p;
+        } else {
+            left += left_over<WIDE>(a, w, x, q, v, sum, hit, v0);
+        }
+    }
+    all = block_sum(all, lds);
+    left = block_sum(left, lds);
+    if (tid == 0) {
+        if constexpr (PART == 0) a.sums[(int64_t)b * a.chunks + j] = all;
+        if (PART == 1 || !q) a.sums[((int64_t)a.B + b) * a.chunks + j] = left;
+    }
+}
+
+// The next token: its chunk by the chunks' sums, then its place in the chunk.
+template <bool WIDE>
+__global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
+    __shared__ uint32_t hit[kVChunk / 32];
+    __shared__ double scan[1024 / 64];
+    __shared__ int pick, last;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
+    Walk w = a.walk[b];
+    if (w.at < 0) return;
+    const double* const all = a.sums + (int64_t)b * a.chunks;
+    const double* left = all + (int64_t)a.B * a.chunks;
+    double sum = 0.0, whole = 0.0;
+    for (int j = 0; j < a.chunks; ++j) {
+        sum += all[j];
+        whole += left[j];
+    }
+    const uint8_t* row = a.logits + b * a.l_nb2 + w.at * a.l_nb1;
+    const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
+    if (!(whole > 0.0)) {  // nothing is left: the target's distribution
+        left = all;
+        whole = sum;
+        q = nullptr;
+        w.kids = 0;
+    }
+    const float uf = a.uniform[(int64_t)b * (a.n_q + 1) + a.n_q];
+    const double aim = (uf > 0.0f ? (double)uf : 0.0) * whole;
+    int chunk = 0;
+    double base = 0.0, run = 0.0;
+    bool got = false;
+    for (int j = 0; j < a.chunks && !got; ++j) {
+        const double y = left[j];
+        if (y > 0.0) {
+            chunk = j;
+            base = run;
+            got = run + y > aim;
+        }
+        run += y;
+    }
+    const int v0 = chunk * kVChunk;
+    mark_kids(a, w, b, v0, hit);
+    if (tid == 0) {
+        pick = 0x7fffffff;
+        last = -1;
+    }
+    constexpr int E = kVChunk / 1024;
+    double r[E], mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int v = v0 + tid * E + e;
+        r[e] = v < a.V ? left_over<WIDE>(a, w, element<WIDE>(row, v), q, v, sum, hit, v0) : 0.0;
+        mine += r[e];
+    }
+    double upto = mine;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+        const double y = shfl_f64(upto, lane >= s ? lane - s : lane);
+        if (lane >= s) upto += y;
+    }
+    if (lane == 63) scan[wave_id()] = upto;
+    __syncthreads();
+    double at = base;
+#pragma unroll
+    for (int i = 0; i < 1024 / 64; ++i) at += i < wave_id() ? scan[i] : 0.0;
+    at += upto - mine;
+    int found = 0x7fffffff, any = -1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        at += r[e];
+        if (r[e] > 0.0) {
+            any = v0 + tid * E + e;
+            if (at > aim) found = min(found, any);
+        }
+    }
+    if (found != 0x7fffffff) atomicMin(&pick, found);
+    if (any >= 0) atomicMax(&last, any);
+    __syncthreads();
+    if (tid == 0) {
+        const int v = pick != 0x7fffffff ? pick : last;  // (the whole sum rounded up: the last one)
+        a.next[b] = v;
+        if (a.logp) {
+            const double x = v >= 0 ? (double)element<WIDE>(row, v) : -INFINITY;
+            a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((x == w.max ? 0.0 : (x - w.max) / w.heat) - log(sum));
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+static xq_status verify_check(const xq_tensor* logits, const char* what) {
+    if (!logits) return failf(XQ_ERR_BAD_ARG, "null %s", what);
+    if (logits->type != XQ_TYPE_F32 && logits->type != XQ_TYPE_BF16) return failf(XQ_ERR_UNSUPPORTED, "%s must be F32 or BF16", what);
+    for (int i = 0; i < 4; ++i)
+        if (logits->ne[i] < 1 || logits->ne[i] > 0x7fffffff) return failf(XQ_ERR_BAD_SHAPE, "%s: bad ne", what);
+    if (logits->ne[3] != 1) return failf(XQ_ERR_BAD_SHAPE, "%s must be [vocabulary, n_q, n_seq]", what);
+    if (logits->ne[0] > (1 << 24)) return failf(XQ_ERR_UNSUPPORTED, "a vocabulary above 2^24");
+    if (logits->ne[1] > kVerifyMax) return failf(XQ_ERR_UNSUPPORTED, "more than 64 tokens of a sequence");
+    if (logits->ne[2] > 65535) return failf(XQ_ERR_UNSUPPORTED, "more than 65535 sequences");
+    const size_t es = type_size(logits->type);
+    if (logits->nb[0] != es) return failf(XQ_ERR_UNSUPPORTED, "%s: elements must be contiguous", what);
+    if (logits->nb[1] % es || logits->nb[2] % es || !aligned(logits->data, es)) return failf(XQ_ERR_UNSUPPORTED, "misaligned %s", what);
+    return XQ_OK;
+}
+
+static size_t verify_space(const xq_tensor* l, size_t* walk_at, size_t* sums_at) {
+    const size_t chunks = (size_t)cdiv(l->ne[0], kVChunk), B = (size_t)l->ne[2];
+    *walk_at = B * (size_t)l->ne[1] * chunks * sizeof(RowStat);
+    *sums_at = *walk_at + B * sizeof(Walk);
+    return *sums_at + 2 * B * chunks * 8;
+}
+
+template <bool WIDE>
+static void verify_launch(const VerifyArgs& a, hipStream_t s) {
+    launch("verify_stats", verify_stats_kernel<WIDE>, dim3((uint32_t)a.chunks, (uint32_t)a.n_q, (uint32_t)a.B), dim3(256), s, a);
+    // (all greedy: the path and the maxima are the whole answer)
+    launch("verify_sums", verify_sums_kernel<WIDE, 0>, dim3(a.uniform ? (uint32_t)a.chunks : 1u, (uint32_t)a.B), dim3(256), s, a);
+    if (!a.uniform) return;
+    if (a.draft) launch("verify_left", verify_sums_kernel<WIDE, 1>, dim3((uint32_t)a.chunks, (uint32_t)a.B), dim3(256), s, a);
+    launch("verify_pick", verify_pick_kernel<WIDE>, dim3((uint32_t)a.B), dim3(1024), s, a);
+}
+
+}  // namespace xq
+
+using namespace xq;
+
+extern "C" {
+
+xq_status xq_verify_tokens_workspace(const xq_tensor* logits, size_t* bytes) {
+    if (!bytes) return failf(XQ_ERR_BAD_ARG, "bytes is null");
+    const xq_status st = verify_check(logits, "logits");
+    if (st != XQ_OK) return st;
+    size_t w, s;
+    *bytes = verify_space(logits, &w, &s);
+    return done_ok();
+}
+
+xq_status xq_verify_tokens(const xq_tensor* logits, const xq_tensor* draft, const int32_t* tokens, const int32_t* parents,
+                           const int32_t* n_tok, const float* temperature, const float* uniform, int32_t* path, int32_t* n_path,
+                           int32_t* next, float* logp, void* workspace, size_t workspace_bytes, void* stream) {
+    xq_status st = verify_check(logits, "logits");
+    if (st == XQ_OK && draft) st = verify_check(draft, "draft");
+    if (st != XQ_OK) return st;
+    if (draft) {
+        if (draft->type != logits->type) return failf(XQ_ERR_UNSUPPORTED, "draft must have logits' type");
+        for (int i = 0; i < 3; ++i)
+            if (draft->ne[i] != logits->ne[i]) return failf(XQ_ERR_BAD_SHAPE, "draft must have logits' shape");
+        if (parents) return failf(XQ_ERR_UNSUPPORTED, "a draft's distributions go with a chain: parents must be NULL");
+        if (!uniform) return failf(XQ_ERR_BAD_ARG, "a draft's distributions need random numbers");
+    }
+    if (!logits->data || (draft && !draft->data) || !tokens || !path || !n_path || !next) return failf(XQ_ERR_BAD_ARG, "null pointer");
+    for (const void* x : {(const void*)tokens, (const void*)parents, (const void*)n_tok, (const void*)temperature, (const void*)uniform,
+                          (const void*)path, (const void*)n_path, (const void*)next, (const void*)logp})
+        if (!aligned(x, 4)) return failf(XQ_ERR_UNSUPPORTED, "misaligned pointer");
+    size_t walk_at, sums_at;
+    const size_t need = verify_space(logits, &walk_at, &sums_at);
+    if (!workspace || workspace_bytes < need) return failf(XQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    if (!aligned(workspace, 256)) return failf(XQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    VerifyArgs a{};
+    a.logits = (const uint8_t*)logits->data;
+    a.l_nb1 = (int64_t)logits->nb[1], a.l_nb2 = (int64_t)logits->nb[2];
+    if (draft) {
+        a.draft = (const uint8_t*)draft->data;
+        a.q_nb1 = (int64_t)draft->nb[1], a.q_nb2 = (int64_t)draft->nb[2];
+    }
+    a.tokens = tokens, a.parents = parents, a.n_tok = n_tok, a.temperature = temperature, a.uniform = uniform;
+    a.path = path, a.n_path = n_path, a.next = next, a.logp = logp;
+    a.V = (int32_t)logits->ne[0], a.n_q = (int32_t)logits->ne[1], a.B = (int32_t)logits->ne[2];
+    a.chunks = (int32_t)cdiv(a.V, kVChunk);
+    a.stats = (RowStat*)workspace;
+    a.walk = (Walk*)((uint8_t*)workspace + walk_at);
+    a.sums = (double*)((uint8_t*)workspace + sums_at);
+    hipStream_t s = (hipStream_t)stream;
+    logits->type == XQ_TYPE_F32 ? verify_launch<true>(a, s) : verify_launch<false>(a, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return failf(XQ_ERR_HIP, "verify_tokens launch: %s", hipGetErrorString(e));
+    return done_ok();
+}
+
+}  // extern "C"

@@ -14,7 +14,8 @@ Mirrors the ggml op interface of the reference path:
   ``fa_range``         RemoteAttnEngine::attend_range (uwp/rkva/remote-attn-engine.h:152-154)
   ``gated_delta_net``  GGML_OP_GATED_DELTA_NET (src/bridge/ggml_d3d12.cpp:77-158,1905-1942)
   ``kv_store``         KV append (shaders/rkva/rkva_store_f16.hlsl:63-85, all KV types)
-The paged KV cache (``qk_norm_rope``, ``fa_tree``, ``kv_pages_*``) is in ``paged.py``.
+The paged KV cache (``qk_norm_rope``, ``fa_tree``, ``fa_chunk``, ``kv_weights``, ``verify_tokens``,
+``kv_pages_*``) is in ``paged.py``.
 """
 from __future__ import annotations
 
@@ -50,6 +51,8 @@ EXPORTS = (
     "xq_supports_qk_norm_rope", "xq_qk_norm_rope", "xq_supports_fa_tree", "xq_fa_tree_workspace", "xq_fa_tree",
     "xq_kv_pages_copy", "xq_kv_pages_compact", "xq_kv_pages_reserve_workspace", "xq_kv_pages_reserve",
     "xq_kv_pages_fork_workspace", "xq_kv_pages_fork", "xq_kv_pages_release",
+    "xq_supports_fa_chunk", "xq_fa_chunk_workspace", "xq_fa_chunk", "xq_kv_weights_workspace", "xq_kv_weights",
+    "xq_kv_pages_evict_workspace", "xq_kv_pages_evict", "xq_verify_tokens_workspace", "xq_verify_tokens",
 )
 
 
@@ -521,6 +524,8 @@ class GgmlBackend:
 # the paged KV cache (needs the names above)
 # ---------------------------------------------------------------------------
 
-from .paged import (ROPE_HALVES, ROPE_PAIRS, KvPages, XqKvPages, XqRopeParams, fa_tree, fa_tree_workspace,  # noqa: E402,F401
-                    kv_pages_compact, kv_pages_copy, kv_pages_fork, kv_pages_release, kv_pages_reserve, pool_tensor,
-                    qk_norm_rope, rope_params, signatures, supports_fa_tree, supports_qk_norm_rope)
+from .paged import (ROPE_HALVES, ROPE_PAIRS, KvPages, XqChunkParams, XqKvPages, XqRopeParams, chunk_params,  # noqa: E402,F401
+                    fa_chunk, fa_chunk_workspace, fa_tree, fa_tree_workspace, kv_pages_compact, kv_pages_copy, kv_pages_evict,
+                    kv_pages_fork, kv_pages_release, kv_pages_reserve, kv_weights, kv_weights_workspace, pool_tensor, qk_norm_rope,
+                    rope_params, signatures, supports_fa_chunk, supports_fa_tree, supports_qk_norm_rope, verify_tokens,
+                    verify_tokens_workspace)

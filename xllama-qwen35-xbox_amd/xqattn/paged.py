@@ -1,6 +1,7 @@
 """Host binding of the paged KV cache (``include/xq_attn.h``, "A KV cache in pages"):
-norms and rotation of queries and keys into the cache, attention of drafted tokens over
-it, and the pages themselves. Like the rest of the binding it only fills descriptors
+norms and rotation of queries and keys into the cache, attention of drafted tokens and of
+whole chunks over it, the weight its rows get, the verification of drafted tokens, and the
+pages themselves. Like the rest of the binding it only fills descriptors
 and hands over workspaces and the stream; torch holds the memory.
 
 ``KvPages`` is one layer's cache; the page operations take a list of pools (K and V of
@@ -45,6 +46,20 @@ class XqRopeParams(ctypes.Structure):
 
 def rope_params(n_rot, freq_base, freq_scale=1.0, attn_factor=1.0, mode=ROPE_HALVES, eps=1e-6, q8_variant=0) -> XqRopeParams:
     return XqRopeParams(n_rot, mode, freq_base, freq_scale, attn_factor, eps, q8_variant, 0)
+
+
+class XqChunkParams(ctypes.Structure):
+    _fields_ = [
+        ("scale", ctypes.c_float),
+        ("max_bias", ctypes.c_float),
+        ("logit_softcap", ctypes.c_float),
+        ("window", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+
+
+def chunk_params(scale, window=0, logit_softcap=0.0, max_bias=0.0) -> XqChunkParams:
+    return XqChunkParams(scale, max_bias, logit_softcap, window)
 
 
 def pool_tensor(t, kv_type: int, head_dim: int, page_rows: int, n_head_kv: int, n_pages: int, head_major=False) -> DevTensor:
@@ -189,6 +204,68 @@ def fa_tree(q: DevTensor, cache: KvPages, dst: DevTensor, scale: float, parents=
     return ws
 
 
+def supports_fa_chunk(q, cache: KvPages, dst) -> bool:
+    dq, c, dd = q.desc(), cache.struct(), dst.desc()
+    return bool(load().xq_supports_fa_chunk(ctypes.byref(dq), ctypes.byref(c), ctypes.byref(dd)))
+
+
+def fa_chunk_workspace(q, cache: KvPages, dst) -> int:
+    dq, c, dd = q.desc(), cache.struct(), dst.desc()
+    n = ctypes.c_size_t(0)
+    _check(load().xq_fa_chunk_workspace(ctypes.byref(dq), ctypes.byref(c), ctypes.byref(dd), ctypes.byref(n)), "fa_chunk_workspace")
+    return int(n.value)
+
+
+def _chunk_masks(q, first, prefix, n_tok):
+    _, n_q, _, n_seq = q.ne
+    for name, t, n in (("first", first, n_q * n_seq), ("prefix", prefix, n_seq), ("n_tok", n_tok, n_seq)):
+        _i32(name, t)
+        _size(name, t, n)
+    return [_ptr(first), _ptr(prefix), _ptr(n_tok)]
+
+
+def fa_chunk(q: DevTensor, cache: KvPages, dst: DevTensor, params: XqChunkParams, first=None, prefix=None, n_tok=None, lse=None,
+             workspace=None, stream=None):
+    """Attention of each sequence's chunk of new tokens over its cached rows and their own.
+    Returns the workspace, for the next call of these shapes."""
+    _, n_q, h, n_seq = q.ne
+    masks = _chunk_masks(q, first, prefix, n_tok)
+    _f32("lse", lse, n_q * h * n_seq)
+    dq, c, dd = q.desc(), cache.struct(), dst.desc()
+    n = fa_chunk_workspace(q, cache, dst)
+    with _on(stream, q.t, dst.t, first, prefix, n_tok, lse, cache.table, cache.rows, cache.k.t, cache.v.t, workspace) as s:
+        ws, wp, wn = _space(n, workspace, dst.t)
+        _check(load().xq_fa_chunk(ctypes.byref(dq), ctypes.byref(c), ctypes.byref(params), *masks, ctypes.byref(dd), _ptr(lse),
+                                  ctypes.c_void_p(wp), wn, s), "fa_chunk")
+    return ws
+
+
+def kv_weights_workspace(q, cache: KvPages) -> int:
+    dq, c = q.desc(), cache.struct()
+    n = ctypes.c_size_t(0)
+    _check(load().xq_kv_weights_workspace(ctypes.byref(dq), ctypes.byref(c), ctypes.byref(n)), "kv_weights_workspace")
+    return int(n.value)
+
+
+def kv_weights(q: DevTensor, cache: KvPages, params: XqChunkParams, lse, scores, scores_out, first=None, prefix=None, n_tok=None,
+               decay=1.0, fresh=True, workspace=None, stream=None):
+    """The cached rows' attention weights of a chunk's tokens, added to `scores` [n_seq, cols] (None: zeros)."""
+    _, n_q, h, n_seq = q.ne
+    masks = _chunk_masks(q, first, prefix, n_tok)
+    _f32("lse", lse, n_q * h * n_seq)
+    if scores_out.dim() != 2 or scores_out.shape[0] != n_seq or (scores is not None and scores.shape != scores_out.shape):
+        raise ValueError("scores and scores_out must be [n_seq, cols]")
+    _f32("scores", scores, scores_out.numel())
+    _f32("scores_out", scores_out, scores_out.numel())
+    dq, c = q.desc(), cache.struct()
+    n = kv_weights_workspace(q, cache)
+    with _on(stream, q.t, first, prefix, n_tok, lse, scores, scores_out, cache.table, cache.rows, cache.k.t, workspace) as s:
+        ws, wp, wn = _space(n, workspace, scores_out)
+        _check(load().xq_kv_weights(ctypes.byref(dq), ctypes.byref(c), ctypes.byref(params), *masks, _ptr(lse), _ptr(scores), _ptr(scores_out),
+                                    scores_out.shape[1], decay, int(fresh), ctypes.c_void_p(wp), wn, s), "kv_weights")
+    return ws
+
+
 def kv_pages_copy(pools, src, dst, stream=None):
     """Page dst[i] of every pool becomes page src[i]'s content."""
     _i32("src", src)
@@ -258,16 +335,83 @@ def kv_pages_release(table, rows, refs, seqs, stream=None):
                "kv_pages_release")
 
 
+def kv_pages_evict(pools, table, rows, refs, keep, scores, rows_out, first_rows=0, last_rows=0, positions=None, scores_out=None,
+                   positions_out=None, workspace=None, stream=None):
+    """Each sequence keeps keep[b] of its rows: protected ones, then those of most weight. refs
+    (or None: no page is shared or given back)."""
+    for name, t, dims in (("table", table, 2), ("rows", rows, 1), ("refs", refs, 1), ("keep", keep, 1), ("positions", positions, 2),
+                          ("positions_out", positions_out, 2), ("rows_out", rows_out, 1)):
+        _i32(name, t, dims)
+    for name, t in (("rows", rows), ("keep", keep), ("rows_out", rows_out)):
+        _size(name, t, table.shape[0])
+    if scores.dim() != 2 or scores.shape[0] != table.shape[0]:
+        raise ValueError("scores must have one row per sequence")
+    for name, t in (("scores", scores), ("scores_out", scores_out)):
+        _f32(name, t, scores.numel())
+    for name, t in (("positions", positions), ("scores_out", scores_out), ("positions_out", positions_out)):
+        if t is not None and t.shape != scores.shape:
+            raise ValueError(f"{name} must have scores' shape")
+    arr, m = _pools(pools)
+    if refs is not None and arr[0].ne[3] != refs.numel():
+        raise ValueError("refs must hold one number per page")
+    n = ctypes.c_size_t(0)
+    _check(load().xq_kv_pages_evict_workspace(table.shape[0], scores.shape[1], ctypes.byref(n)), "kv_pages_evict_workspace")
+    with _on(stream, table, rows, refs, keep, scores, positions, scores_out, positions_out, rows_out, workspace, *_memory(pools)) as s:
+        ws, wp, wn = _space(n.value, workspace, table)
+        _check(load().xq_kv_pages_evict(arr, m, _ptr(table), _ptr(rows), _ptr(refs), *table.shape, _ptr(keep), first_rows, last_rows,
+                                        _ptr(scores), _ptr(positions), scores.shape[1], _ptr(scores_out), _ptr(positions_out),
+                                        _ptr(rows_out), ctypes.c_void_p(wp), wn, s), "kv_pages_evict")
+    return ws
+
+
+def verify_tokens_workspace(logits) -> int:
+    d = logits.desc()
+    n = ctypes.c_size_t(0)
+    _check(load().xq_verify_tokens_workspace(ctypes.byref(d), ctypes.byref(n)), "verify_tokens_workspace")
+    return int(n.value)
+
+
+def verify_tokens(logits: DevTensor, tokens, path, n_path, next_token, uniform=None, draft: DevTensor = None, parents=None, n_tok=None,
+                  temperature=None, logp=None, workspace=None, stream=None):
+    """Which drafted tokens stand (path, n_path) and the token after them; uniform None: greedy."""
+    _, n_q, n_seq, _ = logits.ne
+    for name, t, n in (("tokens", tokens, n_q * n_seq), ("parents", parents, n_q * n_seq), ("n_tok", n_tok, n_seq), ("path", path, n_q * n_seq),
+                       ("n_path", n_path, n_seq), ("next_token", next_token, n_seq)):
+        _i32(name, t)
+        _size(name, t, n)
+    for name, t, n in (("temperature", temperature, n_seq), ("uniform", uniform, n_seq * (n_q + 1)), ("logp", logp, n_seq * (n_q + 1))):
+        _f32(name, t, n)
+    dl, dd = logits.desc(), None if draft is None else draft.desc()
+    n = verify_tokens_workspace(logits)
+    with _on(stream, logits.t, None if draft is None else draft.t, tokens, parents, n_tok, temperature, uniform, path, n_path, next_token,
+             logp, workspace) as s:
+        ws, wp, wn = _space(n, workspace, tokens)
+        _check(load().xq_verify_tokens(ctypes.byref(dl), None if dd is None else ctypes.byref(dd), _ptr(tokens), _ptr(parents), _ptr(n_tok),
+                                       _ptr(temperature), _ptr(uniform), _ptr(path), _ptr(n_path), _ptr(next_token), _ptr(logp),
+                                       ctypes.c_void_p(wp), wn, s), "verify_tokens")
+    return ws
+
+
 def signatures():
     """ctypes argument types of this file's exports."""
     T, P, i32, f32, sz = ctypes.POINTER(XqTensor), ctypes.c_void_p, ctypes.c_int32, ctypes.c_float, ctypes.c_size_t
     C, R, S = ctypes.POINTER(XqKvPages), ctypes.POINTER(XqRopeParams), ctypes.POINTER(ctypes.c_size_t)
+    K = ctypes.POINTER(XqChunkParams)
     return {
         "xq_supports_qk_norm_rope": (ctypes.c_int, [T, T, T, R, T, C]),
         "xq_qk_norm_rope": (i32, [T, T, T, P, P, P, P, P, R, T, C, P]),
         "xq_supports_fa_tree": (ctypes.c_int, [T, C, T]),
         "xq_fa_tree_workspace": (i32, [T, C, T, S]),
         "xq_fa_tree": (i32, [T, C, P, P, T, P, f32, P, sz, P]),
+        "xq_supports_fa_chunk": (ctypes.c_int, [T, C, T]),
+        "xq_fa_chunk_workspace": (i32, [T, C, T, S]),
+        "xq_fa_chunk": (i32, [T, C, K, P, P, P, T, P, P, sz, P]),
+        "xq_kv_weights_workspace": (i32, [T, C, S]),
+        "xq_kv_weights": (i32, [T, C, K, P, P, P, P, P, P, i32, f32, i32, P, sz, P]),
+        "xq_kv_pages_evict_workspace": (i32, [i32, i32, S]),
+        "xq_kv_pages_evict": (i32, [T, i32, P, P, P, i32, i32, P, i32, i32, P, P, i32, P, P, P, P, sz, P]),
+        "xq_verify_tokens_workspace": (i32, [T, S]),
+        "xq_verify_tokens": (i32, [T, T, P, P, P, P, P, P, P, P, P, P, sz, P]),
         "xq_kv_pages_copy": (i32, [T, i32, P, P, i32, P]),
         "xq_kv_pages_compact": (i32, [T, i32, P, P, i32, i32, P, P, i32, P, P]),
         "xq_kv_pages_reserve_workspace": (i32, [i32, i32, S]),
