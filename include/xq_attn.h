@@ -495,7 +495,7 @@ xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chu
  *   lse     F32 [n_seq][n_q][n_head] (device), of xq_fa_chunk or xq_fa_tree; -inf: a token without weight
  *   scores  F32 [n_seq][score_cols] (device), or NULL: zeros; scores_out the same, and may be scores
  * Scores are those of the decoded cache at 22 bits and more whatever q's type, sums in f32, in an order
- * that depends on the shapes alone. decay finite. */
+ * that depends on the shapes alone. decay finite. A table of fewer than 2^28 rows; the workspace may be of 0 bytes. */
 xq_status xq_kv_weights_workspace(const xq_tensor* q, const xq_kv_pages* cache, size_t* bytes);
 xq_status xq_kv_weights(const xq_tensor* q, const xq_kv_pages* cache, const xq_chunk_params* params, const int32_t* first,
                         const int32_t* prefix, const int32_t* n_tok, const float* lse, const float* scores, float* scores_out,
@@ -582,7 +582,7 @@ xq_status xq_kv_pages_evict(const xq_tensor* pools, int32_t n_pools, int32_t* ta
  * and that one is next.
  *   logits  F32|BF16 [V, n_q, n_seq], n_q <= 64, V <= 2^24, elements contiguous, other strides free; NaN counts as -inf, and
  *           of +inf each has the same mass
- *   draft   logits' type and shape (probabilities), or NULL
+ *   draft   logits' type and shape (probabilities; NaN and what is below 0 count as 0), or NULL
  *   tokens  I32 [n_seq][n_q] (device); one outside [0, V) never stands
  *   parents, n_tok  as for xq_fa_tree; a token that does not descend from token 0 is never reached
  *   temperature  F32 [n_seq] (device), or NULL: 1

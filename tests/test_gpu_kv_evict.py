@@ -144,6 +144,13 @@ def test_rows_beyond_table_or_columns_leave_a_sequence(torch_gpu):
     assert {m[0] for m in w.run(torch_gpu, [30] * 3, note="rows beyond")} == {1}
 
 
+@pytest.mark.parametrize("n,k", [(40000, 39990), (33000, 5)])
+def test_more_rows_than_lds_holds(torch_gpu, n, k):
+    w = World(12, "e5m2", 32, 1, 64, [n, 100])
+    w.positions = np.stack([w.rng.permutation(w.width) for _ in range(2)]).astype(np.int32)
+    w.run(torch_gpu, [k, 50], first=4, last=100, note=f"{n} rows to {k}")
+
+
 def test_in_place_again_and_again(torch_gpu):
     """A cache held at its budget: a new row each step, weights and positions moved in place."""
     w = World(8, "q8_0", 128, 2, 16, [41, 50], spare=4)

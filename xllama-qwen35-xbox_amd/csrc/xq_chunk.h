@@ -52,6 +52,58 @@ XQ_DEV float capped_tanh(float z) {
     return fabsf(z) < 0.2f ? near : far;
 }
 
+// A query as matrix operands, which may have the inner elements in any order that the keys have too: with
+// EL 8, operand c takes elements 8lg .. + 7 of the c-th 32; else a lane has EL neighbours of each 4 EL, eight at
+// a time. First as they lie in memory,
+template <int EL>
+constexpr int operand_at(int c) {
+    return c / (EL / 8) * 4 * EL + c % (EL / 8) * 8;
+}
+template <int NB, bool NARROW, int EL = 8>
+XQ_DEV void query_load(const uint8_t* q, int lg, float (&x)[NB][8]) {
+#pragma unroll
+    for (int c = 0; c < NB; ++c) {
+        const int e = operand_at<EL>(c) + EL * lg;
+        if constexpr (NARROW) {
+            const u4half y = *(const u4half*)(q + 2 * e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[c][2 * i] = __uint_as_float(y[i] << 16);
+                x[c][2 * i + 1] = __uint_as_float(y[i] & 0xffff0000u);
+            }
+        } else {
+            const f4el y = *(const f4el*)(q + 4 * e), z = *(const f4el*)(q + 4 * e + 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[c][i] = y[i];
+                x[c][4 + i] = z[i];
+            }
+        }
+    }
+}
+// then in f16 (QP 2: high and low part) times 2^lift, which puts the row's largest element in [2^14, 2^15),
+// and the sign of the scale. Returns the factor that makes scores of the products: |scale| 2^-lift times `unit`,
+// a normal number: an unseen score's -inf stays one, and a score of 0 too.
+template <int NB, int QP>
+XQ_DEV float query_split(const float (&x)[NB][8], float scale, float unit, h8t (&o)[NB][QP]) {
+    float big = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[c][j]));
+    const int lift = 141 - min((int)(__float_as_uint(across_rows_max(big)) >> 23), 254);
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = ldexpf(scale < 0.0f ? -x[c][j] : x[c][j], lift);
+            const _Float16 high = (_Float16)y;
+            o[c][0][j] = high;
+            if constexpr (QP == 2) o[c][1][j] = (_Float16)(y - (float)high);
+        }
+    return fminf(fmaxf(ldexpf(fabsf(scale), -lift) * unit, 1.17549435e-38f), 3.40282347e38f);
+}
+
 // The bits of a 64-row tile from row r0 on that lie in [lo, hi).
 XQ_DEV uint64_t tile_rows(int r0, int lo, int hi) {
     const int a = min(max(lo - r0, 0), 64), b = min(max(hi - r0, 0), 64);

@@ -3,8 +3,8 @@
 // Per sequence with n rows and a budget k below n: the rows are ordered by (protected first, larger
 // weight, lower index) and the first k stay. Those of them that lie at index k or behind move, in
 // order, to the places below k that others leave, in order: no row is both read and written, so all
-// move at once, and no more bytes than have to. One workgroup per sequence selects (the weights are
-// read from L2 a few times: a radix search for the k-th key, then ranks by ballots), and writes a list
+// move at once, and no more bytes than have to. One workgroup per sequence selects (its rows' keys
+// in LDS: a radix search for the k-th, then ranks by ballots), and writes a list
 // of (page, row) pairs; a second launch moves them in every pool and gives pages without rows back.
 #include "xq_pools.h"
 
@@ -54,74 +54,136 @@ XQ_DEV uint32_t before_wave(uint32_t mine, uint32_t* lds, uint32_t* total) {
     return before;
 }
 
+// The keys of up to kHeldRows rows stay in LDS, and so do the lists of their moves: a pass over them costs no
+// memory round trip (about 1 us each, of a lone workgroup). Longer sequences read them again in each pass.
+constexpr int kHeldRows = 24576;
+
+template <bool HELD>
 __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t hist[256], lds[kEvictWaves], found[2];
+    constexpr int BINS = 2048;
+    __shared__ uint32_t hist[BINS], lds[kEvictWaves], found[2];
+    __shared__ uint16_t list[2][HELD ? kHeldRows / 2 + 2 : 2];
+    __shared__ uint32_t keys[HELD ? kHeldRows : 1];
+    __shared__ uint64_t safes[HELD ? kHeldRows / 64 : 1];
     const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wave = wave_id();
     const int n = a.rows[b], k = max(a.keep[b], 0);
     const float* const score = a.scores + (int64_t)b * a.score_cols;
     const int32_t* const position = a.positions ? a.positions + (int64_t)b * a.score_cols : nullptr;
+    float* const score_out = a.scores_out && a.scores_out != a.scores ? a.scores_out + (int64_t)b * a.score_cols : nullptr;
+    int32_t* const position_out = a.positions_out && a.positions_out != a.positions ? a.positions_out + (int64_t)b * a.score_cols : nullptr;
     const bool held = n >= 0 && n <= a.score_cols && n <= a.row_limit;
     const bool cut = held && n > k;
-    auto pos = [&](int r) { return position ? position[r] : r; };
-    // the newest position
-    int newest = -0x7fffffff - 1;
-    if (cut) {
-        for (int r = tid; r < n; r += kEvictThreads) newest = max(newest, pos(r));
+    // rows [w0, w0 + span) are this wave's, 64 at a time
+    const int span = held ? ((n + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64 : 0, w0 = wave * span;
+    int newest = position ? -0x7fffffff - 1 : n - 1;
+    auto is_safe = [&](int p) { return p < a.first_rows || (int64_t)newest - p < a.last_rows; };
+    // ---- keys, the newest position, and the weights and positions that stay where they are
+    constexpr int U = 4;  // loads of a thread at once
+    for (int r0 = w0; r0 < w0 + span; r0 += 64 * U) {
+        float x[U];
+        int32_t p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = min(r0 + 64 * u + lane, n - 1);
+            x[u] = score[r];
+            p[u] = position ? position[r] : r;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + 64 * u + lane;
+            newest = max(newest, p[u]);
+            if (r >= min(n, w0 + span)) continue;
+            if constexpr (HELD) keys[r] = weight_key(x[u]);
+            if (cut && r >= k) continue;
+            if (score_out) score_out[r] = x[u];
+            if (position_out) position_out[r] = p[u];
+        }
+    }
+    if (position) {
 #pragma unroll
         for (int s = 1; s < 64; s *= 2) newest = max(newest, __shfl_xor(newest, s));
         if (lane == 0) lds[wave] = (uint32_t)newest;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kEvictWaves; ++i) newest = max(newest, (int)lds[i]);
-        __syncthreads();
     }
-    auto safe = [&](int r) {
-        const int64_t p = pos(r);
-        return p < a.first_rows || (int64_t)newest - p < a.last_rows;
+    uint32_t my_safe = 0;
+    if (cut)
+        for (int r0 = w0; r0 < w0 + span; r0 += 64 * U) {
+            int32_t p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = min(r0 + 64 * u + lane, n - 1);
+                p[u] = position ? position[r] : r;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + 64 * u + lane;
+                const uint64_t s = __builtin_amdgcn_ballot_w64(r < min(n, w0 + span) && is_safe(p[u]));
+                if (HELD && lane == 0 && r0 + 64 * u < w0 + span) safes[(r0 + 64 * u) / 64] = s;
+                my_safe += __builtin_popcountll(s);
+            }
+        }
+    // f(row, whether it is one, its key, whether it is protected) of this wave's rows; all 64 lanes take part
+    auto each = [&](auto f) {
+        for (int r0 = w0; r0 < w0 + span; r0 += 64) {
+            const int r = min(r0 + lane, n - 1);
+            const bool on = r0 + lane < n;
+            if constexpr (HELD) f(r0 + lane, on, keys[r], (bool)(safes[r0 / 64] >> lane & 1));
+            else f(r0 + lane, on, weight_key(score[r]), on && is_safe(position ? position[r] : r));
+        }
     };
-    // rows [w0, w1) are this wave's, 64 at a time
-    const int span = ((n + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
-    const int w0 = min(n, wave * span), w1 = min(n, w0 + span);
     uint32_t moves = 0;
     bool done = cut;
+    int32_t* const far_list = a.lists + (int64_t)b * 2 * a.half;  // (!HELD)
+    auto hole_at = [&](uint32_t i) -> int { return HELD ? list[0][i] : far_list[i]; };
+    auto tail_at = [&](uint32_t i) -> int { return HELD ? list[1][i] : far_list[a.half + i]; };
     if (cut) {
         uint32_t mine = 0, n_safe;
-        for (int r0 = w0; r0 < w1; r0 += 64) mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r0 + lane < w1 && safe(r0 + lane)));
-        before_wave(mine, lds, &n_safe);
+        before_wave(my_safe, lds, &n_safe);
         // the group that is cut: protected rows where those alone exceed the budget, else the others,
         // of which `want` stay: all keys above `key`, and the first `ties` that equal it
         const bool among_safe = n_safe > (uint32_t)k;
         const uint32_t want = among_safe ? (uint32_t)k : (uint32_t)k - n_safe;
         uint32_t key = 0, left = want;
         if (want) {
-            for (int shift = 24; shift >= 0; shift -= 8) {
+            // the key's 11, 11 and 10 bits from above, by the counts of each value
+#pragma unroll 1
+            for (int step = 0; step < 3; ++step) {
+                const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, seen = step == 0 ? 31 : step == 1 ? 21 : 10;
+                const uint32_t mask = step == 2 ? 1023u : 2047u;
                 __syncthreads();
-                if (tid < 256) hist[tid] = 0;
+                hist[2 * tid] = hist[2 * tid + 1] = 0;
                 __syncthreads();
-                for (int r = tid; r < n; r += kEvictThreads) {
-                    const uint32_t x = weight_key(score[r]);
-                    if (safe(r) == among_safe && (shift == 24 || (x ^ key) >> (shift + 8) == 0)) atomicAdd(&hist[(x >> shift) & 255u], 1u);
+                each([&](int, bool on, uint32_t x, bool s) {
+                    const bool counts = on && s == among_safe && (step == 0 || (x ^ key) >> seen == 0);
+                    const uint32_t bin = counts ? (x >> shift) & mask : ~0u;
+                    // lanes of one lane's bin as one: many rows may have the same weight
+                    const uint32_t one = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
+                    const uint64_t same = __builtin_amdgcn_ballot_w64(bin == one);
+                    if (counts && bin != one) atomicAdd(&hist[bin], 1u);
+                    if (lane == 0 && one != ~0u) atomicAdd(&hist[one], (uint32_t)__builtin_popcountll(same));
+                });
+                __syncthreads();
+                // thread t: bins 2t and 2t + 1; how many lie in the bins above
+                const uint32_t h0 = hist[2 * tid], h1 = hist[2 * tid + 1];
+                uint32_t up = h0 + h1;
+#pragma unroll
+                for (int s = 1; s < 64; s *= 2) {
+                    const uint32_t y = __shfl_down(up, s);
+                    if (lane + s < 64) up += y;
                 }
+                if (lane == 0) lds[wave] = up;
                 __syncthreads();
-                if (wave == 0) {
-                    // lane l: bins 4l .. 4l + 3; how many lie in the bins above
-                    const uint32_t h0 = hist[4 * lane], h1 = hist[4 * lane + 1], h2 = hist[4 * lane + 2], h3 = hist[4 * lane + 3];
-                    uint32_t up = h0 + h1 + h2 + h3;
+                uint32_t above = up - (h0 + h1);
 #pragma unroll
-                    for (int s = 1; s < 64; s *= 2) {
-                        const uint32_t y = __shfl_down(up, s);
-                        if (lane + s < 64) up += y;
-                    }
-                    uint32_t above = up - (h0 + h1 + h2 + h3);
-                    const uint32_t h[4] = {h0, h1, h2, h3};
-#pragma unroll
-                    for (int i = 3; i >= 0; --i) {
-                        if (above < left && above + h[i] >= left) {
-                            found[0] = (uint32_t)(4 * lane + i);
-                            found[1] = left - above;
-                        }
-                        above += h[i];
-                    }
+                for (int i = 0; i < kEvictWaves; ++i) above += i > wave ? lds[i] : 0u;
+                if (above < left && above + h1 >= left) {
+                    found[0] = 2 * tid + 1;
+                    found[1] = left - above;
+                } else if (above + h1 < left && above + h1 + h0 >= left) {
+                    found[0] = 2 * tid;
+                    found[1] = left - above - h1;
                 }
                 __syncthreads();
                 key |= found[0] << shift;
@@ -131,65 +193,86 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
         const uint32_t ties = want ? left : 0u;
         // ranks of the ties, in the rows' order
         mine = 0;
-        for (int r0 = w0; r0 < w1; r0 += 64)
-            mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(r0 + lane < w1 && safe(r0 + lane) == among_safe && weight_key(score[r0 + lane]) == key));
+        each([&](int, bool on, uint32_t x, bool s) { mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && s == among_safe && x == key)); });
         uint32_t total, tie0 = before_wave(mine, lds, &total);
-        // f(row, stays) for this wave's rows; all 64 lanes take part
-        auto rows = [&](auto f) {
+        // f(row, a place that it leaves, whether it is to move)
+        auto sorted = [&](auto f) {
             uint32_t tie = tie0;
-            for (int r0 = w0; r0 < w1; r0 += 64) {
-                const int r = r0 + lane;
-                const bool on = r < w1, s = on && safe(r), group = on && s == among_safe;
-                const uint32_t x = on ? weight_key(score[r]) : 0u;
+            each([&](int r, bool on, uint32_t x, bool s) {
+                const bool group = on && s == among_safe;
                 const uint64_t eq = __builtin_amdgcn_ballot_w64(group && x == key);
                 const uint32_t rank = tie + __builtin_popcountll(eq & (((uint64_t)1 << lane) - 1));
-                f(r, on, on && (group ? want && (x > key || (x == key && rank < ties)) : !among_safe && s));
+                const bool stays = on && (group ? want && (x > key || (x == key && rank < ties)) : !among_safe && s);
                 tie += __builtin_popcountll(eq);
-            }
+                f(r, __builtin_amdgcn_ballot_w64(on && !stays && r < k), __builtin_amdgcn_ballot_w64(stays && r >= k));
+            });
         };
         uint32_t holes = 0, tails = 0;
-        rows([&](int r, bool on, bool stays) {
-            holes += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && !stays && r < k));
-            tails += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && stays && r >= k));
+        sorted([&](int, uint64_t h, uint64_t t) {
+            holes += __builtin_popcountll(h);
+            tails += __builtin_popcountll(t);
         });
         uint32_t hole0 = before_wave(holes, lds, &moves), tail0 = before_wave(tails, lds, &total);
-        int32_t* const hole = a.lists + (int64_t)b * 2 * a.half;
-        int32_t* const tail = hole + a.half;
-        rows([&](int r, bool on, bool stays) {
+        sorted([&](int r, uint64_t h, uint64_t t) {
             const uint64_t below = ((uint64_t)1 << lane) - 1;
-            const uint64_t x = __builtin_amdgcn_ballot_w64(on && !stays && r < k), y = __builtin_amdgcn_ballot_w64(on && stays && r >= k);
-            if (x >> lane & 1) hole[hole0 + __builtin_popcountll(x & below)] = r;
-            if (y >> lane & 1) tail[tail0 + __builtin_popcountll(y & below)] = r;
-            hole0 += __builtin_popcountll(x);
-            tail0 += __builtin_popcountll(y);
+            const uint32_t x = hole0 + __builtin_popcountll(h & below), y = tail0 + __builtin_popcountll(t & below);
+            if (h >> lane & 1) HELD ? (void)(list[0][x] = (uint16_t)r) : (void)(far_list[x] = r);
+            if (t >> lane & 1) HELD ? (void)(list[1][y] = (uint16_t)r) : (void)(far_list[a.half + y] = r);
+            hole0 += __builtin_popcountll(h);
+            tail0 += __builtin_popcountll(t);
         });
         __syncthreads();
         // their places; a page that other sequences hold too is not written
         bool ok = true;
-        for (uint32_t i = tid; i < moves; i += kEvictThreads) {
-            const uint32_t from = (uint32_t)tail[i], to = (uint32_t)hole[i];
-            const uint32_t fc = a.d_page.quot(from), tc = a.d_page.quot(to);
-            const uint32_t fp = (uint32_t)a.table[(int64_t)b * a.cols + fc], tp = (uint32_t)a.table[(int64_t)b * a.cols + tc];
-            ok = ok && fp < (uint32_t)a.n_pages && tp < (uint32_t)a.n_pages && (!a.refs || a.refs[tp] <= 1);
-            a.moves[(int64_t)b * a.half + i] = make_int4((int)fp, (int)(from - fc * a.d_page.d), (int)tp, (int)(to - tc * a.d_page.d));
+        const int32_t* const row = a.table + (int64_t)b * a.cols;
+        for (uint32_t i0 = tid; i0 < moves; i0 += U * kEvictThreads) {
+            uint32_t fp[U], tp[U], fi[U], ti[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t i = min(i0 + u * kEvictThreads, moves - 1);
+                const uint32_t from = (uint32_t)tail_at(i), to = (uint32_t)hole_at(i);
+                const uint32_t fc = a.d_page.quot(from), tc = a.d_page.quot(to);
+                fp[u] = (uint32_t)row[fc], tp[u] = (uint32_t)row[tc];
+                fi[u] = from - fc * a.d_page.d, ti[u] = to - tc * a.d_page.d;
+            }
+            int32_t shared[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) shared[u] = a.refs && tp[u] < (uint32_t)a.n_pages ? a.refs[tp[u]] : 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                ok = ok && fp[u] < (uint32_t)a.n_pages && tp[u] < (uint32_t)a.n_pages && shared[u] <= 1;
+                const uint32_t i = i0 + u * kEvictThreads;
+                if (i < moves) a.moves[(int64_t)b * a.half + i] = make_int4((int)fp[u], (int)fi[u], (int)tp[u], (int)ti[u]);
+            }
         }
         done = __syncthreads_and(ok);
-    }
-    // weights and positions of the rows that are held now
-    const int32_t* const hole = a.lists + (int64_t)b * 2 * a.half;
-    const int rest = held ? (done ? k : n) : 0;
-    if (a.scores_out && a.scores_out != a.scores)
-        for (int r = tid; r < rest; r += kEvictThreads) a.scores_out[(int64_t)b * a.score_cols + r] = score[r];
-    if (a.positions_out && a.positions_out != a.positions)
-        for (int r = tid; r < rest; r += kEvictThreads) a.positions_out[(int64_t)b * a.score_cols + r] = pos(r);
-    __syncthreads();
-    if (done)
-        for (uint32_t i = tid; i < moves; i += kEvictThreads) {
-            const int64_t to = (int64_t)b * a.score_cols + hole[i];
-            const int from = hole[a.half + i];
-            if (a.scores_out) a.scores_out[to] = score[from];
-            if (a.positions_out) a.positions_out[to] = pos(from);
+        // weights and positions of the rows that move; a sequence left as it was keeps all
+        if (done) {
+            for (uint32_t i0 = tid; i0 < moves; i0 += U * kEvictThreads) {
+                float x[U];
+                int32_t p[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int from = tail_at(min(i0 + u * kEvictThreads, moves - 1));
+                    x[u] = a.scores_out ? score[from] : 0.0f;
+                    p[u] = position ? position[from] : from;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t i = i0 + u * kEvictThreads;
+                    if (i >= moves) continue;
+                    const int64_t to = (int64_t)b * a.score_cols + hole_at(i);
+                    if (a.scores_out) a.scores_out[to] = x[u];
+                    if (a.positions_out) a.positions_out[to] = p[u];
+                }
+            }
+        } else {
+            for (int r = k + tid; r < n; r += kEvictThreads) {
+                if (score_out) score_out[r] = score[r];
+                if (position_out) position_out[r] = position ? position[r] : r;
+            }
         }
+    }
     if (tid == 0) {
         a.rows_out[b] = done ? k : n;
         a.count[b] = done ? (int32_t)moves : 0;
@@ -300,7 +383,7 @@ xq_status xq_kv_pages_evict(const xq_tensor* pools, int32_t n_pools, int32_t* ta
     a.half = score_cols / 2 + 1;
     a.d_page = UDivFlat((uint32_t)page_rows);
     hipStream_t s = (hipStream_t)stream;
-    launch("kv_pages_evict", evict_select_kernel, dim3((uint32_t)n_seq), dim3(kEvictThreads), s, a);
+    launch("kv_pages_evict", score_cols <= kHeldRows ? evict_select_kernel<true> : evict_select_kernel<false>, dim3((uint32_t)n_seq), dim3(kEvictThreads), s, a);
     for (int32_t i0 = 0; i0 < n_pools; i0 += kPoolsPerLaunch) {
         const int32_t m = n_pools - i0 < kPoolsPerLaunch ? n_pools - i0 : kPoolsPerLaunch;
         PoolSet set{};

@@ -251,56 +251,18 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
     uint32_t page, in;
     lookup(t_first, page, in);
 
-    // ---- Q operands: pair 16m + lr, elements 8lg.. of each 32, times a power of two that
-    //      puts the row's largest element in [2^14, 2^15)
+    // ---- Q operands: pair 16m + lr
     h8t qo[MT][NB][QP];
     float qf[MT];
     {
-        float xq[MT][NB][8];
+        float x[MT][NB][8];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const int p = min(p0 + 16 * m + lr, n_pairs - 1);
-            const uint8_t* q = a.q + b * a.q_nb3 + tok[m] * a.q_nb1 + (hk * a.G + p - tok[m] * a.G) * a.q_nb2;
-#pragma unroll
-            for (int c = 0; c < NB; ++c) {
-                const int e = 32 * c + 8 * lg;
-                if constexpr (NARROW) {
-                    const u4half x = *(const u4half*)(q + 2 * e);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        xq[m][c][2 * i] = __uint_as_float(x[i] << 16);
-                        xq[m][c][2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
-                    }
-                } else {
-                    const f4el x = *(const f4el*)(q + 4 * e), y = *(const f4el*)(q + 4 * e + 16);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        xq[m][c][i] = x[i];
-                        xq[m][c][4 + i] = y[i];
-                    }
-                }
-            }
+            query_load<NB, NARROW>(a.q + b * a.q_nb3 + tok[m] * a.q_nb1 + (hk * a.G + p - tok[m] * a.G) * a.q_nb2, lg, x[m]);
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float big = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(xq[m][c][j]));
-            const int lift = 141 - min((int)(__float_as_uint(across_rows_max(big)) >> 23), 254);
-            // (a normal number: an unseen score's -inf stays one, and a score of 0 too)
-            qf[m] = fminf(fmaxf(ldexpf(fabsf(a.scale), -lift) * (BIASED ? 1.0f : kLog2e), 1.17549435e-38f), 3.40282347e38f);
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = ldexpf(a.scale < 0.0f ? -xq[m][c][j] : xq[m][c][j], lift);
-                    const _Float16 high = (_Float16)x;
-                    qo[m][c][0][j] = high;
-                    if constexpr (QP == 2) qo[m][c][1][j] = (_Float16)(x - (float)high);
-                }
-        }
+        for (int m = 0; m < MT; ++m) qf[m] = query_split<NB, QP>(x[m], a.scale, BIASED ? 1.0f : kLog2e, qo[m]);
     }
     fetch(page, in);
     uint64_t valid = __builtin_amdgcn_ballot_w64(page < (uint32_t)a.pg.n_pages);  // rows of raw's tile that have a page

@@ -28,7 +28,7 @@ struct RowStat {
 struct Walk {
     int32_t at, n;  // the last token of the path, its length; at -1: nothing left to draw
     uint64_t kids;  // its children
-    double max, heat, whole;  // of row `at`; whole: the stats' sum
+    double max, cool, whole;  // of row `at`: its maximum, 1 / temperature, the stats' sum
 };
 
 struct VerifyArgs {
@@ -85,7 +85,30 @@ XQ_DEV void elements(const uint8_t* row, int v, int V, float (&x)[N]) {
 
 // A weight relative to the maximum; +inf shares the mass where it is the maximum.
 XQ_DEV float weight_f32(float x, float max, float c) { return x == max ? 1.0f : __builtin_amdgcn_exp2f((x - max) * c); }
-XQ_DEV double weight_f64(double x, double max, double heat) { return x == max ? 1.0 : exp((x - max) / heat); }
+// e^d for d <= 0, off by less than 2^-51 of itself: d = k ln 2 + r, |r| <= ln 2 / 2, in two parts of ln 2; r's
+// series to the 13th power (the next term is 4e-18); 0 below 2^-1074. NaN (of +inf less itself) does not come here.
+XQ_DEV double exp_f64(double d) {
+    d = fmax(d, -1100.0);
+    const double k = rint(d * 1.4426950408889634);
+    const double r = fma(-k, 2.3190468138462996e-17, fma(-k, 0.6931471805599453, d));
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)k);
+}
+// `cool`: 1 / temperature
+XQ_DEV double weight_f64(double x, double max, double cool) { return exp_f64(x == max ? 0.0 : (x - max) * cool); }
 
 XQ_DEV float exponent_factor(float heat) { return fminf(kVLog2e / (heat > 0.0f ? heat : 1.0f), 3.40282347e38f); }
 
@@ -140,15 +163,32 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
 
 XQ_DEV uint64_t shfl64(uint64_t x, int l) { return ((uint64_t)(uint32_t)__shfl((int)(x >> 32), l) << 32) | (uint32_t)__shfl((int)(uint32_t)x, l); }
 XQ_DEV double shfl_f64(double x, int l) { return __builtin_bit_cast(double, shfl64(__builtin_bit_cast(uint64_t, x), l)); }
+// of a lane that is the same for all
+XQ_DEV double lane_f64(double x, int l) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)u, l));
+}
 
-// Sum over the workgroup's 256 threads, the same in all; the order is fixed.
+constexpr int kSumThreads = 1024, kSumEach = kVChunk / kSumThreads;
+
+// Sum over the workgroup's threads, the same in all; the order is fixed.
 XQ_DEV double block_sum(double x, double* lds) {
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) x += shfl_f64(x, lane_id() ^ s);
     __syncthreads();
     if (lane_id() == 0) lds[wave_id()] = x;
     __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    x = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSumThreads / 64; ++i) x += lds[i];
+    return x;
+}
+// Elements v .. v + 7 of a row.
+template <bool WIDE>
+XQ_DEV void eight(const uint8_t* row, int v, int V, float (&x)[kSumEach]) {
+    constexpr int N = WIDE ? 4 : 8;
+#pragma unroll
+    for (int i = 0; i < kSumEach; i += N) elements<WIDE, N>(row, v + i, V, *(float(*)[N])(x + i));
 }
 
 // The path, by one wave; a lane is a token. Every lane gets the same result.
@@ -156,7 +196,7 @@ template <bool WIDE>
 XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     const int c = lane_id(), n = a.tokens_of(b);
     const float heat = a.heat(b), f = exponent_factor(heat);
-    const double T = heat > 0.0f ? (double)heat : 1.0;
+    const double cool = heat > 0.0f ? 1.0 / (double)heat : 1.0;
     const bool live = c < n;
     // row c's maximum, sum and first index of the maximum
     float top = -INFINITY;
@@ -183,8 +223,8 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     double p = 0.0, lp = -INFINITY;
     if (known) {
         const double x = element<WIDE>(a.logits + b * a.l_nb2 + up * a.l_nb1, tok);
-        p = weight_f64(x, p_top, T) / p_whole;
-        lp = (x == (double)p_top ? 0.0 : (x - (double)p_top) / T) - log(p_whole);
+        p = weight_f64(x, p_top, cool) / p_whole;
+        lp = (x == (double)p_top ? 0.0 : (x - (double)p_top) * cool) - log(p_whole);
     }
     // earlier children of the same token: whether one has the same token; the mass of the others
     bool twice = false;
@@ -192,8 +232,8 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     uint64_t before = 0;
     if (a.parents)
         for (int i = 1; i < n - 1; ++i) {
-            const int iu = __shfl(up, i), it = __shfl(tok, i);
-            const double ip = shfl_f64(twice ? 0.0 : p, i);  // (lane i is through with its own: i' < i)
+            const int iu = __builtin_amdgcn_readlane(up, i), it = __builtin_amdgcn_readlane(tok, i);
+            const double ip = lane_f64(twice ? 0.0 : p, i);  // (lane i is through with its own: i' < i)
             if (c > i && up >= 0 && iu == up) {
                 before |= 1ull << i;
                 gone += ip;
@@ -206,7 +246,7 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     } else {
         const double u = live ? (double)a.uniform[(int64_t)b * (a.n_q + 1) + c] : 0.0;
         if (a.draft)
-            ok = known && u * (double)element<WIDE>(a.draft + b * a.q_nb2 + up * a.q_nb1, tok) < p;
+            ok = known && u * (double)fmaxf(element<WIDE>(a.draft + b * a.q_nb2 + up * a.q_nb1, tok), 0.0f) < p;
         else
             ok = known && !twice && u * (1.0 - gone) < p;
     }
@@ -230,7 +270,7 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     w.at = len ? last : -1;
     w.kids = __builtin_amdgcn_ballot_w64(live && up >= 0 && up == last) & (len ? ~0ull : 0ull);
     w.max = (double)__shfl(top, last);
-    w.heat = T;
+    w.cool = cool;
     w.whole = shfl_f64(whole, last);
     const int last_arg = __shfl(arg, last);
     if (write) {
@@ -255,12 +295,17 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     return w;
 }
 
-// What is left of element v's weight; `sum`: of row at's weights.
-template <bool WIDE>
-XQ_DEV double left_over(const VerifyArgs& a, const Walk& w, double x, const uint8_t* q, int v, double sum, const uint32_t* hit, int v0) {
-    const double p = weight_f64(x, w.max, w.heat);
-    if (q) return fmax(p / sum - (double)element<WIDE>(q, v), 0.0);
-    return hit[(v - v0) >> 5] >> ((v - v0) & 31) & 1u ? 0.0 : p;
+// Whether element i of the chunk is none of the rejected tokens.
+XQ_DEV bool kept(const uint32_t* hit, int i) { return !(hit[i >> 5] >> (i & 31) & 1u); }
+
+// The sum of n numbers one after another, 64 loaded at a time (every lane gets it).
+XQ_DEV double ordered_sum(const double* x, int n) {
+    double s = 0.0;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const double mine = i0 + lane_id() < n ? x[i0 + lane_id()] : 0.0;
+        for (int i = 0; i < min(64, n - i0); ++i) s += lane_f64(mine, i);
+    }
+    return s;
 }
 
 // The tokens of `kids` in the chunk from v0 on, as bits.
@@ -277,9 +322,9 @@ XQ_DEV void mark_kids(const VerifyArgs& a, const Walk& w, int b, int v0, uint32_
 // PART 0: the path, and the sums of a chunk of the row that the next token is drawn from: of its weights
 // and, without a draft, of what is left of them. PART 1: with a draft, the sum of what is left.
 template <bool WIDE, int PART>
-__global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kSumThreads) void verify_sums_kernel(VerifyArgs a) {
     __shared__ Walk shared;
-    __shared__ double lds[4];
+    __shared__ double lds[kSumThreads / 64];
     __shared__ uint32_t hit[kVChunk / 32];
     const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, v0 = j * kVChunk;
     if constexpr (PART == 0) {
@@ -298,19 +343,21 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
     const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
     if (PART == 1 && !q) return;
     double sum = 0.0;
-    if constexpr (PART == 1)
-        for (int i = 0; i < a.chunks; ++i) sum += a.sums[(int64_t)b * a.chunks + i];
-    else
-        mark_kids(a, w, b, v0, hit);
+    if constexpr (PART == 1) sum = ordered_sum(a.sums + (int64_t)b * a.chunks, a.chunks);
+    const int v = v0 + tid * kSumEach;
+    float x[kSumEach], y[kSumEach];
+    eight<WIDE>(row, v, a.V, x);
+    if constexpr (PART == 1) eight<WIDE>(q, v, a.V, y);
+    else mark_kids(a, w, b, v0, hit);
     double all = 0.0, left = 0.0;
-    for (int v = v0 + tid; v < min(a.V, v0 + kVChunk); v += 256) {
-        const double x = element<WIDE>(row, v);
+#pragma unroll
+    for (int i = 0; i < kSumEach; ++i) {
+        const double p = weight_f64(x[i], w.max, w.cool);
         if constexpr (PART == 0) {
-            const double p = weight_f64(x, w.max, w.heat);
             all += p;
-            left += hit[(v - v0) >> 5] >> ((v - v0) & 31) & 1u ? 0.0 : p;
-        } else {
-            left += left_over<WIDE>(a, w, x, q, v, sum, hit, v0);
+            left += kept(hit, v - v0 + i) ? p : 0.0;
+        } else if (v + i < a.V) {
+            left += fmax(p / sum - (double)fmaxf(y[i], 0.0f), 0.0);
         }
     }
     all = block_sum(all, lds);
@@ -323,20 +370,17 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
 
 // The next token: its chunk by the chunks' sums, then its place in the chunk.
 template <bool WIDE>
-__global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kSumThreads) void verify_pick_kernel(VerifyArgs a) {
     __shared__ uint32_t hit[kVChunk / 32];
-    __shared__ double scan[1024 / 64];
+    __shared__ double scan[kSumThreads / 64];
     __shared__ int pick, last;
     const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
     Walk w = a.walk[b];
     if (w.at < 0) return;
     const double* const all = a.sums + (int64_t)b * a.chunks;
     const double* left = all + (int64_t)a.B * a.chunks;
-    double sum = 0.0, whole = 0.0;
-    for (int j = 0; j < a.chunks; ++j) {
-        sum += all[j];
-        whole += left[j];
-    }
+    const double sum = ordered_sum(all, a.chunks);
+    double whole = ordered_sum(left, a.chunks);
     const uint8_t* row = a.logits + b * a.l_nb2 + w.at * a.l_nb1;
     const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
     if (!(whole > 0.0)) {  // nothing is left: the target's distribution
@@ -347,17 +391,21 @@ __global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
     }
     const float uf = a.uniform[(int64_t)b * (a.n_q + 1) + a.n_q];
     const double aim = (uf > 0.0f ? (double)uf : 0.0) * whole;
+    // the first chunk whose running sum exceeds the aim, else the last one with a mass
     int chunk = 0;
     double base = 0.0, run = 0.0;
     bool got = false;
-    for (int j = 0; j < a.chunks && !got; ++j) {
-        const double y = left[j];
-        if (y > 0.0) {
-            chunk = j;
-            base = run;
-            got = run + y > aim;
+    for (int j0 = 0; j0 < a.chunks && !got; j0 += 64) {
+        const double mine = j0 + lane < a.chunks ? left[j0 + lane] : 0.0;
+        for (int j = 0; j < min(64, a.chunks - j0) && !got; ++j) {
+            const double y = lane_f64(mine, j);
+            if (y > 0.0) {
+                chunk = j0 + j;
+                base = run;
+                got = run + y > aim;
+            }
+            run += y;
         }
-        run += y;
     }
     const int v0 = chunk * kVChunk;
     mark_kids(a, w, b, v0, hit);
@@ -365,12 +413,15 @@ __global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
         pick = 0x7fffffff;
         last = -1;
     }
-    constexpr int E = kVChunk / 1024;
+    constexpr int E = kSumEach;
+    float x[E], y[E];
+    eight<WIDE>(row, v0 + tid * E, a.V, x);
+    if (q) eight<WIDE>(q, v0 + tid * E, a.V, y);
     double r[E], mine = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const int v = v0 + tid * E + e;
-        r[e] = v < a.V ? left_over<WIDE>(a, w, element<WIDE>(row, v), q, v, sum, hit, v0) : 0.0;
+        const double p = weight_f64(x[e], w.max, w.cool);
+        r[e] = q ? (v0 + tid * E + e < a.V ? fmax(p / sum - (double)fmaxf(y[e], 0.0f), 0.0) : 0.0) : kept(hit, tid * E + e) ? p : 0.0;
         mine += r[e];
     }
     double upto = mine;
@@ -383,7 +434,7 @@ __global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
     __syncthreads();
     double at = base;
 #pragma unroll
-    for (int i = 0; i < 1024 / 64; ++i) at += i < wave_id() ? scan[i] : 0.0;
+    for (int i = 0; i < kSumThreads / 64; ++i) at += i < wave_id() ? scan[i] : 0.0;
     at += upto - mine;
     int found = 0x7fffffff, any = -1;
 #pragma unroll
@@ -402,7 +453,7 @@ __global__ __launch_bounds__(1024) void verify_pick_kernel(VerifyArgs a) {
         a.next[b] = v;
         if (a.logp) {
             const double x = v >= 0 ? (double)element<WIDE>(row, v) : -INFINITY;
-            a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((x == w.max ? 0.0 : (x - w.max) / w.heat) - log(sum));
+            a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((x == w.max ? 0.0 : (x - w.max) * w.cool) - log(sum));
         }
     }
 }
@@ -435,10 +486,10 @@ template <bool WIDE>
 static void verify_launch(const VerifyArgs& a, hipStream_t s) {
     launch("verify_stats", verify_stats_kernel<WIDE>, dim3((uint32_t)a.chunks, (uint32_t)a.n_q, (uint32_t)a.B), dim3(256), s, a);
     // (all greedy: the path and the maxima are the whole answer)
-    launch("verify_sums", verify_sums_kernel<WIDE, 0>, dim3(a.uniform ? (uint32_t)a.chunks : 1u, (uint32_t)a.B), dim3(256), s, a);
+    launch("verify_sums", verify_sums_kernel<WIDE, 0>, dim3(a.uniform ? (uint32_t)a.chunks : 1u, (uint32_t)a.B), dim3(kSumThreads), s, a);
     if (!a.uniform) return;
-    if (a.draft) launch("verify_left", verify_sums_kernel<WIDE, 1>, dim3((uint32_t)a.chunks, (uint32_t)a.B), dim3(256), s, a);
-    launch("verify_pick", verify_pick_kernel<WIDE>, dim3((uint32_t)a.B), dim3(1024), s, a);
+    if (a.draft) launch("verify_left", verify_sums_kernel<WIDE, 1>, dim3((uint32_t)a.chunks, (uint32_t)a.B), dim3(kSumThreads), s, a);
+    launch("verify_pick", verify_pick_kernel<WIDE>, dim3((uint32_t)a.B), dim3(kSumThreads), s, a);
 }
 
 }  // namespace xq
