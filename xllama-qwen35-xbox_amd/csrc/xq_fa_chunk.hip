@@ -16,6 +16,7 @@ struct FaChunkArgs : ChunkArgs {
     uint8_t* dst;
     int64_t d_nb1, d_nb2, d_nb3;  // head, token, sequence
     float* lse;
+    uint32_t target;              // above 0: parts dealt by the sequences' lengths, about so many
     int32_t ptiles, splits;       // pair tiles of a sequence with n_q tokens; parts of one
     uint32_t seg_shift, seg_more; // (sequence, KV head) segments: 2^seg_shift of them times seg_more
     UDivFlat d_more, d_splits, d_hkv, d_h, d_q;
@@ -28,7 +29,14 @@ constexpr float kOff = -7.0f;   // weights are 2^(x - reference + 7), in (0, 2^1
 constexpr float kHigh = 6.0f;   // beside f32 Q the reference stays this far below the maximum it was taken from,
                                 // so that a weight's two parts are off by 2^-37 of the largest, or 2^-22 of itself
 
-template <int KT, int D, bool NARROW, int MT, int NW>
+// To nearest, ties to even, by the two-value conversion.
+XQ_DEV uint2 bf16x4(f4t o) {
+    typedef __bf16 b4t __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_convertvector(o, b4t));
+}
+
+// A wave has 16 MT pairs and a WR-th of a tile's rows: WR waves share pairs where there are few.
+template <int KT, int D, bool NARROW, int MT, int WR, int NW>
 struct ChunkCfg {
     static constexpr bool QUANT = KT == XQ_TYPE_Q8_0 || KT == XQ_TYPE_Q4_0;
     static constexpr int PARTS = QUANT && !NARROW ? 2 : 1;  // f16 parts of a cached value
@@ -36,90 +44,172 @@ struct ChunkCfg {
     static constexpr int EL = KT == XQ_TYPE_F16 ? 8 : KT == XQ_TYPE_Q4_0 ? 32 : 16;  // elements of a 16-byte piece
     static constexpr int PPR = D / EL;                      // pieces per row
     static constexpr int TR = 64;                           // KV rows of a tile (a lane per row)
-    static constexpr int RT = 2;                            // 16-row score tiles of a wave at a time
+    static constexpr int RW = TR / WR;                      // of a wave
+    static constexpr int RT = RW >= 32 ? 2 : 1;             // 16-row score tiles of a wave at a time
     static constexpr int PIECES = TR * PPR;
     static constexpr int NPT = (PIECES + 64 * NW - 1) / (64 * NW);  // per thread
     static constexpr int RS = 2 * D + 32;                   // image rows, bytes: 8 banks of 64 apart
     static constexpr int PB = TR * RS;                      // one part of K or V
-    static constexpr int PW = 16 * MT * NW;                 // pairs of a workgroup
+    static constexpr int PW = 16 * MT * (NW / WR);          // pairs of a workgroup
+    static constexpr int IMG = 2 * PARTS * PB, MS = D + 4, MERGE = WR > 1 ? NW * 16 * MS * 4 : 0, SMEM = IMG > MERGE ? IMG : MERGE;  // (MS: floats of a merged row)
 };
 
-template <int KT, int D, bool NARROW, bool BIASED, int MT, int NW>
+// The workgroup's segment (sequence b, KV head hk), pair tile and part; false where there is none. A segment's
+// workgroups share an XCD (or 8 / 2^seg_shift of them): its rows stay in that L2. Late pair tiles, which see
+// the most, go first.
+XQ_DEV bool chunk_place(const FaChunkArgs& a, int& b, int& hk, int& pt, int& part) {
+    const uint32_t xcd = blockIdx.x & 7u, slot = blockIdx.x >> 3;
+    const uint32_t turn = a.d_more.quot(slot);
+    const uint32_t seg = (xcd & ((1u << a.seg_shift) - 1u)) + ((slot - turn * a.seg_more) << a.seg_shift);
+    const uint32_t order = (xcd >> a.seg_shift) + (turn << (3 - a.seg_shift));
+    const uint32_t po = a.d_splits.quot(order);
+    part = (int)(order - po * (uint32_t)a.splits), pt = a.ptiles - 1 - (int)po;
+    b = (int)a.d_hkv.quot(seg), hk = (int)seg - b * a.pg.n_head_kv;
+    return pt >= 0;
+}
+
+// One pair tile per segment (few tokens): the rows' tiles of all sequences are dealt out in parts of `per`, sequence after
+// sequence, so that a batch of all lengths has parts of one size. From the device's lengths, so a captured graph
+// follows them. (Equal numbers of parts per sequence: a decode of 16 chats of up to 6001 rows 37 us; dealt 31.)
+struct ChunkDeal {
+    uint32_t per;
+    int b0;
+    uint32_t tiles, parts, upto;  // of sequence b0 + lane; parts up to and with its
+    // the tiles that some token of sequence b may see: first one, number
+    static XQ_DEV uint32_t tiles_of(const FaChunkArgs& a, int b, uint32_t& first) {
+        int held, n_tok, end;
+        a.lengths(b, held, n_tok, end);
+        first = a.window ? (uint32_t)max(held + 1 - a.window, 0) / 64u : 0u;
+        return n_tok ? ((uint32_t)end + 63u) / 64u - min(first, ((uint32_t)end + 63u) / 64u) : 0u;
+    }
+    XQ_DEV void load(const FaChunkArgs& a, int first, uint32_t before) {
+        b0 = first;
+        uint32_t t0;
+        tiles = b0 + lane_id() < a.B ? tiles_of(a, b0 + lane_id(), t0) : 0u;
+        parts = b0 + lane_id() < a.B ? max((tiles + per - 1) / per, 1u) * (uint32_t)a.pg.n_head_kv : 0u;
+        upto = before + wave_scan(parts);
+    }
+    XQ_DEV explicit ChunkDeal(const FaChunkArgs& a) : per(1) {
+        uint64_t all = 0;
+        for (int b = 0; b < a.B; b += 64) {
+            load(a, b, 0);
+            all += lane_get(wave_scan(tiles), 63);
+        }
+        per = uniform((uint32_t)max((all * (uint32_t)a.pg.n_head_kv + a.target - 1) / a.target, (uint64_t)1));
+        load(a, 0, 0);
+    }
+    XQ_DEV uint32_t last() const { return lane_get(upto, 63); }
+};
+
+// Rows that some of several tokens see, and those that all do.
+struct Range {
+    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = 0;
+    XQ_DEV void of(int lo, int hi) {
+        if (lo < hi) {  // (what sees nothing asks for no tile)
+            lo_min = min(lo_min, lo);
+            hi_max = max(hi_max, hi);
+        }
+        lo_max = max(lo_max, lo);
+        hi_min = min(hi_min, hi);
+    }
+    XQ_DEV void with(const Range& o) {
+        lo_min = min(lo_min, o.lo_min), lo_max = max(lo_max, o.lo_max);
+        hi_min = min(hi_min, o.hi_min), hi_max = max(hi_max, o.hi_max);
+    }
+    XQ_DEV void wave() {  // over its lanes, in scalar registers
+#pragma unroll
+        for (int s = 1; s < 64; s *= 2) with(Range{__shfl_xor(lo_min, s), __shfl_xor(lo_max, s), __shfl_xor(hi_min, s), __shfl_xor(hi_max, s)});
+        lo_min = (int)uniform((uint32_t)lo_min), lo_max = (int)uniform((uint32_t)lo_max);
+        hi_min = (int)uniform((uint32_t)hi_min), hi_max = (int)uniform((uint32_t)hi_max);
+    }
+    template <int NW>
+    XQ_DEV Range group(int (*lds)[NW], int wave) const {  // over the workgroup's waves
+        if (lane_id() == 0) lds[0][wave] = lo_min, lds[1][wave] = lo_max, lds[2][wave] = hi_min, lds[3][wave] = hi_max;
+        __syncthreads();
+        Range r;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) r.with(Range{lds[0][i], lds[1][i], lds[2][i], lds[3][i]});
+        return r;
+    }
+};
+
+// The tiles of a workgroup's part of what its pairs see (below 2^25 tiles, up to 64 parts).
+template <int TR>
+XQ_DEV void chunk_tiles(const FaChunkArgs& a, const Range& r, int part, uint32_t& t_first, uint32_t& t_last) {
+    const uint32_t tile0 = r.lo_min < r.hi_max ? (uint32_t)r.lo_min / TR : 0u;
+    const uint32_t tiles = r.lo_min < r.hi_max ? ((uint32_t)r.hi_max + TR - 1) / TR - tile0 : 0u;
+    t_first = tile0 + uniform(a.d_splits.quot(tiles * (uint32_t)part));
+    t_last = part + 1 == a.splits ? tile0 + tiles : tile0 + uniform(a.d_splits.quot(tiles * (uint32_t)(part + 1)));
+}
+
+template <int KT, int D, bool NARROW, bool BIASED, int MT, int WR, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
-    using C = ChunkCfg<KT, D, NARROW, MT, NW>;
+    static_assert(MT == 1 || WR == 1);
+    using C = ChunkCfg<KT, D, NARROW, MT, WR, NW>;
     constexpr int PARTS = C::PARTS, QP = C::QP, NB = D / 32, ND = D / 16, NPT = C::NPT, PPR = C::PPR, PW = C::PW, TR = C::TR, RT = C::RT;
     constexpr bool QUANT = C::QUANT, BY_V = PARTS == 2;
     constexpr int KC = PARTS == 2 ? 2 : 4, VC = PARTS == 2 ? 2 : 4;  // K chunks, V columns read at once
-    __shared__ __attribute__((aligned(16))) uint8_t imgK[PARTS * C::PB], imgV[PARTS * C::PB];
+    __shared__ __attribute__((aligned(16))) uint8_t img[C::SMEM];
+    uint8_t* const imgK = img;
+    uint8_t* const imgV = img + PARTS * C::PB;
+    __shared__ float sM[WR > 1 ? NW : 1][16], sL[WR > 1 ? NW : 1][16];
     __shared__ __attribute__((aligned(16))) int sEk[PARTS == 2 ? TR : 4], sEv[PARTS == 2 ? TR : 4];
     __shared__ unsigned long long sBad[2];
     __shared__ int sRange[4][NW];
     const int lane = lane_id(), wave = wave_id(), tid = threadIdx.x, lr = lane & 15, lg = lane >> 4;
     const int r0 = tid / PPR, c0 = tid % PPR;  // row and piece of a tile that this thread brings
 
-    // ---- the workgroup's segment, pair tile and part. A segment's workgroups share an XCD (or
-    // 8 / 2^seg_shift of them): its rows stay in that L2. Late pair tiles, which see the most, go first.
-    const uint32_t xcd = blockIdx.x & 7u, slot = blockIdx.x >> 3;
-    const uint32_t turn = a.d_more.quot(slot);
-    const uint32_t seg = (xcd & ((1u << a.seg_shift) - 1u)) + ((slot - turn * a.seg_more) << a.seg_shift);
-    const uint32_t order = (xcd >> a.seg_shift) + (turn << (3 - a.seg_shift));
-    const uint32_t po = a.d_splits.quot(order);
-    const int part = (int)(order - po * (uint32_t)a.splits), pt = a.ptiles - 1 - (int)po;
-    if (pt < 0) return;
-    const int b = (int)a.d_hkv.quot(seg), hk = (int)seg - b * a.pg.n_head_kv;
+    int b, hk, pt = 0, part;
+    int n_parts = a.splits;
+    int64_t piece;
+    uint32_t dealt = 0;  // its tiles of a part, or 0
+    constexpr bool FEW = NW == 4;
+    if (FEW && a.target) {
+        ChunkDeal d(a);
+        while (blockIdx.x >= d.last() && d.b0 + 64 < a.B) d.load(a, d.b0 + 64, d.last());
+        if (blockIdx.x >= d.last()) return;
+        const int sl = __builtin_ctzll(__builtin_amdgcn_ballot_w64(blockIdx.x < d.upto));
+        const uint32_t mine = lane_get(d.parts, sl), in_b = blockIdx.x - (lane_get(d.upto, sl) - mine), of_head = mine / (uint32_t)a.pg.n_head_kv;
+        b = d.b0 + sl;
+        hk = (int)uniform(in_b / of_head), part = (int)(in_b - (uint32_t)hk * of_head);
+        n_parts = (int)of_head;
+        piece = blockIdx.x;
+        dealt = d.per;
+    } else {
+        if (!chunk_place(a, b, hk, pt, part)) return;
+        piece = ((int64_t)(b * a.pg.n_head_kv + hk) * a.ptiles + pt) * a.splits + part;
+    }
     int held, n_tok, end;
     a.lengths(b, held, n_tok, end);
     const int n_pairs = n_tok * a.G;
     if (pt * PW >= n_pairs) return;
-    const int p0 = pt * PW + wave * 16 * MT;  // this wave's first pair
+    const int wp = wave / WR, row_first = wave % WR * C::RW;  // the wave's pairs, and rows of a tile
+    const int p0 = pt * PW + wp * 16 * MT;
 
     int tok[MT], lo[MT], hi[MT], at[MT];
     float slope[MT];
-    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = 0;
+    Range wr;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int p = min(p0 + 16 * m + lr, n_pairs - 1);
         tok[m] = (int)a.d_g.quot((uint32_t)p);
         a.range(b, tok[m], held, end, at[m], lo[m], hi[m]);
         slope[m] = BIASED ? a.slope(hk * a.G + p - tok[m] * a.G) : 0.0f;
-        // (what sees nothing asks for no tile)
-        if (lo[m] < hi[m]) {
-            lo_min = min(lo_min, lo[m]);
-            hi_max = max(hi_max, hi[m]);
-        }
-        lo_max = max(lo_max, lo[m]);
-        hi_min = min(hi_min, hi[m]);
+        wr.of(lo[m], hi[m]);
     }
-#pragma unroll
-    for (int s = 1; s < 16; s *= 2) {
-        lo_min = min(lo_min, __shfl_xor(lo_min, s));
-        lo_max = max(lo_max, __shfl_xor(lo_max, s));
-        hi_min = min(hi_min, __shfl_xor(hi_min, s));
-        hi_max = max(hi_max, __shfl_xor(hi_max, s));
-    }
-    lo_min = (int)uniform((uint32_t)lo_min), lo_max = (int)uniform((uint32_t)lo_max);
-    hi_min = (int)uniform((uint32_t)hi_min), hi_max = (int)uniform((uint32_t)hi_max);
-    if (lane == 0) {
-        sRange[0][wave] = lo_min;
-        sRange[1][wave] = lo_max;
-        sRange[2][wave] = hi_min;
-        sRange[3][wave] = hi_max;
-    }
+    wr.wave();
     if (tid < 2) sBad[tid] = 0;
-    __syncthreads();
-    int wg_lo_min = sRange[0][0], wg_lo_max = sRange[1][0], wg_hi_min = sRange[2][0], wg_hi_max = sRange[3][0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) {
-        wg_lo_min = min(wg_lo_min, sRange[0][i]);
-        wg_lo_max = max(wg_lo_max, sRange[1][i]);
-        wg_hi_min = min(wg_hi_min, sRange[2][i]);
-        wg_hi_max = max(wg_hi_max, sRange[3][i]);
+    const Range wg = wr.group<NW>(sRange, wave);
+    uint32_t t_first, t_last;
+    if (FEW && dealt) {
+        uint32_t t0;
+        const uint32_t tiles = ChunkDeal::tiles_of(a, b, t0);
+        const bool any = wg.lo_min < wg.hi_max;
+        t_first = max(uniform(t0 + (uint32_t)part * dealt), any ? (uint32_t)wg.lo_min / TR : 0u);
+        t_last = any ? min(uniform(t0 + min((uint32_t)(part + 1) * dealt, tiles)), ((uint32_t)wg.hi_max + TR - 1) / TR) : t_first;
+    } else {
+        chunk_tiles<TR>(a, wg, part, t_first, t_last);
     }
-    const uint32_t tile0 = wg_lo_min < wg_hi_max ? (uint32_t)wg_lo_min / TR : 0u;
-    const uint32_t tiles = wg_lo_min < wg_hi_max ? ((uint32_t)wg_hi_max + TR - 1) / TR - tile0 : 0u;
-    // (tiles below 2^25, parts up to 64)
-    const uint32_t t_first = tile0 + uniform(a.d_splits.quot(tiles * (uint32_t)part));
-    const uint32_t t_last = part + 1 == a.splits ? tile0 + tiles : tile0 + uniform(a.d_splits.quot(tiles * (uint32_t)(part + 1)));
 
     const uint8_t* const kb = a.pg.k + hk * a.pg.k_head;
     const uint8_t* const vb = a.pg.v + hk * a.pg.v_head;
@@ -282,7 +372,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
     for (uint32_t t = t_first; t < t_last; ++t) {
         const int first = (int)(t * TR);
         __syncthreads();  // the image is free, the flags are zero
-        commit(t, first < wg_lo_max || first + TR > wg_hi_min);
+        commit(t, first < wg.lo_max || first + TR > wg.hi_min);
         __syncthreads();
         const uint64_t now = valid;
         if (t + 1 < t_last) {
@@ -291,18 +381,18 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
             lookup(t + 2, page, in);
         }
         if (tid == 0) sBad[(t + 1) & 1] = 0;
-        if (p0 >= n_pairs || first >= hi_max || first + TR <= lo_min) continue;  // (a wave without pairs that see the tile)
+        if (p0 >= n_pairs || first >= wr.hi_max || first + TR <= wr.lo_min) continue;  // (a wave without pairs that see the tile)
 
         // which of the tile's rows each pair sees
-        const bool careful = first < lo_max || first + TR > hi_min || now != ~0ull;
+        const bool careful = first < wr.lo_max || first + TR > wr.hi_min || now != ~0ull;
         uint64_t sees[MT];
         if (careful) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) sees[m] = tile_rows(first, lo[m], hi[m]) & now;
         }
 #pragma unroll 1
-        for (int sub = 0; sub < TR / (16 * RT); ++sub) {
-            const int row0 = 16 * RT * sub;
+        for (int sub = 0; sub < C::RW / (16 * RT); ++sub) {
+            const int row0 = row_first + 16 * RT * sub;
             f4t s[MT][RT];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -440,8 +530,11 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
             }
             // O^T += V^T P^T
             auto product = [&](const h4t (&x)[RT], const h4t (&p)[RT], f4t& o) {
-                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                                          __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4, 5, 6, 7), o, 0, 0, 0);
+                if constexpr (RT == 2)
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(x[0], x[RT - 1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                              __builtin_shufflevector(p[0], p[RT - 1], 0, 1, 2, 3, 4, 5, 6, 7), o, 0, 0, 0);
+                else
+                    o = __builtin_amdgcn_mfma_f32_16x16x16f16(x[0], p[0], o, 0, 0, 0);
             };
 #pragma unroll
             for (int n0 = 0; n0 < ND; n0 += VC) {
@@ -462,6 +555,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
         // non-finite values of rows that not every pair sees: to the pairs that do
         if (careful) {
             uint64_t bad = sBad[t & 1];
+            if constexpr (WR > 1) bad &= (~0ull >> (64 - C::RW)) << row_first;
             bad = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(bad >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)bad);
             while (bad) {
                 const int r = __builtin_ctzll(bad);
@@ -487,92 +581,152 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
     }
 
     // ---- the pairs' results, or this workgroup's part of them
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int p = p0 + 16 * m + lr;
-        const float l = across_rows_sum(l_run[m]);
-        if (p >= n_pairs) continue;
-        if (a.splits > 1) {
-            const int64_t y = (((int64_t)seg * a.ptiles + pt) * a.splits + part) * PW + (p - pt * PW);
-#pragma unroll
-            for (int n = 0; n < ND; ++n) *(f4t*)(a.part_o + y * D + 16 * n + 4 * lg) = acc[m][n];
-            if (lg == 0) a.part_ml[y] = make_float2(m_run[m], l);
-            continue;
+    auto emit = [&](int p, int d, f4t o, float mm, float l, bool first) {  // pair p, dims d..d+3
+        const int tk = (int)a.d_g.quot((uint32_t)p), h = hk * a.G + p - tk * a.G;
+        if (n_parts > 1) {
+            const int64_t y = piece * PW + (p - pt * PW);
+            *(f4t*)(a.part_o + y * D + d) = o;
+            if (first) a.part_ml[y] = make_float2(mm, l);
+            return;
         }
-        const int h = hk * a.G + p - tok[m] * a.G;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint8_t* y = a.dst + b * a.d_nb3 + tok[m] * a.d_nb2 + h * a.d_nb1;
+        o *= l == 0.0f ? 0.0f : 1.0f / l;
+        uint8_t* y = a.dst + b * a.d_nb3 + tk * a.d_nb2 + h * a.d_nb1;
+        if constexpr (NARROW) *(uint2*)(y + 2 * d) = bf16x4(o);
+        else *(f4t*)(y + 4 * d) = o;
+        if (first && a.lse) a.lse[((int64_t)b * a.n_q + tk) * a.H + h] = l == 0.0f ? -INFINITY : (mm + kOff) * kLn2 + logf(l);
+    };
 #pragma unroll
-        for (int n = 0; n < ND; ++n) {
-            const f4t o = acc[m][n] * inv;
-            if constexpr (NARROW)
-                *(uint2*)(y + 2 * (16 * n + 4 * lg)) = make_uint2(f32_to_bf16_bits(o[0]) | (f32_to_bf16_bits(o[1]) << 16), f32_to_bf16_bits(o[2]) | (f32_to_bf16_bits(o[3]) << 16));
-            else
-                *(f4t*)(y + 4 * (16 * n + 4 * lg)) = o;
+    for (int m = 0; m < MT; ++m) l_run[m] = across_rows_sum(l_run[m]);
+    if constexpr (WR > 1) {
+        if (lg == 0) {
+            sM[wave][lr] = m_run[0];
+            sL[wave][lr] = l_run[0];
         }
-        if (a.lse && lg == 0) a.lse[((int64_t)b * a.n_q + tok[m]) * a.H + h] = l == 0.0f ? -INFINITY : (m_run[m] + kOff) * kLn2 + logf(l);
+        __syncthreads();  // the last tile is read, the states are there
+        float* const mg = (float*)img;
+        // the waves of a pair group bring their sums to their largest reference
+        auto largest = [&](int w0, int q) {
+            float x = sM[w0][q];
+#pragma unroll
+            for (int i = 1; i < WR; ++i) x = fmaxf(x, sM[w0 + i][q]);
+            return x;
+        };
+        const float f = m_run[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[0] - largest(wp * WR, lr));
+#pragma unroll
+        for (int n = 0; n < ND; ++n) *(f4t*)(mg + (16 * wave + lr) * C::MS + 16 * n + 4 * lg) = acc[0][n] * f;
+        __syncthreads();
+        for (int i = tid; i < PW * D / 4; i += 64 * NW) {
+            const int q = i / (D / 4), d = 4 * (i % (D / 4)), w0 = q / 16 * WR;
+            if (pt * PW + q >= n_pairs) continue;
+            const float mm = largest(w0, q % 16);
+            float l = 0.0f;
+            f4t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int x = w0; x < w0 + WR; ++x) {
+                // (a wave without a reference: its sum is 0, or NaN by a NaN score)
+                l = fmaf(sL[x][q % 16], sM[x][q % 16] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[x][q % 16] - mm), l);
+                o += *(const f4t*)(mg + (16 * x + q % 16) * C::MS + d);
+            }
+            emit(pt * PW + q, d, o, mm, l, d == 0);
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (p0 + 16 * m + lr >= n_pairs) continue;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) emit(p0 + 16 * m + lr, 16 * n + 4 * lg, acc[m][n], m_run[m], l_run[m], n == 0 && lg == 0);
+        }
     }
 }
 
-// Joins the parts of each (sequence, token, head): a wave per row, D / 4 lanes a part.
-template <int D, bool NARROW>
+// Joins the parts of each row (sequence, token, head). NWR waves a row: D / 4 lanes read a part's dims, NG parts at a time and
+// four of those in flight, each group of lanes with a running reference of its own.
+template <int D, bool NARROW, int NWR>
 __global__ __launch_bounds__(256) void fa_chunk_join(FaChunkArgs a, uint32_t rows, int32_t PW) {
-    constexpr int L = D / 4, NG = 64 / L;
-    const uint32_t row = uniform(blockIdx.x * 4 + threadIdx.x / 64);
-    if (row >= rows) return;
-    const uint32_t bt = a.d_h.quot(row), h = row - bt * (uint32_t)a.H;
+    constexpr int L = D / 4, NG = 64 * NWR / L, UN = 4, RB = 4 / NWR;
+    __shared__ __attribute__((aligned(16))) float sO[RB][NG][D], sM[RB][NG], sL[RB][NG];
+    const int rb = RB == 1 ? 0 : wave_id(), tid = threadIdx.x % (64 * NWR);
+    const uint32_t row = uniform(blockIdx.x * RB + rb);
+    const bool real = row < rows;
+    const uint32_t bt = a.d_h.quot(real ? row : 0u), h = (real ? row : 0u) - bt * (uint32_t)a.H;
     const uint32_t b = a.d_q.quot(bt), t = bt - b * (uint32_t)a.n_q;
     int held, n_tok, end;
     a.lengths((int)b, held, n_tok, end);
-    if ((int)t >= n_tok) return;
     const uint32_t hk = a.d_g.quot(h), pair = t * (uint32_t)a.G + h - hk * (uint32_t)a.G, pt = pair / (uint32_t)PW;
-    const int64_t y0 = (((int64_t)(b * a.pg.n_head_kv + hk) * a.ptiles + pt) * a.splits) * PW + (pair - pt * PW);
-    const int lane = lane_id(), g = lane / L, d = 4 * (lane % L);
+    int n_parts = a.splits;
+    int64_t piece = ((int64_t)(b * a.pg.n_head_kv + hk) * a.ptiles + pt) * a.splits;
+    if (a.target) {
+        ChunkDeal deal(a);
+        while ((uint32_t)deal.b0 + 64 <= b) deal.load(a, deal.b0 + 64, deal.last());
+        const int sl = (int)b - deal.b0;
+        const uint32_t mine = lane_get(deal.parts, sl);
+        n_parts = (int)(mine / (uint32_t)a.pg.n_head_kv);
+        piece = (int64_t)(lane_get(deal.upto, sl) - mine) + hk * n_parts;
+    }
+    const bool on = real && (int)t < n_tok && n_parts > 1;  // (one part: its workgroup has written the row)
+    const int64_t y0 = piece * PW + (pair - pt * PW);
+    const int g = tid / L, d = 4 * (tid % L);
     f4t o = {0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    for (int s = g; s < a.splits; s += NG) {
-        const float2 ml = a.part_ml[y0 + (int64_t)s * PW];
-        const f4t v = *(const f4t*)(a.part_o + (y0 + (int64_t)s * PW) * D + d);
-        const float top = fmaxf(m, ml.x);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top), w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        l = fmaf(ml.y, w, l * f);
+    for (int s0 = g; on && s0 < n_parts; s0 += NG * UN) {
+        f4t y[UN];
+        float2 ml[UN];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], w, o[e] * f);
-        m = top;
-    }
-    if constexpr (NG == 2) {  // the other half of the wave has the other parts
-        const float om = __shfl_xor(m, 32), ol = __shfl_xor(l, 32);
-        const float top = fmaxf(m, om);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top), w = om == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(om - top);
-        l = l * f + ol * w;
+        for (int i = 0; i < UN; ++i) {
+            const int64_t at = y0 + (int64_t)min(s0 + NG * i, n_parts - 1) * PW;
+            ml[i] = a.part_ml[at];
+            y[i] = *(const f4t*)(a.part_o + at * D + d);
+            if (s0 + NG * i >= n_parts) {  // not a part: no weight, and nothing that a product could make NaN
+                ml[i] = make_float2(-INFINITY, 0.0f);
+                y[i] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+        float top = m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = o[e] * f + __shfl_xor(o[e], 32) * w;
+        for (int i = 0; i < UN; ++i) top = fmaxf(top, ml[i].x);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        o *= f;
+        l *= f;
         m = top;
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const float w = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - top);
+            l = fmaf(ml[i].y, w, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(y[i][e], w, o[e]);
+        }
     }
-    if (g) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *(f4t*)&sO[rb][g][d] = o;
+    if (d == 0) {
+        sM[rb][g] = m;
+        sL[rb][g] = l;
+    }
+    __syncthreads();
+    if (!on || g) return;
+    float top = sM[rb][0], sum = 0.0f;
+#pragma unroll
+    for (int i = 1; i < NG; ++i) top = fmaxf(top, sM[rb][i]);
+    o = f4t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const float w = sM[rb][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[rb][i] - top);
+        sum = fmaf(sL[rb][i], w, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(sO[rb][i][d + e], w, o[e]);
+    }
+    o *= sum == 0.0f ? 0.0f : 1.0f / sum;
     uint8_t* y = a.dst + b * a.d_nb3 + t * a.d_nb2 + h * a.d_nb1;
-    o *= inv;
-    if constexpr (NARROW)
-        *(uint2*)(y + 2 * d) = make_uint2(f32_to_bf16_bits(o[0]) | (f32_to_bf16_bits(o[1]) << 16), f32_to_bf16_bits(o[2]) | (f32_to_bf16_bits(o[3]) << 16));
-    else
-        *(f4t*)(y + 4 * d) = o;
-    if (a.lse && d == 0) a.lse[(int64_t)bt * a.H + h] = l == 0.0f ? -INFINITY : (m + kOff) * kLn2 + logf(l);
+    if constexpr (NARROW) *(uint2*)(y + 2 * d) = bf16x4(o);
+    else *(f4t*)(y + 4 * d) = o;
+    if (a.lse && d == 0) a.lse[(int64_t)bt * a.H + h] = sum == 0.0f ? -INFINITY : (top + kOff) * kLn2 + logf(sum);
 }
 
 // ---------------------------------------------------------------- host
 
-template <int MT_, int NW_> struct ChunkForm { static constexpr int MT = MT_, NW = NW_; };
-
-// f(KT, D, NARROW, BIASED, form) of the call
+// f(KT, D, NARROW, BIASED) of the call
 template <typename F>
-static void chunk_variant(int kt, int64_t D, bool narrow, bool biased, bool large, F f) {
-    auto with = [&](auto k, auto d, auto n, auto bi) {
-        constexpr int DD = decltype(d)::value;
-        if (large) f(k, d, n, bi, ChunkForm<DD == 128 ? 2 : 1, 8>{});
-        else f(k, d, n, bi, ChunkForm<1, 4>{});
-    };
-    auto bias = [&](auto k, auto d, auto n) { biased ? with(k, d, n, std::true_type{}) : with(k, d, n, std::false_type{}); };
+static void chunk_variant(int kt, int64_t D, bool narrow, bool biased, F f) {
+    auto bias = [&](auto k, auto d, auto n) { biased ? f(k, d, n, std::true_type{}) : f(k, d, n, std::false_type{}); };
     auto width = [&](auto k, auto d) { narrow ? bias(k, d, std::true_type{}) : bias(k, d, std::false_type{}); };
     auto dim = [&](auto k) { D == 128 ? width(k, std::integral_constant<int, 128>{}) : width(k, std::integral_constant<int, 256>{}); };
     switch (kt) {
@@ -586,29 +740,39 @@ static void chunk_variant(int kt, int64_t D, bool narrow, bool biased, bool larg
 // The form, parts and workspace of a call: of its shapes alone.
 struct ChunkPlan {
     bool large;
-    int32_t pw, ptiles, splits;
-    uint32_t seg_shift, seg_more;
+    int32_t form, pw, ptiles, splits;
+    uint32_t seg_shift, seg_more, target;
     int64_t wgs;
     size_t ml_at, bytes;
 };
 static ChunkPlan chunk_plan(const xq_tensor* q, const xq_kv_pages* c) {
     ChunkPlan P{};
     const int64_t D = q->ne[0], Hkv = c->k.ne[2], B = q->ne[3], pairs = q->ne[1] * (q->ne[2] / Hkv);
-    P.large = pairs > 64;
-    P.pw = !P.large ? 64 : D == 128 ? 256 : 128;
+    P.form = pairs <= 16 ? 0 : pairs <= 32 ? 1 : pairs <= 64 ? 2 : 3;
+    P.large = P.form == 3;
+    P.pw = P.form < 3 ? 16 << P.form : D == 128 ? 256 : 128;
     P.ptiles = (int32_t)cdiv(pairs, P.pw);
     const int64_t segs = B * Hkv, base = segs * P.ptiles;
     int64_t limit = (int64_t)c->table_cols * c->k.ne[1];
-    int64_t splits = cdiv(P.large ? 512 : 1024, base);
-    const int64_t most = cdiv(limit, 256);
-    if (splits > most) splits = most;
+    // A part costs its workgroup a start and a state written (131 KB of 256 pairs of 128): one part for each CU (512 tokens on
+    // 4096 rows: 68 us, with two 81), of a tile at least.
+    const int64_t tiles = cdiv(limit, 64);
+    int64_t splits = cdiv(256, base);
+    if (splits > tiles) splits = tiles;
     if (splits > 64) splits = 64;
     P.splits = (int32_t)(splits < 1 ? 1 : splits);
+    if (P.form < 3) {
+        // two workgroups for each CU; one of 140 KB of LDS (f32 beside quantized rows of 256)
+        const bool big = D == 256 && q->type == XQ_TYPE_F32 && (c->k.type == XQ_TYPE_Q8_0 || c->k.type == XQ_TYPE_Q4_0);
+        const int64_t target = big ? 256 : 512;
+        if (tiles > 1 && segs < 2 * target) P.target = (uint32_t)target;
+    }
     P.seg_shift = segs % 8 == 0 ? 3 : segs % 4 == 0 ? 2 : segs % 2 == 0 ? 1 : 0;
     P.seg_more = (uint32_t)(segs >> P.seg_shift);
     P.wgs = 8 * (int64_t)P.seg_more * cdiv((int64_t)P.ptiles * P.splits, 8 >> P.seg_shift);
-    if (P.splits > 1) {
-        const size_t rows = (size_t)base * P.splits * P.pw;
+    if (P.target) P.wgs = P.target + segs;
+    if (P.splits > 1 || P.target) {
+        const size_t rows = (size_t)(P.target ? P.wgs : base * P.splits) * P.pw;
         P.ml_at = rows * D * 4;
         P.bytes = P.ml_at + rows * 8;
     }
@@ -666,21 +830,27 @@ xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chu
     a.dst = (uint8_t*)dst->data;
     a.d_nb1 = (int64_t)dst->nb[1], a.d_nb2 = (int64_t)dst->nb[2], a.d_nb3 = (int64_t)dst->nb[3];
     a.lse = lse;
-    a.ptiles = P.ptiles, a.splits = P.splits;
+    a.ptiles = P.ptiles, a.splits = P.splits, a.target = P.target;
     a.seg_shift = P.seg_shift, a.seg_more = P.seg_more;
     a.d_more = UDivFlat(P.seg_more), a.d_splits = UDivFlat((uint32_t)P.splits), a.d_hkv = UDivFlat((uint32_t)a.pg.n_head_kv);
     a.d_h = UDivFlat((uint32_t)a.H), a.d_q = UDivFlat((uint32_t)a.n_q);
     a.part_o = (float*)workspace, a.part_ml = (float2*)((uint8_t*)workspace + P.ml_at);
     const bool biased = a.cap > 0.0f || a.max_bias > 0.0f;
     hipStream_t s = (hipStream_t)stream;
-    chunk_variant(cache->k.type, q->ne[0], q->type == XQ_TYPE_BF16, biased, P.large, [&](auto k, auto d, auto nar, auto bi, auto fm) {
-        using F = decltype(fm);
-        constexpr int D = decltype(d)::value;
-        constexpr bool NARROW = decltype(nar)::value;
-        launch("fa_chunk", fa_chunk_kernel<decltype(k)::value, D, NARROW, decltype(bi)::value, F::MT, F::NW>, dim3((uint32_t)P.wgs), dim3(64 * F::NW), s, a);
-        if (P.splits > 1) {
+    chunk_variant(cache->k.type, q->ne[0], q->type == XQ_TYPE_BF16, biased, [&](auto k, auto d, auto nar, auto bi) {
+        constexpr int KT = decltype(k)::value, D = decltype(d)::value;
+        constexpr bool NARROW = decltype(nar)::value, BIASED = decltype(bi)::value;
+        const dim3 grid((uint32_t)P.wgs);
+        switch (P.form) {
+        case 0: launch("fa_chunk", fa_chunk_kernel<KT, D, NARROW, BIASED, 1, 4, 4>, grid, dim3(256), s, a); break;
+        case 1: launch("fa_chunk", fa_chunk_kernel<KT, D, NARROW, BIASED, 1, 2, 4>, grid, dim3(256), s, a); break;
+        case 2: launch("fa_chunk", fa_chunk_kernel<KT, D, NARROW, BIASED, 1, 1, 4>, grid, dim3(256), s, a); break;
+        default: launch("fa_chunk", fa_chunk_kernel<KT, D, NARROW, BIASED, D == 128 ? 2 : 1, 1, 8>, grid, dim3(512), s, a); break;
+        }
+        if (P.splits > 1 || P.target) {
             const uint32_t rows = (uint32_t)((int64_t)a.B * a.n_q * a.H);
-            launch("fa_chunk_join", fa_chunk_join<D, NARROW>, dim3((rows + 3) / 4), dim3(256), s, a, rows, P.pw);
+            if (rows <= 2048) launch("fa_chunk_join", fa_chunk_join<D, NARROW, 4>, dim3(rows), dim3(256), s, a, rows, P.pw);
+            else launch("fa_chunk_join", fa_chunk_join<D, NARROW, 1>, dim3((rows + 3) / 4), dim3(256), s, a, rows, P.pw);
         }
     });
     const hipError_t e = hipGetLastError();

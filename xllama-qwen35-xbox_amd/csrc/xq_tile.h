@@ -108,4 +108,19 @@ XQ_DEV void products_done() {
 // A number that every lane has, in a scalar register: what is formed from it stays scalar.
 XQ_DEV uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
+// Inclusive sum over the 64 lanes: inside rows of 16, then from row to row.
+template <int CTRL, int ROWS>
+XQ_DEV uint32_t dpp_add(uint32_t x) {
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+XQ_DEV uint32_t wave_scan(uint32_t x) {
+    x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3
+    return dpp_add<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
+}
+XQ_DEV uint32_t lane_get(uint32_t x, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)x, l); }
+
 }  // namespace xq
