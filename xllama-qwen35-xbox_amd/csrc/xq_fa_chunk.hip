@@ -18,8 +18,8 @@ struct FaChunkArgs : ChunkArgs {
     float* lse;
     uint32_t target;              // above 0: parts dealt by the sequences' lengths, about so many
     int32_t ptiles, splits;       // pair tiles of a sequence with n_q tokens; parts of one
-    uint32_t seg_shift, seg_more; // (sequence, KV head) segments: 2^seg_shift of them times seg_more
-    UDivFlat d_more, d_splits, d_hkv, d_h, d_q;
+    uint32_t head_shift;          // 2^head_shift KV heads side by side on the XCDs
+    UDivFlat d_seq, d_more, d_splits, d_h, d_q;  // by a sequence's workgroups (of an XCD); by the heads one after another; ...
     float* part_o;                // [segment][pair tile][split][PW][D]
     float2* part_ml;              // [segment][pair tile][split][PW] reference, sum
 };
@@ -54,17 +54,19 @@ struct ChunkCfg {
     static constexpr int IMG = 2 * PARTS * PB, MS = D + 4, MERGE = WR > 1 ? NW * 16 * MS * 4 : 0, SMEM = IMG > MERGE ? IMG : MERGE;  // (MS: floats of a merged row)
 };
 
-// The workgroup's segment (sequence b, KV head hk), pair tile and part; false where there is none. A segment's
-// workgroups share an XCD (or 8 / 2^seg_shift of them): its rows stay in that L2. Late pair tiles, which see
-// the most, go first.
+// The workgroup's sequence, KV head, pair tile and part; false where there is none. Workgroups go out in order of their
+// numbers, to the eight XCDs in turn: those of one sequence after another, late pair tiles first, which see the most,
+// the heads (and, for fewer than eight, neighbouring pair tiles) over the XCDs. So those that run at one time cost
+// about the same and a head's rows stay in an XCD's L2. (Sequences over the XCDs instead, eight prompts of up to 777 tokens
+// with 78 to 3001 rows before them: 233 us for 129. Two prompts of 8191 tokens are 3 % the slower for it.)
 XQ_DEV bool chunk_place(const FaChunkArgs& a, int& b, int& hk, int& pt, int& part) {
     const uint32_t xcd = blockIdx.x & 7u, slot = blockIdx.x >> 3;
-    const uint32_t turn = a.d_more.quot(slot);
-    const uint32_t seg = (xcd & ((1u << a.seg_shift) - 1u)) + ((slot - turn * a.seg_more) << a.seg_shift);
-    const uint32_t order = (xcd >> a.seg_shift) + (turn << (3 - a.seg_shift));
+    b = (int)a.d_seq.quot(slot);
+    const uint32_t in_b = slot - (uint32_t)b * a.d_seq.d, turn = a.d_more.quot(in_b);
+    hk = (int)((xcd & ((1u << a.head_shift) - 1u)) + ((in_b - turn * a.d_more.d) << a.head_shift));
+    const uint32_t order = (xcd >> a.head_shift) + (turn << (3 - a.head_shift));
     const uint32_t po = a.d_splits.quot(order);
     part = (int)(order - po * (uint32_t)a.splits), pt = a.ptiles - 1 - (int)po;
-    b = (int)a.d_hkv.quot(seg), hk = (int)seg - b * a.pg.n_head_kv;
     return pt >= 0;
 }
 
@@ -741,8 +743,8 @@ static void chunk_variant(int kt, int64_t D, bool narrow, bool biased, F f) {
 struct ChunkPlan {
     bool large;
     int32_t form, pw, ptiles, splits;
-    uint32_t seg_shift, seg_more, target;
-    int64_t wgs;
+    uint32_t head_shift, target;
+    int64_t more, per_seq, wgs;
     size_t ml_at, bytes;
 };
 static ChunkPlan chunk_plan(const xq_tensor* q, const xq_kv_pages* c) {
@@ -767,9 +769,10 @@ static ChunkPlan chunk_plan(const xq_tensor* q, const xq_kv_pages* c) {
         const int64_t target = big ? 256 : 512;
         if (tiles > 1 && segs < 2 * target) P.target = (uint32_t)target;
     }
-    P.seg_shift = segs % 8 == 0 ? 3 : segs % 4 == 0 ? 2 : segs % 2 == 0 ? 1 : 0;
-    P.seg_more = (uint32_t)(segs >> P.seg_shift);
-    P.wgs = 8 * (int64_t)P.seg_more * cdiv((int64_t)P.ptiles * P.splits, 8 >> P.seg_shift);
+    P.head_shift = Hkv % 8 == 0 ? 3 : Hkv % 4 == 0 ? 2 : Hkv % 2 == 0 ? 1 : 0;
+    P.more = Hkv >> P.head_shift;
+    P.per_seq = P.more * cdiv((int64_t)P.ptiles * P.splits, 8 >> P.head_shift);
+    P.wgs = 8 * B * P.per_seq;
     if (P.target) P.wgs = P.target + segs;
     if (P.splits > 1 || P.target) {
         const size_t rows = (size_t)(P.target ? P.wgs : base * P.splits) * P.pw;
@@ -831,8 +834,8 @@ xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chu
     a.d_nb1 = (int64_t)dst->nb[1], a.d_nb2 = (int64_t)dst->nb[2], a.d_nb3 = (int64_t)dst->nb[3];
     a.lse = lse;
     a.ptiles = P.ptiles, a.splits = P.splits, a.target = P.target;
-    a.seg_shift = P.seg_shift, a.seg_more = P.seg_more;
-    a.d_more = UDivFlat(P.seg_more), a.d_splits = UDivFlat((uint32_t)P.splits), a.d_hkv = UDivFlat((uint32_t)a.pg.n_head_kv);
+    a.head_shift = P.head_shift;
+    a.d_seq = UDivFlat((uint32_t)P.per_seq), a.d_more = UDivFlat((uint32_t)P.more), a.d_splits = UDivFlat((uint32_t)P.splits);
     a.d_h = UDivFlat((uint32_t)a.H), a.d_q = UDivFlat((uint32_t)a.n_q);
     a.part_o = (float*)workspace, a.part_ml = (float2*)((uint8_t*)workspace + P.ml_at);
     const bool biased = a.cap > 0.0f || a.max_bias > 0.0f;
