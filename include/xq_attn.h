@@ -475,9 +475,10 @@ typedef struct xq_chunk_params {
  *           are left as they were
  *   dst     q's type [D, n_head, n_q, n_seq], strides multiples of 16 bytes; not q's memory
  *   lse     F32 [n_seq][n_q][n_head], natural logarithm of the softmax sum, or NULL
- * A token that sees no row gets O = 0, LSE = -inf. Fewer than 2^25 query rows (n_q * n_head * n_seq) and
- * 2^22 workgroups (of at least 64 of a KV head's n_q * group rows); row and page strides of the pools below 2^32 bytes. Roundings and non-finite values are
- * xq_fa_tree's. The workspace may be of 0 bytes; calls that may run at the same time need one each. */
+ * A token that sees no row gets O = 0, LSE = -inf. Roundings and non-finite values are xq_fa_tree's.
+ * Refused: 2^25 query rows (n_q * n_head * n_seq) or 2^22 workgroups and more, row and page strides of the
+ * pools of 2^32 bytes and more. The workspace may be of 0 bytes; calls that may run at the same time need one
+ * each. */
 int xq_supports_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst);
 xq_status xq_fa_chunk_workspace(const xq_tensor* q, const xq_kv_pages* cache, const xq_tensor* dst, size_t* bytes);
 xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chunk_params* params, const int32_t* first,
@@ -495,7 +496,8 @@ xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chu
  *   lse     F32 [n_seq][n_q][n_head] (device), of xq_fa_chunk or xq_fa_tree; -inf: a token without weight
  *   scores  F32 [n_seq][score_cols] (device), or NULL: zeros; scores_out the same, and may be scores
  * Scores are those of the decoded cache at 22 bits and more whatever q's type, sums in f32, in an order
- * that depends on the shapes alone. decay finite. A table of fewer than 2^28 rows; the workspace may be of 0 bytes. */
+ * that depends on the shapes and n_tok alone. decay finite. A table of fewer than 2^28 rows; the workspace may
+ * be of 0 bytes. */
 xq_status xq_kv_weights_workspace(const xq_tensor* q, const xq_kv_pages* cache, size_t* bytes);
 xq_status xq_kv_weights(const xq_tensor* q, const xq_kv_pages* cache, const xq_chunk_params* params, const int32_t* first,
                         const int32_t* prefix, const int32_t* n_tok, const float* lse, const float* scores, float* scores_out,

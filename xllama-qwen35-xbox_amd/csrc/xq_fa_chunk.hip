@@ -5,7 +5,17 @@
 // [lo, hi) (ChunkArgs::range): with x = log2(e) (f(scale q.k) + slope (r - its row)) over them, f the
 // identity or cap tanh(./cap), and any m near their maximum,
 //   O = sum_r 2^(x_r - m) v_r / sum_r 2^(x_r - m),    lse = (m + log2 sum) / log2(e).
-// A workgroup takes PW pairs and walks the 64-row tiles that any of them sees, once.
+// A workgroup takes PW pairs and walks the 64-row tiles that any of them sees, once: K and V as f16 images in LDS,
+// S = K Q^T and O^T = V^T P^T on the matrix cores, so that a lane's four scores are four rows of one pair and become
+// the second product's operand where they stand. Beside f32 Q, Q and the weights are two f16 parts, and so are
+// quantized values (exact integers times a scale's upper bits, and the remainder).
+//
+// What bounds it. Chunks: matrix products and vector issue, which overlap little: two prompts of 8191 bf16 tokens, f16 rows
+// of 128, 1.1 TFLOP: 1280 us, 0.86 PFLOP/s of the 1.22 of a large library product; the matrix cores are busy 38 % of
+// the time and vector issue 49 %. Without any staging or barrier it would be 1003 us, so a second image buys
+// little (32x32x16 products, two images and the stages interleaved by hand: 1187 us for 1185 of the 16x16x32
+// form as it then was). Few tokens: the rows' bytes where there are many (32 chats of up to 8000 fp8 rows 39 us, 28 at
+// 5.0 TB/s); else the two launches and a workgroup's chain of reads (lengths, table, rows, 20 us in all).
 #include <type_traits>
 
 #include "xq_chunk.h"
@@ -741,7 +751,6 @@ static void chunk_variant(int kt, int64_t D, bool narrow, bool biased, F f) {
 
 // The form, parts and workspace of a call: of its shapes alone.
 struct ChunkPlan {
-    bool large;
     int32_t form, pw, ptiles, splits;
     uint32_t head_shift, target;
     int64_t more, per_seq, wgs;
@@ -750,8 +759,10 @@ struct ChunkPlan {
 static ChunkPlan chunk_plan(const xq_tensor* q, const xq_kv_pages* c) {
     ChunkPlan P{};
     const int64_t D = q->ne[0], Hkv = c->k.ne[2], B = q->ne[3], pairs = q->ne[1] * (q->ne[2] / Hkv);
+    // As many waves share a tile's rows as the pairs leave without: all four waves on one pair group's 16 rows each
+    // (decode of 16 chats of fp8 rows 37 us, with three waves idle 45), up to 64 pairs a wave for each 16; above, eight waves
+    // with all pairs that the registers hold (32 each of D 128, 16 of 256), for a tile staged is then used most.
     P.form = pairs <= 16 ? 0 : pairs <= 32 ? 1 : pairs <= 64 ? 2 : 3;
-    P.large = P.form == 3;
     P.pw = P.form < 3 ? 16 << P.form : D == 128 ? 256 : 128;
     P.ptiles = (int32_t)cdiv(pairs, P.pw);
     const int64_t segs = B * Hkv, base = segs * P.ptiles;

@@ -12,6 +12,11 @@
 // the path by ballots and pointer doubling, a lane a token. Only the next token needs sums that hold
 // next to a border: those of one row per sequence, in f64 throughout. A row's sum over the tests is of
 // f32 exponentials (each off by 2^-22 of itself, the sum by less) joined in f64.
+//
+// What bounds it: the one pass over the logits (16 x 16 rows of 128000 f32, 131 MB: 24 us, 5.5 TB/s, some of it from the
+// Infinity Cache), then two launches of one row per sequence, 12 and 16 us, each a chain of dependent reads
+// (statistics, path, row) before f64 arithmetic on one or a few CUs. Loops in place of unrolled f64 code, a third of
+// its size, did not change that; a sum of the drawn row in the first launch would form all rows' f64 sums.
 #include "xq_tile.h"
 
 namespace xq {
@@ -204,13 +209,26 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     int arg = -1;
     if (live) {
         const RowStat* r = a.stats + ((int64_t)b * a.n_q + c) * a.chunks;
-        for (int j = 0; j < a.chunks; ++j) top = fmaxf(top, r[j].max);
-        if (top > -INFINITY)
-            for (int j = 0; j < a.chunks; ++j) {
-                const RowStat s = r[j];
-                whole += (double)s.sum * (double)weight_f32(s.max, top, f);
-                if (arg < 0 && s.max == top) arg = s.arg;
+        // (eight chunks in flight at a time: 16 sequences of 19 chunks 11.6 us, one after another 12.5)
+        constexpr int UN = 8;
+        for (int j = 0; j < a.chunks; j += UN) {
+            float x[UN];
+#pragma unroll
+            for (int i = 0; i < UN; ++i) x[i] = r[min(j + i, a.chunks - 1)].max;
+#pragma unroll
+            for (int i = 0; i < UN; ++i) top = fmaxf(top, x[i]);
+        }
+        for (int j = 0; j < a.chunks && top > -INFINITY; j += UN) {
+            RowStat x[UN];
+#pragma unroll
+            for (int i = 0; i < UN; ++i) x[i] = r[min(j + i, a.chunks - 1)];
+#pragma unroll
+            for (int i = 0; i < UN; ++i) {
+                if (j + i >= a.chunks) break;
+                whole += (double)x[i].sum * (double)weight_f32(x[i].max, top, f);
+                if (arg < 0 && x[i].max == top) arg = x[i].arg;
             }
+        }
     }
     const int tok = live ? a.tokens[(int64_t)b * a.n_q + c] : -1;
     int up = !live || c == 0 ? -1 : a.parents ? a.parents[(int64_t)b * a.n_q + c] : c - 1;
@@ -224,7 +242,7 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
     if (known) {
         const double x = element<WIDE>(a.logits + b * a.l_nb2 + up * a.l_nb1, tok);
         p = weight_f64(x, p_top, cool) / p_whole;
-        lp = (x == (double)p_top ? 0.0 : (x - (double)p_top) * cool) - log(p_whole);
+        if (write && a.logp) lp = (x == (double)p_top ? 0.0 : (x - (double)p_top) * cool) - log(p_whole);
     }
     // earlier children of the same token: whether one has the same token; the mass of the others
     bool twice = false;
@@ -374,11 +392,13 @@ __global__ __launch_bounds__(kSumThreads) void verify_pick_kernel(VerifyArgs a) 
     __shared__ uint32_t hit[kVChunk / 32];
     __shared__ double scan[kSumThreads / 64];
     __shared__ int pick, last;
+    __shared__ double log_sum;
     const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
     Walk w = a.walk[b];
-    if (w.at < 0) return;
+    const float uf = a.uniform[(int64_t)b * (a.n_q + 1) + a.n_q];
     const double* const all = a.sums + (int64_t)b * a.chunks;
     const double* left = all + (int64_t)a.B * a.chunks;
+    if (w.at < 0) return;
     const double sum = ordered_sum(all, a.chunks);
     double whole = ordered_sum(left, a.chunks);
     const uint8_t* row = a.logits + b * a.l_nb2 + w.at * a.l_nb1;
@@ -389,7 +409,6 @@ __global__ __launch_bounds__(kSumThreads) void verify_pick_kernel(VerifyArgs a) 
         q = nullptr;
         w.kids = 0;
     }
-    const float uf = a.uniform[(int64_t)b * (a.n_q + 1) + a.n_q];
     const double aim = (uf > 0.0f ? (double)uf : 0.0) * whole;
     // the first chunk whose running sum exceeds the aim, else the last one with a mass
     int chunk = 0;
@@ -408,15 +427,16 @@ __global__ __launch_bounds__(kSumThreads) void verify_pick_kernel(VerifyArgs a) 
         }
     }
     const int v0 = chunk * kVChunk;
-    mark_kids(a, w, b, v0, hit);
-    if (tid == 0) {
-        pick = 0x7fffffff;
-        last = -1;
-    }
     constexpr int E = kSumEach;
     float x[E], y[E];
     eight<WIDE>(row, v0 + tid * E, a.V, x);
     if (q) eight<WIDE>(q, v0 + tid * E, a.V, y);
+    if (tid == 0) {
+        pick = 0x7fffffff;
+        last = -1;
+    }
+    if (wave_id() == kSumThreads / 64 - 1 && a.logp) log_sum = log(sum);  // (while the row comes)
+    mark_kids(a, w, b, v0, hit);
     double r[E], mine = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -448,12 +468,16 @@ __global__ __launch_bounds__(kSumThreads) void verify_pick_kernel(VerifyArgs a) 
     if (found != 0x7fffffff) atomicMin(&pick, found);
     if (any >= 0) atomicMax(&last, any);
     __syncthreads();
-    if (tid == 0) {
-        const int v = pick != 0x7fffffff ? pick : last;  // (the whole sum rounded up: the last one)
+    const int v = pick != 0x7fffffff ? pick : last;  // (the whole sum rounded up: the last one)
+    if (tid == (v >= 0 ? (v - v0) / E : 0)) {
         a.next[b] = v;
         if (a.logp) {
-            const double x = v >= 0 ? (double)element<WIDE>(row, v) : -INFINITY;
-            a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((x == w.max ? 0.0 : (x - w.max) * w.cool) - log(sum));
+            float l = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (v == v0 + tid * E + e) l = x[e];
+            const double d = l;
+            a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((d == w.max ? 0.0 : (d - w.max) * w.cool) - log_sum);
         }
     }
 }
