@@ -763,18 +763,21 @@ static ChunkPlan chunk_plan(const xq_tensor* q, const xq_kv_pages* c) {
     // (decode of 16 chats of fp8 rows 37 us, with three waves idle 45), up to 64 pairs a wave for each 16; above, eight waves
     // with all pairs that the registers hold (32 each of D 128, 16 of 256), for a tile staged is then used most.
     P.form = pairs <= 16 ? 0 : pairs <= 32 ? 1 : pairs <= 64 ? 2 : 3;
-    P.pw = P.form < 3 ? 16 << P.form : D == 128 ? 256 : 128;
+    const int64_t segs = B * Hkv, tiles = cdiv((int64_t)c->table_cols * c->k.ne[1], 64);
+    const auto pw = [&](int form) { return form < 3 ? 16 << form : D == 128 ? 256 : 128; };
+    // Smaller ones where parts of a tile each would not be one for each CU (us by this rule and without: 17 f32 tokens on 500 q8_0
+    // rows of 256 18.7 and 20.6; 200 bf16 tokens alone, f16 rows of 128, 14.1 and 18.3; 64 on 2000 f16 rows 18.5 and 18.7).
+    while (P.form > 0 && segs * cdiv(pairs, pw(P.form)) * tiles < 256) --P.form;
+    P.pw = pw(P.form);
     P.ptiles = (int32_t)cdiv(pairs, P.pw);
-    const int64_t segs = B * Hkv, base = segs * P.ptiles;
-    int64_t limit = (int64_t)c->table_cols * c->k.ne[1];
+    const int64_t base = segs * P.ptiles;
     // A part costs its workgroup a start and a state written (131 KB of 256 pairs of 128): one part for each CU (512 tokens on
     // 4096 rows: 68 us, with two 81), of a tile at least.
-    const int64_t tiles = cdiv(limit, 64);
     int64_t splits = cdiv(256, base);
     if (splits > tiles) splits = tiles;
     if (splits > 64) splits = 64;
     P.splits = (int32_t)(splits < 1 ? 1 : splits);
-    if (P.form < 3) {
+    if (P.form < 3 && P.ptiles == 1) {
         // two workgroups for each CU; one of 140 KB of LDS (f32 beside quantized rows of 256)
         const bool big = D == 256 && q->type == XQ_TYPE_F32 && (c->k.type == XQ_TYPE_Q8_0 || c->k.type == XQ_TYPE_Q4_0);
         const int64_t target = big ? 256 : 512;
