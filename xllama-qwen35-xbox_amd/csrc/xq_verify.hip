@@ -49,6 +49,7 @@ struct VerifyArgs {
     RowStat* stats;  // [sequence][token][chunk]
     Walk* walk;      // [sequence]
     double* sums;    // [2][sequence][chunk]: of p's weights; of what is left
+    double* parts;   // [2][sequence][chunk][kVParts]: the same
 
     XQ_DEV int tokens_of(int b) const { return n_tok ? min(max(n_tok[b], 0), n_q) : n_q; }
     // the temperature of a sequence; 0: greedy. (Any above 1e30 leaves all finite logits the same mass.)
@@ -176,16 +177,19 @@ XQ_DEV double lane_f64(double x, int l) {
 
 constexpr int kSumThreads = 1024, kSumEach = kVChunk / kSumThreads;
 
-// Sum over the workgroup's threads, the same in all; the order is fixed.
-XQ_DEV double block_sum(double x, double* lds) {
+constexpr int kVParts = kSumThreads / 64, kVPart = kVChunk / kVParts;  // a chunk's parts are its waves' elements
+
+// Sum over the workgroup's threads, the same in all; the order is fixed. Each wave's own goes to parts[wave] too.
+XQ_DEV double block_sum(double x, double* lds, double* parts) {
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) x += shfl_f64(x, lane_id() ^ s);
     __syncthreads();
     if (lane_id() == 0) lds[wave_id()] = x;
+    if (lane_id() == 0 && parts) parts[wave_id()] = x;
     __syncthreads();
     x = 0.0;
 #pragma unroll
-    for (int i = 0; i < kSumThreads / 64; ++i) x += lds[i];
+    for (int i = 0; i < kVParts; ++i) x += lds[i];
     return x;
 }
 // Elements v .. v + 7 of a row.
@@ -326,13 +330,14 @@ XQ_DEV double ordered_sum(const double* x, int n) {
     return s;
 }
 
-// The tokens of `kids` in the chunk from v0 on, as bits.
-XQ_DEV void mark_kids(const VerifyArgs& a, const Walk& w, int b, int v0, uint32_t* hit) {
-    for (int i = threadIdx.x; i < kVChunk / 32; i += blockDim.x) hit[i] = 0;
+// The tokens (`tok`, of thread i's child i) of `kids` among the N elements from v0 on, as bits.
+template <int N>
+XQ_DEV void mark_kids(uint64_t kids, int tok, int v0, uint32_t* hit) {
+    for (int i = threadIdx.x; i < N / 32; i += blockDim.x) hit[i] = 0;
     __syncthreads();
-    if (threadIdx.x < 64 && (w.kids >> threadIdx.x & 1)) {
-        const int64_t t = (int64_t)a.tokens[(int64_t)b * a.n_q + threadIdx.x] - v0;
-        if (t >= 0 && t < kVChunk) atomicOr(&hit[t >> 5], 1u << (t & 31));
+    if (threadIdx.x < 64 && (kids >> threadIdx.x & 1)) {
+        const int64_t t = (int64_t)tok - v0;
+        if (t >= 0 && t < N) atomicOr(&hit[t >> 5], 1u << (t & 31));
     }
     __syncthreads();
 }
@@ -366,7 +371,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sums_kernel(VerifyArgs a) 
     float x[kSumEach], y[kSumEach];
     eight<WIDE>(row, v, a.V, x);
     if constexpr (PART == 1) eight<WIDE>(q, v, a.V, y);
-    else mark_kids(a, w, b, v0, hit);
+    else mark_kids<kVChunk>(w.kids, tid < a.n_q ? a.tokens[(int64_t)b * a.n_q + tid] : -1, v0, hit);
     double all = 0.0, left = 0.0;
 #pragma unroll
     for (int i = 0; i < kSumEach; ++i) {
@@ -378,107 +383,105 @@ __global__ __launch_bounds__(kSumThreads) void verify_sums_kernel(VerifyArgs a) 
             left += fmax(p / sum - (double)fmaxf(y[i], 0.0f), 0.0);
         }
     }
-    all = block_sum(all, lds);
-    left = block_sum(left, lds);
-    if (tid == 0) {
-        if constexpr (PART == 0) a.sums[(int64_t)b * a.chunks + j] = all;
-        if (PART == 1 || !q) a.sums[((int64_t)a.B + b) * a.chunks + j] = left;
+    const int64_t of_p = (int64_t)b * a.chunks + j, of_rest = ((int64_t)a.B + b) * a.chunks + j;
+    if constexpr (PART == 0) {
+        all = block_sum(all, lds, a.parts + of_p * kVParts);
+        if (tid == 0) a.sums[of_p] = all;
+    }
+    if (PART == 1 || !q) {
+        left = block_sum(left, lds, a.parts + of_rest * kVParts);
+        if (tid == 0) a.sums[of_rest] = left;
     }
 }
 
-// The next token: its chunk by the chunks' sums, then its place in the chunk.
+// The next token, by one wave: its chunk by the chunks' sums, its part by the parts', then its place in the part.
 template <bool WIDE>
-__global__ __launch_bounds__(kSumThreads) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ uint32_t hit[kVChunk / 32];
-    __shared__ double scan[kSumThreads / 64];
-    __shared__ int pick, last;
-    __shared__ double log_sum;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = lane_id();
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+    constexpr int E = kVPart / 64;
+    __shared__ uint32_t hit[kVPart / 32];
+    const int b = blockIdx.x, lane = lane_id();
     Walk w = a.walk[b];
     const float uf = a.uniform[(int64_t)b * (a.n_q + 1) + a.n_q];
-    const double* const all = a.sums + (int64_t)b * a.chunks;
-    const double* left = all + (int64_t)a.B * a.chunks;
+    const int tok = lane < a.n_q ? a.tokens[(int64_t)b * a.n_q + lane] : -1;
+    int64_t at = (int64_t)b * a.chunks;
+    const double sum = ordered_sum(a.sums + at, a.chunks);
     if (w.at < 0) return;
-    const double sum = ordered_sum(all, a.chunks);
-    double whole = ordered_sum(left, a.chunks);
+    double whole = ordered_sum(a.sums + (int64_t)a.B * a.chunks + at, a.chunks);
     const uint8_t* row = a.logits + b * a.l_nb2 + w.at * a.l_nb1;
     const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
-    if (!(whole > 0.0)) {  // nothing is left: the target's distribution
-        left = all;
+    if (whole > 0.0) {
+        at += (int64_t)a.B * a.chunks;
+    } else {  // nothing is left: the target's distribution
         whole = sum;
         q = nullptr;
         w.kids = 0;
     }
     const double aim = (uf > 0.0f ? (double)uf : 0.0) * whole;
-    // the first chunk whose running sum exceeds the aim, else the last one with a mass
-    int chunk = 0;
-    double base = 0.0, run = 0.0;
-    bool got = false;
-    for (int j0 = 0; j0 < a.chunks && !got; j0 += 64) {
-        const double mine = j0 + lane < a.chunks ? left[j0 + lane] : 0.0;
-        for (int j = 0; j < min(64, a.chunks - j0) && !got; ++j) {
-            const double y = lane_f64(mine, j);
-            if (y > 0.0) {
-                chunk = j0 + j;
-                base = run;
-                got = run + y > aim;
+    // the first of n numbers whose running sum exceeds the aim, else the last one with a mass; `run`: the sum before it
+    double run = 0.0;
+    auto reach = [&](const double* x, int n) {
+        int found = 0;
+        double next = run, before = run;
+        bool got = false;
+        for (int j0 = 0; j0 < n && !got; j0 += 64) {
+            const double mine = j0 + lane < n ? x[j0 + lane] : 0.0;
+            for (int j = 0; j < min(64, n - j0) && !got; ++j) {
+                const double y = lane_f64(mine, j);
+                if (y > 0.0) {
+                    found = j0 + j;
+                    before = next;
+                    got = next + y > aim;
+                }
+                next += y;
             }
-            run += y;
         }
-    }
-    const int v0 = chunk * kVChunk;
-    constexpr int E = kSumEach;
+        run = before;
+        return found;
+    };
+    const int chunk = reach(a.sums + at, a.chunks);
+    const int part = reach(a.parts + (at + chunk) * kVParts, kVParts);
+    const int v0 = chunk * kVChunk + part * kVPart, v = v0 + lane * E;
     float x[E], y[E];
-    eight<WIDE>(row, v0 + tid * E, a.V, x);
-    if (q) eight<WIDE>(q, v0 + tid * E, a.V, y);
-    if (tid == 0) {
-        pick = 0x7fffffff;
-        last = -1;
-    }
-    if (wave_id() == kSumThreads / 64 - 1 && a.logp) log_sum = log(sum);  // (while the row comes)
-    mark_kids(a, w, b, v0, hit);
+    eight<WIDE>(row, v, a.V, x);
+    if (q) eight<WIDE>(q, v, a.V, y);
+    const double log_sum = a.logp ? log(sum) : 0.0;  // (while the row comes)
+    mark_kids<kVPart>(w.kids, tok, v0, hit);
     double r[E], mine = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const double p = weight_f64(x[e], w.max, w.cool);
-        r[e] = q ? (v0 + tid * E + e < a.V ? fmax(p / sum - (double)fmaxf(y[e], 0.0f), 0.0) : 0.0) : kept(hit, tid * E + e) ? p : 0.0;
+        r[e] = q ? (v + e < a.V ? fmax(p / sum - (double)fmaxf(y[e], 0.0f), 0.0) : 0.0) : kept(hit, lane * E + e) ? p : 0.0;
         mine += r[e];
     }
     double upto = mine;
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) {
-        const double y = shfl_f64(upto, lane >= s ? lane - s : lane);
-        if (lane >= s) upto += y;
+        const double z = shfl_f64(upto, lane >= s ? lane - s : lane);
+        if (lane >= s) upto += z;
     }
-    if (lane == 63) scan[wave_id()] = upto;
-    __syncthreads();
-    double at = base;
-#pragma unroll
-    for (int i = 0; i < kSumThreads / 64; ++i) at += i < wave_id() ? scan[i] : 0.0;
-    at += upto - mine;
-    int found = 0x7fffffff, any = -1;
+    run += upto - mine;
+    int found = -1, any = -1;  // the lane's first element beyond the aim, its last one with a mass
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        at += r[e];
+        run += r[e];
         if (r[e] > 0.0) {
-            any = v0 + tid * E + e;
-            if (at > aim) found = min(found, any);
+            any = e;
+            if (found < 0 && run > aim) found = e;
         }
     }
-    if (found != 0x7fffffff) atomicMin(&pick, found);
-    if (any >= 0) atomicMax(&last, any);
-    __syncthreads();
-    const int v = pick != 0x7fffffff ? pick : last;  // (the whole sum rounded up: the last one)
-    if (tid == (v >= 0 ? (v - v0) / E : 0)) {
-        a.next[b] = v;
-        if (a.logp) {
-            float l = -INFINITY;
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(found >= 0), massy = __builtin_amdgcn_ballot_w64(any >= 0);
+    // (where the sums were rounded up: the last one)
+    const int who = beyond ? __builtin_ctzll(beyond) : massy ? 63 - __builtin_clzll(massy) : 0;
+    if (lane != who) return;
+    const int e = beyond ? found : any;
+    a.next[b] = e < 0 ? -1 : v + e;
+    if (a.logp) {
+        float l = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (v == v0 + tid * E + e) l = x[e];
-            const double d = l;
-            a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((d == w.max ? 0.0 : (d - w.max) * w.cool) - log_sum);
-        }
+        for (int i = 0; i < E; ++i)
+            if (i == e) l = x[i];
+        const double d = l;
+        a.logp[(int64_t)b * (a.n_q + 1) + a.n_q] = (float)((d == w.max ? 0.0 : (d - w.max) * w.cool) - log_sum);
     }
 }
 
@@ -503,7 +506,7 @@ static size_t verify_space(const xq_tensor* l, size_t* walk_at, size_t* sums_at)
     const size_t chunks = (size_t)cdiv(l->ne[0], kVChunk), B = (size_t)l->ne[2];
     *walk_at = B * (size_t)l->ne[1] * chunks * sizeof(RowStat);
     *sums_at = *walk_at + B * sizeof(Walk);
-    return *sums_at + 2 * B * chunks * 8;
+    return *sums_at + 2 * B * chunks * (1 + kVParts) * 8;
 }
 
 template <bool WIDE>
@@ -513,7 +516,7 @@ static void verify_launch(const VerifyArgs& a, hipStream_t s) {
     launch("verify_sums", verify_sums_kernel<WIDE, 0>, dim3(a.uniform ? (uint32_t)a.chunks : 1u, (uint32_t)a.B), dim3(kSumThreads), s, a);
     if (!a.uniform) return;
     if (a.draft) launch("verify_left", verify_sums_kernel<WIDE, 1>, dim3((uint32_t)a.chunks, (uint32_t)a.B), dim3(kSumThreads), s, a);
-    launch("verify_pick", verify_pick_kernel<WIDE>, dim3((uint32_t)a.B), dim3(kSumThreads), s, a);
+    launch("verify_pick", verify_pick_kernel<WIDE>, dim3((uint32_t)a.B), dim3(64), s, a);
 }
 
 }  // namespace xq
@@ -566,6 +569,7 @@ xq_status xq_verify_tokens(const xq_tensor* logits, const xq_tensor* draft, cons
     a.stats = (RowStat*)workspace;
     a.walk = (Walk*)((uint8_t*)workspace + walk_at);
     a.sums = (double*)((uint8_t*)workspace + sums_at);
+    a.parts = a.sums + 2 * (size_t)a.B * (size_t)a.chunks;
     hipStream_t s = (hipStream_t)stream;
     logits->type == XQ_TYPE_F32 ? verify_launch<true>(a, s) : verify_launch<false>(a, s);
     const hipError_t e = hipGetLastError();
