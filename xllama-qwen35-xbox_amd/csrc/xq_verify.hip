@@ -45,11 +45,11 @@ struct VerifyArgs {
     const float *temperature, *uniform;
     int32_t *path, *n_path, *next;
     float* logp;
-    int32_t V, n_q, B, chunks;
+    int32_t V, n_q, B, chunks, sum_chunks;
     RowStat* stats;  // [sequence][token][chunk]
     Walk* walk;      // [sequence]
-    double* sums;    // [2][sequence][chunk]: of p's weights; of what is left
-    double* parts;   // [2][sequence][chunk][kVParts]: the same
+    double* sums;    // [2][sequence][sum chunk]: of p's weights; of what is left
+    double* parts;   // [2][sequence][sum chunk][kVParts]: the same
 
     XQ_DEV int tokens_of(int b) const { return n_tok ? min(max(n_tok[b], 0), n_q) : n_q; }
     // the temperature of a sequence; 0: greedy. (Any above 1e30 leaves all finite logits the same mass.)
@@ -175,9 +175,11 @@ XQ_DEV double lane_f64(double x, int l) {
     return __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)u, l));
 }
 
-constexpr int kSumThreads = 1024, kSumEach = kVChunk / kSumThreads;
+// The sums of the drawn row: a workgroup has 2048 elements, a wave 512. (f64 is what they cost: 16 waves of a workgroup
+// on one CU take longer than four on each of four.)
+constexpr int kSumThreads = 256, kSumEach = 8, kVSum = kSumThreads * kSumEach;
 
-constexpr int kVParts = kSumThreads / 64, kVPart = kVChunk / kVParts;  // a chunk's parts are its waves' elements
+constexpr int kVParts = kSumThreads / 64, kVPart = kVSum / kVParts;  // a workgroup's parts are its waves' elements
 
 // Sum over the workgroup's threads, the same in all; the order is fixed. Each wave's own goes to parts[wave] too.
 XQ_DEV double block_sum(double x, double* lds, double* parts) {
@@ -320,14 +322,22 @@ XQ_DEV Walk walk_path(const VerifyArgs& a, int b, bool write) {
 // Whether element i of the chunk is none of the rejected tokens.
 XQ_DEV bool kept(const uint32_t* hit, int i) { return !(hit[i >> 5] >> (i & 31) & 1u); }
 
-// The sum of n numbers one after another, 64 loaded at a time (every lane gets it).
-XQ_DEV double ordered_sum(const double* x, int n) {
+// The sum of n numbers, the same in all lanes; the order is fixed.
+XQ_DEV double wave_total(const double* x, int n) {
     double s = 0.0;
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        const double mine = i0 + lane_id() < n ? x[i0 + lane_id()] : 0.0;
-        for (int i = 0; i < min(64, n - i0); ++i) s += lane_f64(mine, i);
-    }
+    for (int i = lane_id(); i < n; i += 64) s += x[i];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) s += shfl_f64(s, lane_id() ^ d);
     return s;
+}
+// Sums of this lane's and all lower lanes' numbers.
+XQ_DEV double wave_upto(double x) {
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+        const double y = shfl_f64(x, lane_id() >= s ? lane_id() - s : lane_id());
+        if (lane_id() >= s) x += y;
+    }
+    return x;
 }
 
 // The tokens (`tok`, of thread i's child i) of `kids` among the N elements from v0 on, as bits.
@@ -347,9 +357,9 @@ XQ_DEV void mark_kids(uint64_t kids, int tok, int v0, uint32_t* hit) {
 template <bool WIDE, int PART>
 __global__ __launch_bounds__(kSumThreads) void verify_sums_kernel(VerifyArgs a) {
     __shared__ Walk shared;
-    __shared__ double lds[kSumThreads / 64];
-    __shared__ uint32_t hit[kVChunk / 32];
-    const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, v0 = j * kVChunk;
+    __shared__ double lds[kVParts];
+    __shared__ uint32_t hit[kVSum / 32];
+    const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, v0 = j * kVSum;
     if constexpr (PART == 0) {
         if (wave_id() == 0) {
             const Walk w = walk_path<WIDE>(a, b, j == 0);
@@ -366,12 +376,12 @@ __global__ __launch_bounds__(kSumThreads) void verify_sums_kernel(VerifyArgs a) 
     const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
     if (PART == 1 && !q) return;
     double sum = 0.0;
-    if constexpr (PART == 1) sum = ordered_sum(a.sums + (int64_t)b * a.chunks, a.chunks);
+    if constexpr (PART == 1) sum = wave_total(a.sums + (int64_t)b * a.sum_chunks, a.sum_chunks);
     const int v = v0 + tid * kSumEach;
     float x[kSumEach], y[kSumEach];
     eight<WIDE>(row, v, a.V, x);
     if constexpr (PART == 1) eight<WIDE>(q, v, a.V, y);
-    else mark_kids<kVChunk>(w.kids, tid < a.n_q ? a.tokens[(int64_t)b * a.n_q + tid] : -1, v0, hit);
+    else mark_kids<kVSum>(w.kids, tid < a.n_q ? a.tokens[(int64_t)b * a.n_q + tid] : -1, v0, hit);
     double all = 0.0, left = 0.0;
 #pragma unroll
     for (int i = 0; i < kSumEach; ++i) {
@@ -383,7 +393,7 @@ __global__ __launch_bounds__(kSumThreads) void verify_sums_kernel(VerifyArgs a) 
             left += fmax(p / sum - (double)fmaxf(y[i], 0.0f), 0.0);
         }
     }
-    const int64_t of_p = (int64_t)b * a.chunks + j, of_rest = ((int64_t)a.B + b) * a.chunks + j;
+    const int64_t of_p = (int64_t)b * a.sum_chunks + j, of_rest = ((int64_t)a.B + b) * a.sum_chunks + j;
     if constexpr (PART == 0) {
         all = block_sum(all, lds, a.parts + of_p * kVParts);
         if (tid == 0) a.sums[of_p] = all;
@@ -403,14 +413,15 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
     Walk w = a.walk[b];
     const float uf = a.uniform[(int64_t)b * (a.n_q + 1) + a.n_q];
     const int tok = lane < a.n_q ? a.tokens[(int64_t)b * a.n_q + lane] : -1;
-    int64_t at = (int64_t)b * a.chunks;
-    const double sum = ordered_sum(a.sums + at, a.chunks);
+    int64_t at = (int64_t)b * a.sum_chunks;
+    const int64_t rest = (int64_t)a.B * a.sum_chunks;
+    const double sum = wave_total(a.sums + at, a.sum_chunks);
     if (w.at < 0) return;
-    double whole = ordered_sum(a.sums + (int64_t)a.B * a.chunks + at, a.chunks);
+    double whole = wave_total(a.sums + rest + at, a.sum_chunks);
     const uint8_t* row = a.logits + b * a.l_nb2 + w.at * a.l_nb1;
     const uint8_t* q = a.draft && w.kids ? a.draft + b * a.q_nb2 + w.at * a.q_nb1 : nullptr;
     if (whole > 0.0) {
-        at += (int64_t)a.B * a.chunks;
+        at += rest;
     } else {  // nothing is left: the target's distribution
         whole = sum;
         q = nullptr;
@@ -421,26 +432,23 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
     double run = 0.0;
     auto reach = [&](const double* x, int n) {
         int found = 0;
-        double next = run, before = run;
-        bool got = false;
-        for (int j0 = 0; j0 < n && !got; j0 += 64) {
-            const double mine = j0 + lane < n ? x[j0 + lane] : 0.0;
-            for (int j = 0; j < min(64, n - j0) && !got; ++j) {
-                const double y = lane_f64(mine, j);
-                if (y > 0.0) {
-                    found = j0 + j;
-                    before = next;
-                    got = next + y > aim;
-                }
-                next += y;
+        double next = run;
+        for (int j0 = 0; j0 < n; j0 += 64) {
+            const double mine = j0 + lane < n ? x[j0 + lane] : 0.0, upto = next + wave_upto(mine);
+            const uint64_t massy = __builtin_amdgcn_ballot_w64(mine > 0.0), beyond = __builtin_amdgcn_ballot_w64(mine > 0.0 && upto > aim);
+            if (massy) {
+                const int l = beyond ? __builtin_ctzll(beyond) : 63 - __builtin_clzll(massy);
+                found = j0 + l;
+                run = l ? lane_f64(upto, l - 1) : next;
             }
+            if (beyond) break;
+            next = lane_f64(upto, 63);
         }
-        run = before;
         return found;
     };
-    const int chunk = reach(a.sums + at, a.chunks);
+    const int chunk = reach(a.sums + at, a.sum_chunks);
     const int part = reach(a.parts + (at + chunk) * kVParts, kVParts);
-    const int v0 = chunk * kVChunk + part * kVPart, v = v0 + lane * E;
+    const int v0 = chunk * kVSum + part * kVPart, v = v0 + lane * E;
     float x[E], y[E];
     eight<WIDE>(row, v, a.V, x);
     if (q) eight<WIDE>(q, v, a.V, y);
@@ -453,13 +461,7 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
         r[e] = q ? (v + e < a.V ? fmax(p / sum - (double)fmaxf(y[e], 0.0f), 0.0) : 0.0) : kept(hit, lane * E + e) ? p : 0.0;
         mine += r[e];
     }
-    double upto = mine;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-        const double z = shfl_f64(upto, lane >= s ? lane - s : lane);
-        if (lane >= s) upto += z;
-    }
-    run += upto - mine;
+    run += wave_upto(mine) - mine;
     int found = -1, any = -1;  // the lane's first element beyond the aim, its last one with a mass
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -503,19 +505,19 @@ static xq_status verify_check(const xq_tensor* logits, const char* what) {
 }
 
 static size_t verify_space(const xq_tensor* l, size_t* walk_at, size_t* sums_at) {
-    const size_t chunks = (size_t)cdiv(l->ne[0], kVChunk), B = (size_t)l->ne[2];
+    const size_t chunks = (size_t)cdiv(l->ne[0], kVChunk), sums = (size_t)cdiv(l->ne[0], kVSum), B = (size_t)l->ne[2];
     *walk_at = B * (size_t)l->ne[1] * chunks * sizeof(RowStat);
     *sums_at = *walk_at + B * sizeof(Walk);
-    return *sums_at + 2 * B * chunks * (1 + kVParts) * 8;
+    return *sums_at + 2 * B * sums * (1 + kVParts) * 8;
 }
 
 template <bool WIDE>
 static void verify_launch(const VerifyArgs& a, hipStream_t s) {
     launch("verify_stats", verify_stats_kernel<WIDE>, dim3((uint32_t)a.chunks, (uint32_t)a.n_q, (uint32_t)a.B), dim3(256), s, a);
     // (all greedy: the path and the maxima are the whole answer)
-    launch("verify_sums", verify_sums_kernel<WIDE, 0>, dim3(a.uniform ? (uint32_t)a.chunks : 1u, (uint32_t)a.B), dim3(kSumThreads), s, a);
+    launch("verify_sums", verify_sums_kernel<WIDE, 0>, dim3(a.uniform ? (uint32_t)a.sum_chunks : 1u, (uint32_t)a.B), dim3(kSumThreads), s, a);
     if (!a.uniform) return;
-    if (a.draft) launch("verify_left", verify_sums_kernel<WIDE, 1>, dim3((uint32_t)a.chunks, (uint32_t)a.B), dim3(kSumThreads), s, a);
+    if (a.draft) launch("verify_left", verify_sums_kernel<WIDE, 1>, dim3((uint32_t)a.sum_chunks, (uint32_t)a.B), dim3(kSumThreads), s, a);
     launch("verify_pick", verify_pick_kernel<WIDE>, dim3((uint32_t)a.B), dim3(64), s, a);
 }
 
@@ -565,11 +567,11 @@ xq_status xq_verify_tokens(const xq_tensor* logits, const xq_tensor* draft, cons
     a.tokens = tokens, a.parents = parents, a.n_tok = n_tok, a.temperature = temperature, a.uniform = uniform;
     a.path = path, a.n_path = n_path, a.next = next, a.logp = logp;
     a.V = (int32_t)logits->ne[0], a.n_q = (int32_t)logits->ne[1], a.B = (int32_t)logits->ne[2];
-    a.chunks = (int32_t)cdiv(a.V, kVChunk);
+    a.chunks = (int32_t)cdiv(a.V, kVChunk), a.sum_chunks = (int32_t)cdiv(a.V, kVSum);
     a.stats = (RowStat*)workspace;
     a.walk = (Walk*)((uint8_t*)workspace + walk_at);
     a.sums = (double*)((uint8_t*)workspace + sums_at);
-    a.parts = a.sums + 2 * (size_t)a.B * (size_t)a.chunks;
+    a.parts = a.sums + 2 * (size_t)a.B * (size_t)a.sum_chunks;
     hipStream_t s = (hipStream_t)stream;
     logits->type == XQ_TYPE_F32 ? verify_launch<true>(a, s) : verify_launch<false>(a, s);
     const hipError_t e = hipGetLastError();
