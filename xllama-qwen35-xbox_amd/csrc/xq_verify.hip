@@ -14,9 +14,10 @@
 // f32 exponentials (each off by 2^-22 of itself, the sum by less) joined in f64.
 //
 // What bounds it: the one pass over the logits (16 x 16 rows of 128000 f32, 131 MB: 24 us, 5.5 TB/s, some of it from the
-// Infinity Cache), then two launches of one row per sequence, 12 and 16 us, each a chain of dependent reads
-// (statistics, path, row) before f64 arithmetic on one or a few CUs. Loops in place of unrolled f64 code, a third of
-// its size, did not change that; a sum of the drawn row in the first launch would form all rows' f64 sums.
+// Infinity Cache), then two launches of one row per sequence, 12 and 6 us, each a chain of dependent reads
+// (statistics, path, row; sums, part, row) before its f64 arithmetic. The drawn token's place by a workgroup of 16 waves took
+// 17 us, with sums kept for every 512 elements one wave has it. Loops in place of unrolled f64 code, a third of
+// its size, changed nothing; the drawn row's sums in the first launch would have to be formed of all rows.
 #include "xq_tile.h"
 
 namespace xq {
