@@ -8,9 +8,10 @@
 // of (page, row) pairs; a second launch moves them in every pool and gives pages without rows back.
 //
 // What bounds it: the moves by their bytes, read and written (4 x 12001 rows cut to 4096 in 16 f16 pools, 0.7 GB: 151 us,
-// 4.7 TB/s); the selection by its chain of passes on one CU per sequence (39 us of 12001 rows, 16 us of 2049;
+// 4.7 TB/s); the selection by its chain of passes on one CU per sequence (33 us of 12001 rows, 15 us of 2049;
 // each pass 2 to 4 us, LDS and barriers), which only grows with a sequence's rows, not with the batch.
 #include "xq_pools.h"
+#include "xq_tile.h"
 
 namespace xq {
 
@@ -57,6 +58,11 @@ XQ_DEV uint32_t before_wave(uint32_t mine, uint32_t* lds, uint32_t* total) {
     *total = all;
     return before;
 }
+
+// The lowest c bits.
+XQ_DEV uint64_t low_bits(int c) { return c <= 0 ? 0ull : c >= 64 ? ~0ull : ((uint64_t)1 << c) - 1; }
+// x of lane l, the same for all
+XQ_DEV uint64_t lane_get64(uint64_t x, int l) { return ((uint64_t)lane_get((uint32_t)(x >> 32), l) << 32) | lane_get((uint32_t)x, l); }
 
 // The keys of up to kHeldRows rows stay in LDS, and so do the lists of their moves: a pass over them costs no
 // memory round trip (about 1 us each, of a lone workgroup). Longer sequences read them again in each pass.
@@ -195,36 +201,79 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictArgs a
             }
         }
         const uint32_t ties = want ? left : 0u;
-        // ranks of the ties, in the rows' order
-        mine = 0;
-        each([&](int, bool on, uint32_t x, bool s) { mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && s == among_safe && x == key)); });
-        uint32_t total, tie0 = before_wave(mine, lds, &total);
-        // f(row, a place that it leaves, whether it is to move)
-        auto sorted = [&](auto f) {
-            uint32_t tie = tie0;
-            each([&](int r, bool on, uint32_t x, bool s) {
-                const bool group = on && s == among_safe;
-                const uint64_t eq = __builtin_amdgcn_ballot_w64(group && x == key);
-                const uint32_t rank = tie + __builtin_popcountll(eq & (((uint64_t)1 << lane) - 1));
-                const bool stays = on && (group ? want && (x > key || (x == key && rank < ties)) : !among_safe && s);
-                tie += __builtin_popcountll(eq);
-                f(r, __builtin_amdgcn_ballot_w64(on && !stays && r < k), __builtin_amdgcn_ballot_w64(stays && r >= k));
-            });
-        };
-        uint32_t holes = 0, tails = 0;
-        sorted([&](int, uint64_t h, uint64_t t) {
-            holes += __builtin_popcountll(h);
-            tails += __builtin_popcountll(t);
-        });
-        uint32_t hole0 = before_wave(holes, lds, &moves), tail0 = before_wave(tails, lds, &total);
-        sorted([&](int r, uint64_t h, uint64_t t) {
+        uint32_t total;
+        if constexpr (HELD) {
+            // One more pass over the keys: lane g of a wave has its g-th 64 rows as masks, and what stays, the places
+            // left and the rows that fill them are a few operations of masks. (Passes over the rows for each of these: 12001
+            // rows 40 us; with the masks 33 us. Keys read four groups ahead changed nothing.)
+            static_assert(kHeldRows / kEvictWaves <= 64 * 64);
+            uint64_t eq = 0, gt = 0;
+            for (int g = 0; g < span / 64; ++g) {
+                const uint32_t x = keys[min(w0 + 64 * g + lane, n - 1)];
+                const uint64_t e = __builtin_amdgcn_ballot_w64(x == key), t = __builtin_amdgcn_ballot_w64(x > key);
+                if (lane == g) eq = e, gt = t;
+            }
+            const int g0 = w0 + 64 * lane;
+            const uint64_t in = lane < span / 64 ? low_bits(n - g0) : 0, safe = in ? safes[g0 / 64] & in : 0;
+            const uint64_t group = among_safe ? safe : in & ~safe;
+            eq &= group, gt &= group;
+            const uint32_t n_eq = (uint32_t)__builtin_popcountll(eq), eq_upto = wave_scan(n_eq);
+            const uint32_t tie0 = before_wave(lane_get(eq_upto, 63), lds, &total) + eq_upto - n_eq;
+            // of the ties the first ones
+            uint32_t few = ties > tie0 ? ties - tie0 : 0u;
+            if (few < n_eq) {
+                uint64_t first = 0;
+                for (; few; --few) {
+                    first |= eq & (~eq + 1);
+                    eq &= eq - 1;
+                }
+                eq = first;
+            }
+            const uint64_t stays = (want ? eq | gt : 0ull) | (among_safe ? 0ull : safe), front = low_bits(k - g0);
+            const uint64_t hole = in & ~stays & front, tail = stays & ~front;
+            const uint32_t holes = (uint32_t)__builtin_popcountll(hole), tails = (uint32_t)__builtin_popcountll(tail);
+            const uint32_t h_upto = wave_scan(holes), t_upto = wave_scan(tails);
+            const uint32_t h0 = before_wave(lane_get(h_upto, 63), lds, &moves) + h_upto - holes;
+            const uint32_t t0 = before_wave(lane_get(t_upto, 63), lds, &total) + t_upto - tails;
             const uint64_t below = ((uint64_t)1 << lane) - 1;
-            const uint32_t x = hole0 + __builtin_popcountll(h & below), y = tail0 + __builtin_popcountll(t & below);
-            if (h >> lane & 1) HELD ? (void)(list[0][x] = (uint16_t)r) : (void)(far_list[x] = r);
-            if (t >> lane & 1) HELD ? (void)(list[1][y] = (uint16_t)r) : (void)(far_list[a.half + y] = r);
-            hole0 += __builtin_popcountll(h);
-            tail0 += __builtin_popcountll(t);
-        });
+            for (int g = 0; g < span / 64; ++g) {
+                const uint64_t h = lane_get64(hole, g), t = lane_get64(tail, g);
+                const uint16_t r = (uint16_t)(w0 + 64 * g + lane);
+                if (h >> lane & 1) list[0][lane_get(h0, g) + __builtin_popcountll(h & below)] = r;
+                if (t >> lane & 1) list[1][lane_get(t0, g) + __builtin_popcountll(t & below)] = r;
+            }
+        } else {
+            // ranks of the ties, in the rows' order
+            mine = 0;
+            each([&](int, bool on, uint32_t x, bool s) { mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on && s == among_safe && x == key)); });
+            const uint32_t tie0 = before_wave(mine, lds, &total);
+            // f(row, a place that it leaves, whether it is to move)
+            auto sorted = [&](auto f) {
+                uint32_t tie = tie0;
+                each([&](int r, bool on, uint32_t x, bool s) {
+                    const bool group = on && s == among_safe;
+                    const uint64_t eq = __builtin_amdgcn_ballot_w64(group && x == key);
+                    const uint32_t rank = tie + __builtin_popcountll(eq & (((uint64_t)1 << lane) - 1));
+                    const bool stays = on && (group ? want && (x > key || (x == key && rank < ties)) : !among_safe && s);
+                    tie += __builtin_popcountll(eq);
+                    f(r, __builtin_amdgcn_ballot_w64(on && !stays && r < k), __builtin_amdgcn_ballot_w64(stays && r >= k));
+                });
+            };
+            uint32_t holes = 0, tails = 0;
+            sorted([&](int, uint64_t h, uint64_t t) {
+                holes += __builtin_popcountll(h);
+                tails += __builtin_popcountll(t);
+            });
+            uint32_t hole0 = before_wave(holes, lds, &moves), tail0 = before_wave(tails, lds, &total);
+            sorted([&](int r, uint64_t h, uint64_t t) {
+                const uint64_t below = ((uint64_t)1 << lane) - 1;
+                const uint32_t x = hole0 + __builtin_popcountll(h & below), y = tail0 + __builtin_popcountll(t & below);
+                if (h >> lane & 1) far_list[x] = r;
+                if (t >> lane & 1) far_list[a.half + y] = r;
+                hole0 += __builtin_popcountll(h);
+                tail0 += __builtin_popcountll(t);
+            });
+        }
         __syncthreads();
         // their places; a page that other sequences hold too is not written
         bool ok = true;
