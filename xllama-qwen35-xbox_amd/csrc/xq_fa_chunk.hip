@@ -383,8 +383,10 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
 
     for (uint32_t t = t_first; t < t_last; ++t) {
         const int first = (int)(t * TR);
+        // where some pair of the workgroup does not see all rows, non-finite values stay out of the image that all share
+        const bool clean = first < wg.lo_max || first + TR > wg.hi_min;
         __syncthreads();  // the image is free, the flags are zero
-        commit(t, first < wg.lo_max || first + TR > wg.hi_min);
+        commit(t, clean);
         __syncthreads();
         const uint64_t now = valid;
         if (t + 1 < t_last) {
@@ -398,7 +400,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
         // which of the tile's rows each pair sees
         const bool careful = first < wr.lo_max || first + TR > wr.hi_min || now != ~0ull;
         uint64_t sees[MT];
-        if (careful) {
+        if (careful || clean) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) sees[m] = tile_rows(first, lo[m], hi[m]) & now;
         }
@@ -564,8 +566,8 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
             }
         }
         products_done();
-        // non-finite values of rows that not every pair sees: to the pairs that do
-        if (careful) {
+        // the values that the image was cleaned of, to the pairs that see them (all of a wave's may)
+        if (clean) {
             uint64_t bad = sBad[t & 1];
             if constexpr (WR > 1) bad &= (~0ull >> (64 - C::RW)) << row_first;
             bad = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(bad >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)bad);
