@@ -452,8 +452,8 @@ xq_status xq_fa_tree(const xq_tensor* q, const xq_kv_pages* cache, const int32_t
                      xq_tensor* dst, float* lse, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* How a chunk of new tokens meets the paged cache: the scores are scale q.k, then (logit_softcap
- * above 0) logit_softcap * tanh(./logit_softcap), then (max_bias above 0) slope_h * (row - the token's
- * row), with ggml's ALiBi slopes. window above 0: a token sees its own row and the window - 1 before
+ * above 0) logit_softcap * tanh(./logit_softcap), then (max_bias above 0) less slope_h * |row - the
+ * token's row|, with ggml's ALiBi slopes. window above 0: a token sees its own row and the window - 1 before
  * it, 0: all before it. scale finite, the others finite and not negative, reserved 0. */
 typedef struct xq_chunk_params {
     float scale;

@@ -2,7 +2,7 @@
 // paged cache.
 //
 // Pair p of a KV head is (token p / G, query head p % G of the group). A token sees the rows
-// [lo, hi) (ChunkArgs::range): with x = log2(e) (f(scale q.k) + slope (r - its row)) over them, f the
+// [lo, hi) (ChunkArgs::range): with x = log2(e) (f(scale q.k) - slope |r - its row|) over them, f the
 // identity or cap tanh(./cap), and any m near their maximum,
 //   O = sum_r 2^(x_r - m) v_r / sum_r 2^(x_r - m),    lse = (m + log2 sum) / log2(e).
 // A workgroup takes PW pairs and walks the 64-row tiles that any of them sees, once: K and V as f16 images in LDS,
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
                         for (int i = 0; i < 4; ++i) {
                             float x = s[m][r][i] * qf[m];
                             if (a.cap > 0.0f) x = a.cap * capped_tanh(x * inv_cap);
-                            x = fmaf(slope[m], (float)(first + row0 + 16 * r + 4 * lg + i - at[m]), x);
+                            x = less_distance(x, slope[m], first + row0 + 16 * r + 4 * lg + i, at[m]);
                             s[m][r][i] = x * kLog2e;
                         }
             }

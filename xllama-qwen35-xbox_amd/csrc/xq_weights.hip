@@ -1,7 +1,7 @@
 // xq_weights.hip — the attention weight that each cached row gets from a chunk's tokens, accumulated.
 //
 // With the lse of every (token, head) known, a row's weight is a plain sum,
-//   w_r = sum_{pairs that see r} 2^(x_r - log2(e) lse),   x_r = log2(e) (f(scale q.k_r) + slope (r - at)),
+//   w_r = sum_{pairs that see r} 2^(x_r - log2(e) lse),   x_r = log2(e) (f(scale q.k_r) - slope |r - at|),
 // and nothing of V is read. A wave has 16 or 32 rows of K of one head as matrix operands and takes the
 // head's pairs 16 at a time: the product leaves four rows of one pair in a lane, whose
 // weights add up in the lane; the 16 lanes of a row join at the end.
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(WeightsArgs a) {
                 if constexpr (BIASED) {
                     z *= m.factor;
                     if (a.cap > 0.0f) z = a.cap * capped_tanh(z * inv_cap);
-                    z = fmaf(m.slope, (float)(first + 16 * r + 4 * lg + i - m.at), z);
+                    z = less_distance(z, m.slope, first + 16 * r + 4 * lg + i, m.at);
                     z = fmaf(z, kLog2e, -m.lse2);
                 } else {
                     z = fmaf(z, m.factor, -m.lse2);
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256, 2) void weights_few_kernel(WeightsArgs a) {
             if constexpr (BIASED) {
                 z *= factor;
                 if (a.cap > 0.0f) z = a.cap * capped_tanh(z * inv_cap);
-                z = fmaf(slope, (float)(first + 16 * tile + 4 * lg + i - at), z);
+                z = less_distance(z, slope, first + 16 * tile + 4 * lg + i, at);
                 z = fmaf(z, kLog2e, -lse2);
             } else {
                 z = fmaf(z, factor, -lse2);
