@@ -16,7 +16,7 @@ struct ChunkArgs {
     PagesView pg;
     const int32_t *first, *prefix, *n_tok;
     int32_t n_q, H, G, B, window;
-    float scale, cap, max_bias, m0, m1;
+    float scale, cap, inv_cap, max_bias, m0, m1;
     int32_t n_head_log2;
     uint32_t k_page, k_row, v_page, v_row;  // strides, below 2^32
     UDivFlat d_g;                           // by the group
@@ -157,6 +157,8 @@ inline void chunk_fill(ChunkArgs& a, const xq_tensor* q, const xq_chunk_params* 
     a.n_q = (int32_t)q->ne[1], a.H = (int32_t)q->ne[2], a.B = (int32_t)q->ne[3];
     a.G = a.H / a.pg.n_head_kv;
     a.window = p->window, a.scale = p->scale, a.cap = p->logit_softcap, a.max_bias = p->max_bias;
+    // (finite, so that a score of 0 stays 0 under a subnormal cap; what that makes of others is below 2^-126)
+    a.inv_cap = p->logit_softcap > 0.0f ? fminf(1.0f / p->logit_softcap, 3.40282347e38f) : 0.0f;
     a.n_head_log2 = 1;
     while (2 * a.n_head_log2 <= a.H) a.n_head_log2 *= 2;
     a.m0 = powf(2.0f, -p->max_bias / (float)a.n_head_log2);

@@ -379,7 +379,6 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
 #pragma unroll
         for (int n = 0; n < ND; ++n) acc[m][n] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
 
     for (uint32_t t = t_first; t < t_last; ++t) {
         const int first = (int)(t * TR);
@@ -471,7 +470,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_chunk_kernel(FaChunkArgs a) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             float x = s[m][r][i] * qf[m];
-                            if (a.cap > 0.0f) x = a.cap * capped_tanh(x * inv_cap);
+                            if (a.cap > 0.0f) x = a.cap * capped_tanh(x * a.inv_cap);
                             x = less_distance(x, slope[m], first + row0 + 16 * r + 4 * lg + i, at[m]);
                             s[m][r][i] = x * kLog2e;
                         }

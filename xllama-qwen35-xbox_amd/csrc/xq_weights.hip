@@ -193,7 +193,6 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(WeightsArgs a) {
     f4t sum[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) sum[r] = f4t{0.0f, 0.0f, 0.0f, 0.0f};
-    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
 
     // a chunk's pairs on their way
     u4t piece[NPT], meta0, meta1;
@@ -290,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void weights_kernel(WeightsArgs a) {
                 if constexpr (QUANT) z = ldexpf(z, ek[r][i]);
                 if constexpr (BIASED) {
                     z *= m.factor;
-                    if (a.cap > 0.0f) z = a.cap * capped_tanh(z * inv_cap);
+                    if (a.cap > 0.0f) z = a.cap * capped_tanh(z * a.inv_cap);
                     z = less_distance(z, m.slope, first + 16 * r + 4 * lg + i, m.at);
                     z = fmaf(z, kLog2e, -m.lse2);
                 } else {
@@ -366,7 +365,6 @@ __global__ __launch_bounds__(256, 2) void weights_few_kernel(WeightsArgs a) {
         for (int g = 0; g < NG; ++g) raw[g].load(rec, g, lg);
     };
     if (u < u_end) fetch(u);
-    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     int hk = -1, lo = 0, hi = 0, at = 0;
     float factor = 0.0f, lse2 = 0.0f, slope = 0.0f;
     h8t q[NB][QP];
@@ -413,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void weights_few_kernel(WeightsArgs a) {
             if constexpr (QUANT) z = ldexpf(z, __shfl(e, 4 * lg + i));
             if constexpr (BIASED) {
                 z *= factor;
-                if (a.cap > 0.0f) z = a.cap * capped_tanh(z * inv_cap);
+                if (a.cap > 0.0f) z = a.cap * capped_tanh(z * a.inv_cap);
                 z = less_distance(z, slope, first + 16 * tile + 4 * lg + i, at);
                 z = fmaf(z, kLog2e, -lse2);
             } else {
