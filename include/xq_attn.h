@@ -493,11 +493,16 @@ xq_status xq_fa_chunk(const xq_tensor* q, const xq_kv_pages* cache, const xq_chu
  * layers' calls add to them: decay 1, fresh 0).
  *   q, cache, params, first, prefix, n_tok  as for xq_fa_chunk (V is not read). A view of a chunk's last
  *           tokens, with rows moved up by those left out, gives the weights of these alone
- *   lse     F32 [n_seq][n_q][n_head] (device), of xq_fa_chunk or xq_fa_tree; -inf: a token without weight
+ *   lse     F32 [n_seq][n_q][n_head] (device), of xq_fa_chunk or xq_fa_tree; -inf: a token without weight.
+ *           With a tree's (xq_fa_tree with parents) only the rows below rows[b] get the tokens' weights: a token of a tree does not
+ *           see all the rows of the tokens before it, and what is added to rows[b] and behind means nothing
  *   scores  F32 [n_seq][score_cols] (device), or NULL: zeros; scores_out the same, and may be scores
  * Scores are those of the decoded cache at 22 bits and more whatever q's type, sums in f32, in an order
- * that depends on the shapes and n_tok alone. decay finite. A table of fewer than 2^28 rows; the workspace may
- * be of 0 bytes. */
+ * that depends on the shapes and n_tok alone. (BF16 q on q8_0 / q4_0 pools: the lse is of keys d * q rounded to 11 bits,
+ * so that a token's weights are 1 in all only to 2^-11 of |q|.|k| scale.) Nothing moves scores with rows but
+ * xq_kv_pages_evict: after xq_kv_pages_compact those of the accepted rows are where the tokens were.
+ * decay finite. A table of fewer than 2^28 rows; the workspace may be of 0 bytes; calls that may run at the same
+ * time need one each. */
 xq_status xq_kv_weights_workspace(const xq_tensor* q, const xq_kv_pages* cache, size_t* bytes);
 xq_status xq_kv_weights(const xq_tensor* q, const xq_kv_pages* cache, const xq_chunk_params* params, const int32_t* first,
                         const int32_t* prefix, const int32_t* n_tok, const float* lse, const float* scores, float* scores_out,
