@@ -475,7 +475,11 @@ typedef struct xq_chunk_params {
  *           are left as they were
  *   dst     q's type [D, n_head, n_q, n_seq], strides multiples of 16 bytes; not q's memory
  *   lse     F32 [n_seq][n_q][n_head], natural logarithm of the softmax sum, or NULL
- * A token that sees no row gets O = 0, LSE = -inf. Roundings and non-finite values are xq_fa_tree's.
+ * A token that sees no row gets O = 0, LSE = -inf. Roundings and non-finite values are xq_fa_tree's. For up to 64
+ * tokens without masks xq_fa_tree gives the same, and is the one to call where the rows are many (8 sequences of up to 4096 f16
+ * rows, heads of 128: 1 to 5 tokens take the same time, 25 take 26 us there and 41 here, 64 take 37 and 54).
+ * The forms and parts go by the table's columns: a table far wider than its rows costs a chunk of up to some hundred
+ * tokens up to 8 us.
  * Refused: 2^25 query rows (n_q * n_head * n_seq) or 2^22 workgroups and more, row and page strides of the
  * pools of 2^32 bytes and more. The workspace may be of 0 bytes; calls that may run at the same time need one
  * each. */
@@ -568,7 +572,8 @@ xq_status xq_kv_pages_release(int32_t* table, int32_t* rows, int32_t* refs, int3
  * are given back (the table's entry -1, refs less 1), and a sequence of which a page to be written has refs
  * above 1 is left as it was. So is one
  * with a row to be moved from or to a page that is none, or with rows below 0, above score_cols or
- * past the table's columns. At most 65535 sequences, score_cols up to 2^30; rows_out is not rows, no pool is given twice. */
+ * past the table's columns. At most 65535 sequences, score_cols up to 2^30; rows_out is not rows, no pool is given twice.
+ * Calls that may run at the same time need a workspace each. */
 xq_status xq_kv_pages_evict_workspace(int32_t n_seq, int32_t score_cols, size_t* bytes);
 xq_status xq_kv_pages_evict(const xq_tensor* pools, int32_t n_pools, int32_t* table, const int32_t* rows, int32_t* refs,
                             int32_t n_seq, int32_t table_cols, const int32_t* keep, int32_t first_rows, int32_t last_rows,
@@ -598,7 +603,8 @@ xq_status xq_kv_pages_evict(const xq_tensor* pools, int32_t n_pools, int32_t* ta
  *           xq_kv_pages_compact takes); next I32 [n_seq]: -1 where n_tok is 0 or the row holds nothing but -inf
  *   logp    F32 [n_seq][n_q + 1], or NULL: ln p of each token with a parent after that parent, and of the next
  *           one; 0 where there is none; greedy ones at temperature 1
- * Sums of the next token's row are formed in f64. */
+ * Sums of the next token's row are formed in f64, those for the tests of f32 exponentials (a test whose
+ * sides differ by less than 2^-17 of themselves may go either way). Calls that may run at the same time need a workspace each. */
 xq_status xq_verify_tokens_workspace(const xq_tensor* logits, size_t* bytes);
 xq_status xq_verify_tokens(const xq_tensor* logits, const xq_tensor* draft, const int32_t* tokens, const int32_t* parents,
                            const int32_t* n_tok, const float* temperature, const float* uniform, int32_t* path, int32_t* n_path,

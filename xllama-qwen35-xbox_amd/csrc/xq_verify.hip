@@ -10,8 +10,9 @@
 // Whether a child would be accepted if its parent were reached does not depend on the walk: all rows'
 // maxima and sums are formed at once (one pass over the logits, bound by HBM), then one wave has
 // the path by ballots and pointer doubling, a lane a token. Only the next token needs sums that hold
-// next to a border: those of one row per sequence, in f64 throughout. A row's sum over the tests is of
-// f32 exponentials (each off by 2^-22 of itself, the sum by less) joined in f64.
+// next to a border: those of one row per sequence, in f64 throughout. A row's sum for the tests is of f32
+// exponentials joined in f64: a weight e^-d is off by up to (4 d + 2) 2^-24 of itself (the difference, two roundings of its
+// factor, their product, the exponential's step), the sum by the mean of that over its mass.
 //
 // What bounds it: the one pass over the logits (16 x 16 rows of 128000 f32, 131 MB: 24 us, 5.5 TB/s, some of it from the
 // Infinity Cache), then two launches of one row per sequence, 12 and 6 us, each a chain of dependent reads
