@@ -11,7 +11,7 @@
 // quantized values (exact integers times a scale's upper bits, and the remainder).
 //
 // What bounds it. Chunks: matrix products and vector issue, which overlap little: two prompts of 8191 bf16 tokens, f16 rows
-// of 128, 1.1 TFLOP: 1181 to 1280 us, 0.86 to 0.93 PFLOP/s of the 1.22 of a large library product; the matrix cores are busy
+// of 128, 1.1 TFLOP: 1169 to 1280 us, 0.86 to 0.94 PFLOP/s of the 1.22 of a large library product; the matrix cores are busy
 // 38 % of the time and vector issue 48 %. Without any staging or barrier it would be 1003 us, so a second image buys
 // little (32x32x16 products, two images and the stages interleaved by hand: 1187 us for 1185 of the 16x16x32
 // form as it then was). Few tokens: the rows' bytes where there are many (32 chats of up to 8000 fp8 rows 39 us, 28 at
